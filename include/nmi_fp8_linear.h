@@ -17,7 +17,8 @@
  * nmi_last_error() describes the last failure of the calling thread.
  * NMI_ERR_ASYNC reports a failure of an earlier launch on the device that the host learnt of
  * since (a stream-K GEMM that gave up waiting for a partial tile, see nmi_linear_fp8_w8a16_ws):
- * every entry point that launches a linear, a GEMM or a block returns it, launching nothing, at
+ * every entry point that launches a linear, a GEMM or a block, or works on a paged cache or packed
+ * prompts (whose kernels report device data out of range the same way), returns it, launching nothing, at
  * its first call after that launch has finished; nmi_sync after synchronising, nmi_async_status
  * without synchronising.  Each such failure is reported once.
  *
@@ -374,6 +375,98 @@ int nmi_attn_forward_fp8(const void* input_bf16, const float* norm_w, const void
                          const void* o_w_e4m3, const float* o_scale, void* out_bf16, int S, void* k_cache_bf16,
                          void* v_cache_bf16, int cache_cap, int hidden, int n_heads, int n_kv_heads, float eps,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention for many sequences at once: keys and values in the pages of a pool, every sequence its own
+ * length.  The reference serves one sequence from contiguous caches and has no counterpart.
+ *
+ * A paged KV cache: k_pages and v_pages hold n_pages pages of page_size positions of n_kv_heads head
+ * vectors of 128, as bf16 (NMI_KV_BF16) or OCP e4m3 codes (NMI_KV_E4M3, one byte) that stand for code *
+ * k_scale[head], code * v_scale[head] (float32 [n_kv_heads], positive; NULL: 1; NULL for bf16).  Head h
+ * of position p of sequence b is at element
+ *     page_table[b * page_table_stride + p / page_size] * page_stride + h * head_stride
+ *         + (p % page_size) * token_stride
+ * of either, so [n_pages, n_kv_heads, page_size, 128] and [n_pages, page_size, n_kv_heads, 128] are
+ * both possible, as are slices of a pool that several layers share.  page_size is a power of two from
+ * 16 to 2^20; page_table has max_pages entries per sequence, of which only those that a sequence's
+ * length reaches are read; max_pages * page_size <= 2^30.  Pages and strides are multiples of 16
+ * bytes, strides at least 128 elements, token_stride at most 2^24.  The struct is read during the call only.
+ *
+ * Page tables, lengths, positions and offsets are device data (so that a captured graph can be replayed
+ * as the sequences grow) and are not seen by the host.  The kernels never follow one that is out of
+ * range -- a page id outside [0, n_pages), a position or length that a row of the table does not
+ * hold, offsets that do not ascend within the rows given --: the token is not stored, or the
+ * sequence's output of that KV head is NaN, or the rows are cut to those given, and NMI_ERR_ASYNC
+ * reports it as described at the top of this file.
+ */
+enum { NMI_KV_BF16 = 0, NMI_KV_E4M3 = 1 };
+typedef struct nmi_paged_kv {
+    void* k_pages;
+    void* v_pages;
+    int64_t page_stride, head_stride, token_stride; /* elements */
+    const int32_t* page_table;
+    int64_t page_table_stride; /* entries */
+    const float* k_scale;
+    const float* v_scale;
+    int kv_type;
+    int n_pages;
+    int page_size;
+    int max_pages;
+    int n_kv_heads;
+} nmi_paged_kv;
+
+/*
+ * Keys and values of new tokens stored in the cache, q and k rotated by position on the way.  Row t of
+ * q [tokens, >= n_heads * 128], k and v [tokens, >= n_kv_heads * 128] (bf16, row strides ldq, ldk, ldv)
+ * belongs to the sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1] (int32 [batch + 1]; NULL: one
+ * token per sequence, b = t) and has position start_pos[b] + t - cu_seqlens[b] (start_pos int32
+ * [batch]; a negative one marks a sequence that is not in use: nothing of it is read or written).
+ * Rows outside [cu_seqlens[0], cu_seqlens[batch]) are left alone.
+ *   rotation   rotary_dim > 0 (a multiple of 8, at most 128) with inv_freq float32 [rotary_dim / 2]: the
+ *              angle of pair i is position * inv_freq[i], formed in 64 bits; pairs are dims (i, i +
+ *              rotary_dim / 2), or (2i, 2i + 1) where interleaved is not 0; (x, y) becomes
+ *              (x cos - y sin, x sin + y cos) in float32; dims from rotary_dim on stay.  rotary_dim = 0
+ *              and inv_freq NULL: none (the framework's own model has none).
+ *   cache      k rotated, v as it is: rounded once, to bf16, or divided by the head's scale (float32) to
+ *              e4m3, to nearest even, values past +-448 as +-448, NaN as NaN.
+ *   q_out, k_out  the rotated q and k as bf16 (q and q_out both or neither; k_out for the attention over
+ *              the prompt itself); each may be its input, else must not overlap anything.
+ * No two tokens of a call may have the same place in the pool.  One launch, no workspace.
+ */
+int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, const void* k_bf16, int64_t ldk,
+                        const void* v_bf16, int64_t ldv, void* q_out_bf16, int64_t ldqo, void* k_out_bf16, int64_t ldko,
+                        const int32_t* cu_seqlens, const int32_t* start_pos, int batch, int tokens, int n_heads,
+                        const float* inv_freq, int rotary_dim, int interleaved, void* stream);
+
+/*
+ * Decode attention over a paged cache, one query token per sequence:
+ *   o[b, h] = bf16( softmax_s(scale * q[b, h] . k_s) . v_s ),  s < kv_lens[b],
+ * KV head h / (n_heads / n_kv_heads); float32 arithmetic.  Every length counts the positions attended,
+ * so a token just appended is included by a length that counts it (nmi_sdpa_decode_bf16 attends the
+ * positions before the new one).  A length of 0 (or below) gives o = 0: the unused rows of a padded batch.
+ * q [batch, >= n_heads * 128], o [batch, >= n_heads * 128] bf16, row strides ldq (multiple of 8) and
+ * ldo (even); kv_lens int32 [batch]; scale positive (1 / sqrt(128) for plain attention).  Any n_heads
+ * that is a multiple of n_kv_heads (up to 16 query heads per KV head share one read of the cache).
+ * The work is split by the lengths found on the device: the launch depends on the batch size only.
+ * workspace: nmi_sdpa_decode_paged_workspace_bytes(batch, n_heads, n_kv_heads) bytes, 16-byte aligned,
+ * no initialisation; NULL takes it from the bump allocator.  Two launches, the second joining the splits
+ * in a fixed order: equal calls give the same bytes.
+ */
+size_t nmi_sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv_heads);
+int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,
+                          const int32_t* kv_lens, int batch, int n_heads, float scale, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention over packed prompts: nmi_sdpa_prefill_bf16 for each sequence b on rows [cu_seqlens[b],
+ * cu_seqlens[b + 1]) of q, k, v and o, with softmax(scale * q . k), in one launch whose grid depends on
+ * batch and tokens only.  cu_seqlens int32 [batch + 1], ascending (a sequence may be empty); rows of the
+ * `tokens` given that belong to no sequence are left as they were.  Layouts, alignment and strides as
+ * nmi_sdpa_prefill_bf16, strides at most 2^24; scale positive.  No workspace.
+ */
+int nmi_sdpa_prefill_packed_bf16(const void* q_bf16, int64_t ldq, const void* k_bf16, int64_t ldk, const void* v_bf16,
+                                 int64_t ldv, void* o_bf16, int64_t ldo, const int32_t* cu_seqlens, int batch, int tokens,
+                                 int n_heads, int n_kv_heads, float scale, void* stream);
 
 /*
  * The fp8 Mamba-2 block at decode, one token per sequence (replaces

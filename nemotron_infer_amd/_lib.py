@@ -17,7 +17,7 @@ NMI_ERR_ALIGNMENT = -2
 NMI_ERR_UNSUPPORTED = -3
 NMI_ERR_WORKSPACE = -4
 NMI_ERR_ALLOC = -5
-NMI_ERR_ASYNC = -6            # an earlier launch's asynchronous error (stream-K wait gave up)
+NMI_ERR_ASYNC = -6            # an earlier launch's asynchronous error (stream-K wait, paged device data out of range)
 NMI_WS_ERROR_OFFSET = 65532   # byte offset of the stream-K error word in a linear workspace
 
 # Every symbol the header declares, with its ctypes signature.
@@ -51,6 +51,10 @@ SIGNATURES = {
     "nmi_mamba_decode_fp8": ([_vp] * 15 + [_i] * 7 + [_f, _vp, _sz, _vp], _i),
     "nmi_attn_decode_fp8": ([_vp] * 12 + [_i, _i, _vp, _i, _i, _i, _f, _vp, _sz, _vp], _i),
     "nmi_mlp_forward_fp8_noalloc": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp], _i),
+    "nmi_kv_append_paged": ([_vp] + [_vp, _i64] * 5 + [_vp, _vp, _i, _i, _i, _vp, _i, _i, _vp], _i),
+    "nmi_sdpa_decode_paged_workspace_bytes": ([_i] * 3, _sz),
+    "nmi_sdpa_decode_paged": ([_vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _vp, _sz, _vp], _i),
+    "nmi_sdpa_prefill_packed_bf16": ([_vp, _i64] * 4 + [_vp] + [_i] * 4 + [_f, _vp], _i),
     "nmi_tuning_set": ([ctypes.c_char_p, _i], _i),
     "nmi_alloc": ([_sz, ctypes.POINTER(_vp)], _i),
     "nmi_alloc_rewind": ([], _i),
@@ -86,6 +90,17 @@ class GemvPhase(ctypes.Structure):
     """nmi_gemv_phase of include/nmi_fp8_linear.h."""
     _fields_ = [("x_bf16", _vp), ("K", _i), ("ngroups", _i), ("wait_prev", _i),
                 ("groups", LinearGroup * MAX_GROUPS)]
+
+
+NMI_KV_BF16, NMI_KV_E4M3 = 0, 1
+
+
+class PagedKv(ctypes.Structure):
+    """nmi_paged_kv of include/nmi_fp8_linear.h."""
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("page_stride", _i64), ("head_stride", _i64),
+                ("token_stride", _i64), ("page_table", _vp), ("page_table_stride", _i64), ("k_scale", _vp),
+                ("v_scale", _vp), ("kv_type", _i), ("n_pages", _i), ("page_size", _i), ("max_pages", _i),
+                ("n_kv_heads", _i)]
 
 
 _lib = None

@@ -97,34 +97,47 @@ Tuning& tuning() {
 
 namespace {
 constexpr int kAsyncMaxDevices = 64;
-std::atomic<uint32_t*> g_async_words{nullptr};
+std::atomic<uint32_t*> g_async_words{nullptr};      // [kAsyncKinds][kAsyncMaxDevices]
 std::once_flag g_async_once;
 }  // namespace
 
-uint32_t* async_error_word() {
+uint32_t* async_error_word(AsyncKind kind) {
     std::call_once(g_async_once, [] {
         // pinned, coherent host memory: the kernel's system-scope store is visible to the host
-        // without a GPU synchronisation; one word per device
+        // without a GPU synchronisation; one word per kind and device.  The first call may come while
+        // a stream is being captured, which this allocation has no part in.
+        constexpr size_t bytes = (size_t)kAsyncKinds * kAsyncMaxDevices * sizeof(uint32_t);
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
         void* p = nullptr;
-        if (hipHostMalloc(&p, kAsyncMaxDevices * sizeof(uint32_t), hipHostMallocCoherent | hipHostMallocPortable) ==
-                hipSuccess &&
-            p) {
-            std::memset(p, 0, kAsyncMaxDevices * sizeof(uint32_t));
+        if (hipHostMalloc(&p, bytes, hipHostMallocCoherent | hipHostMallocPortable) == hipSuccess && p) {
+            std::memset(p, 0, bytes);
             g_async_words.store(static_cast<uint32_t*>(p), std::memory_order_release);
         } else {
             (void)hipGetLastError();
         }
+        if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
     });
     uint32_t* w = g_async_words.load(std::memory_order_acquire);
     const int dev = device_info().device;
-    return (w && dev >= 0 && dev < kAsyncMaxDevices) ? w + dev : nullptr;
+    return (w && dev >= 0 && dev < kAsyncMaxDevices) ? w + (int)kind * kAsyncMaxDevices + dev : nullptr;
 }
 
 bool take_async_error(const char* fn) {
     uint32_t* w = g_async_words.load(std::memory_order_acquire);
-    if (!w) return false;                           // no stream-K launch yet in this process
+    if (!w) return false;                           // no launch yet that could have one
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kAsyncMaxDevices) return false;
+    uint32_t* paged = w + (int)AsyncKind::Paged * kAsyncMaxDevices + dev;
+    if (__atomic_load_n(paged, __ATOMIC_ACQUIRE) != 0u) {
+        __atomic_store_n(paged, 0u, __ATOMIC_RELAXED);
+        set_last_error("%s: a call on a paged KV cache or on packed prompts launched earlier on device %d met device "
+                       "data out of range: a page id outside the pool, a length or position that its row of the page "
+                       "table does not hold, or sequence offsets that do not ascend within the rows given; nothing was "
+                       "launched by this call",
+                       fn, dev);
+        return true;
+    }
     if (__atomic_load_n(w + dev, __ATOMIC_ACQUIRE) == 0u) return false;
     __atomic_store_n(w + dev, 0u, __ATOMIC_RELAXED);
     set_last_error("%s: a stream-K GEMM launched earlier on device %d gave up waiting for a partial tile, so that "

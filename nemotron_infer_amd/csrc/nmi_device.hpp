@@ -148,6 +148,24 @@ __device__ __forceinline__ float wave_sum(float v) {
     return (r0 + r1) + (r2 + r3);
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add_u32(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+// Inclusive sums over the 64 lanes; the value of one lane for all.
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    v = dpp_add_u32<0x111, 0xF>(v);     // row_shr 1
+    v = dpp_add_u32<0x112, 0xF>(v);     // row_shr 2
+    v = dpp_add_u32<0x114, 0xF>(v);     // row_shr 4
+    v = dpp_add_u32<0x118, 0xF>(v);     // row_shr 8
+    v = dpp_add_u32<0x142, 0xA>(v);     // row 0's sum to row 1, row 2's to row 3
+    v = dpp_add_u32<0x143, 0xC>(v);     // rows 0 and 1's to rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, int lane) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
 // 16-byte global load that bypasses the caches' retention policy (streamed weights).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 load_stream16(const uint8_t* p) {

@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "nmi_paged.hpp"
+
 namespace nmi {
 
 struct DeviceInfo {
@@ -22,13 +24,17 @@ void set_last_error(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
 // Per-device properties, queried once per device (thread-safe).
 const DeviceInfo& device_info();
 
-// Asynchronous errors of the stream-K GEMM: a finisher that gave up waiting for a partial tile
-// (that launch's output is wrong) sets the current device's word in pinned host memory as well as
-// the workspace's.  async_error_word() returns the device's word (allocated on first use, one
-// array for the process; nullptr if that fails, and then the GEMM does not use stream-K).
-// take_async_error(fn) reads and clears it without synchronising the GPU; when it was set it
+// Asynchronous errors, of two kinds.  StreamK: a finisher of the stream-K GEMM that gave up waiting
+// for a partial tile (that launch's output is wrong) sets the current device's word in pinned host
+// memory as well as the workspace's.  Paged: a kernel met a page id, length or offset in device
+// memory that it must not follow (nmi_paged.hpp).  async_error_word() returns the device's word of a
+// kind (allocated on first use, one array for the process; nullptr if that fails, and then the GEMM
+// does not use stream-K and the paged kernels report nothing).
+// take_async_error(fn) reads and clears one without synchronising the GPU; when one was set it
 // records a message naming fn and returns true (the caller returns NMI_ERR_ASYNC).
-uint32_t* async_error_word();
+enum class AsyncKind { StreamK = 0, Paged = 1 };
+constexpr int kAsyncKinds = 2;
+uint32_t* async_error_word(AsyncKind kind = AsyncKind::StreamK);
 bool take_async_error(const char* fn);
 
 // Tuning knobs (0 = automatic).  Set through nmi_tuning_set() for sweeps; never needed for
@@ -254,6 +260,43 @@ hipError_t launch_sdpa_decode(const uint16_t* q, uint16_t* k_cache, uint16_t* v_
                               const uint16_t* v_new, uint16_t* o, int S, int cap, int n_heads, int n_kv,
                               void* workspace, hipStream_t stream);
 
+// Paged KV caches (bf16, or e4m3 with a scale per KV head).  Append (kv_append.hip): row t of k and v
+// (and of q, rotated only) belongs to sequence b with cu[b] <= t < cu[b + 1] (cu nullptr: b = t) and
+// position start[b] + t - cu[b].
+struct AppendArgs {
+    PagedKv kv;
+    const uint16_t* q;          // [tokens, ldq] or nullptr
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* q_out;
+    uint16_t* k_out;            // or nullptr
+    int64_t ldq, ldk, ldv, ldqo, ldko;
+    const int32_t* cu;          // [batch + 1] or nullptr
+    const int32_t* start;       // [batch]
+    const float* inv_freq;      // [rotary / 2] or nullptr
+    int batch, tokens, H, rotary;
+    bool interleaved;
+};
+hipError_t launch_kv_append(const AppendArgs& a, bool e4m3, hipStream_t stream);
+
+// Decode attention over a paged cache (sdpa_decode_paged.hip): q [batch, ldq] against each sequence's
+// first lens[b] positions.
+struct PagedDecodeArgs {
+    PagedKv kv;
+    const uint16_t* q;
+    uint16_t* o;
+    int64_t ldq, ldo;
+    const int32_t* lens;        // [batch]
+    float* part_o;              // [slots, H, 128] sums of each split, and
+    float* part_ml;             // [slots, H, 2] its maximum and row sum
+    int batch, H, group;        // group: query heads per KV head
+    int budget;                 // splits beyond one per sequence
+    float scale2;               // log2(e) * softmax scale
+};
+int sdpa_decode_paged_budget(int batch, int n_kv, int group);
+size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv);
+hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, bool e4m3, void* workspace, hipStream_t stream);
+
 // Mamba-2 mixer at decode (mamba_decode.hip): conv1d step + SiLU, SSM state update and
 // output, gated RMSNorm, for `batch` sequences of one token.  Shapes: H heads of P, G groups,
 // state size kMambaDState, conv width kMambaConvK (mamba_decode_supported).
@@ -308,6 +351,14 @@ hipError_t launch_mamba_prefill_mixer(const MambaPrefillArgs& a, int batch, hipS
 hipError_t launch_sdpa_prefill(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
                                int64_t ldv, uint16_t* o, int64_t ldo, int S, int H, int H_KV, uint16_t* k_cache,
                                uint16_t* v_cache, int cap, hipStream_t stream);
+
+// The same over packed prompts: rows [cu[b], cu[b + 1]) of `tokens` are sequence b (device data).  At
+// most sdpa_prefill_packed_tiles query tiles per head (the launch's workgroups): a sequence ends in at
+// most one partial tile.
+int64_t sdpa_prefill_packed_tiles(int tokens, int batch);
+hipError_t launch_sdpa_prefill_packed(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
+                                      int64_t ldv, uint16_t* o, int64_t ldo, const int32_t* cu, int batch, int tokens,
+                                      int H, int H_KV, float scale, hipStream_t stream);
 
 hipError_t launch_sk_flags_clear(void* ws, hipStream_t stream);
 // Several matrices sharing x: one launch of the DMA-fed kernel (from M = 512 where it takes them all,

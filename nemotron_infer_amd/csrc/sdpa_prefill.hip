@@ -48,6 +48,7 @@
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 
+#include <algorithm>
 #include <cfloat>
 #include <type_traits>
 
@@ -76,6 +77,10 @@ struct PrefillArgs {
     uint16_t* k_cache;      // [H_KV, cap, 128] caches to fill from k and v (positions [0, S)), or nullptr
     uint16_t* v_cache;
     int cap;
+    // packed prompts: S rows in all, sequence b's are [cu[b], cu[b + 1])
+    const int32_t* cu;
+    int batch;
+    uint32_t* error;        // host word to set where cu does not ascend within [0, S], or nullptr
 };
 
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -85,6 +90,54 @@ __device__ __forceinline__ int k_off(int r, int c) { return r * 256 + ((c ^ (r &
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
+// Query tiles of packed sequence b (none past the last); its rows [*first, *first + *len).
+__device__ __forceinline__ int packed_tiles(const PrefillArgs& a, int b, int* first, int* len, bool* bad) {
+    *first = *len = 0;
+    if (b < a.batch) *len = checked_span(a.cu[b], a.cu[b + 1], a.S, first, bad);
+    return (*len + kBQ - 1) / kBQ;
+}
+// Tiles of all sequences that are their sequence's tile x or a later one; with the tiles of the first
+// 64 sequences at hand.
+__device__ __forceinline__ int packed_from(const PrefillArgs& a, int nt, int x, int lane) {
+    uint32_t n = lane_u32(wave_scan_u32((uint32_t)max(0, nt - x)), 63);
+    for (int b0 = 64; b0 < a.batch; b0 += 64) {
+        int first, len;
+        bool bad = false;
+        n += lane_u32(wave_scan_u32((uint32_t)max(0, packed_tiles(a, b0 + lane, &first, &len, &bad) - x)), 63);
+    }
+    return (int)n;
+}
+// Tile `rank` of all sequences' tiles, longest (latest in its sequence) first: its number in its
+// sequence, and that sequence's rows.  Every wave finds it by itself: a binary search for the tile
+// number, the tiles of the first 64 sequences in the lanes, then the rank-th of the sequences that
+// have such a tile.
+__device__ __forceinline__ int packed_find(const PrefillArgs& a, int nt, int first, int len, int rank, int lane,
+                                           int* row0, int* S) {
+    int lo = 0, hi = (a.S + kBQ - 1) / kBQ;                     // tiles from lo on: more than rank; from hi: not
+    while (hi - lo > 1) {
+        const int x = (lo + hi) / 2;
+        if (packed_from(a, nt, x, lane) > rank) lo = x;
+        else hi = x;
+    }
+    int j = rank - packed_from(a, nt, lo + 1, lane);
+    for (int b0 = 0;; b0 += 64) {
+        bool bad = false;
+        if (b0) nt = packed_tiles(a, b0 + lane, &first, &len, &bad);
+        const uint64_t has = __builtin_amdgcn_ballot_w64(nt > lo);
+        const int n = __popcll(has);
+        if (j < n || b0 + 64 >= a.batch) {
+            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+            const uint64_t it = __builtin_amdgcn_ballot_w64(nt > lo && before == j);
+            const int i = it ? __builtin_ctzll(it) : 0;
+            *row0 = __builtin_amdgcn_readlane(first, i);
+            *S = __builtin_amdgcn_readlane(len, i);
+            return lo;
+        }
+        j -= n;
+    }
+}
+
+template <bool PACKED>
 __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs a) {
     typedef __attribute__((address_space(3))) void lds_void;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -96,23 +149,40 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
     // r % H.  The dispatcher gives each CU one workgroup per pass (workgroups g and g + nslot
     // share a CU), so the second pass takes its ranks in reverse: a CU then holds a long and a
     // short tile of about the same sum; the rest follow longest first.
-    const int total = a.qtiles * a.H, g = (int)blockIdx.x;
+    const int g = (int)blockIdx.x;
+    int total = a.qtiles * a.H, nt0 = 0, first0 = 0, len0 = 0;
+    if constexpr (PACKED) {
+        bool bad = false;
+        nt0 = packed_tiles(a, lane, &first0, &len0, &bad);
+        total = packed_from(a, nt0, 0, lane) * a.H;
+        if (g == 0 && wave == 0 && a.error) {
+            for (int b0 = 64; b0 < a.batch; b0 += 64) {
+                int first, len;
+                (void)packed_tiles(a, b0 + lane, &first, &len, &bad);
+            }
+            if (bad) __hip_atomic_store(a.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        }
+        if (g >= total) return;                                 // the grid holds the most tiles there could be
+    }
     const int n2 = min(2 * a.nslot, total);
     const int rank = (g >= a.nslot && g < n2) ? a.nslot + (n2 - 1 - g) : g;
-    const int qt = a.qtiles - 1 - rank / a.H;
     const int head = rank - rank / a.H * a.H;
     const int kvh = head / (a.H / a.H_KV);
+    int qt = a.qtiles - 1 - rank / a.H, S = a.S, row0 = 0;
+    if constexpr (PACKED) {
+        qt = packed_find(a, nt0, first0, len0, rank / a.H, lane, &row0, &S);
+        if (qt * kBQ >= S) return;                              // (only if cu changes under the launch)
+    }
     const int q0 = qt * kBQ;
     const int qw = q0 + 32 * wave;                              // the wave's first query row
     const int qrow = qw + l32;                                  // this lane's query (B operand column)
-    const int S = a.S;
     const int kv_end = min(S, q0 + kBQ);                        // keys this workgroup needs
     const int ntiles = (kv_end + kBK - 1) / kBK;
 
     // the wave's query rows as B fragments: k step s holds dims 16 s + 8 h .. + 7 of row qrow
     bf16x8 qf[8];
     {
-        const uint16_t* qp = a.q + (int64_t)min(qrow, S - 1) * a.ldq + head * kD + 8 * h;
+        const uint16_t* qp = a.q + (int64_t)(row0 + min(qrow, S - 1)) * a.ldq + head * kD + 8 * h;
 #pragma unroll
         for (int s = 0; s < 8; ++s) qf[s] = __builtin_bit_cast(bf16x8, load16(qp + 16 * s));
     }
@@ -129,8 +199,8 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
     const uint32_t koff = (uint32_t)(kr0 * ldk2) + kchunk;
     const uint32_t vchunk = 16u * (uint32_t)((lane & 15) ^ (4 * (kr0 & 3)));
     const uint32_t voff = (uint32_t)(kr0 * ldv2) + vchunk;
-    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + kvh * kD);
-    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + kvh * kD);
+    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.k + row0 * a.ldk + kvh * kD);
+    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.v + row0 * a.ldv + kvh * kD);
     const int nblk = 2 * ntiles;
     // K block g into slot g % 4; rows past S - 1 (of a last, partial block, or of a block wholly
     // past S) read row S - 1
@@ -398,7 +468,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
     if (nblk > 2) asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(4)\n\ts_barrier" ::: "memory");
     // this workgroup's share of the KV cache fill: its own rows, by one query head of the group
-    const bool fill = a.k_cache && head % (a.H / a.H_KV) == qt % (a.H / a.H_KV);
+    const bool fill = !PACKED && a.k_cache && head % (a.H / a.H_KV) == qt % (a.H / a.H_KV);
     uint4 kr[8], vr[8];
     if (fill) {
 #pragma unroll
@@ -474,7 +544,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
     // O = O^T / l: register r of block b is dim 32 b + 8 (r / 4) + 4 h + r % 4 of query qrow
     if (qrow < S) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        uint16_t* op = a.o + (int64_t)qrow * a.ldo + head * kD;
+        uint16_t* op = a.o + (int64_t)(row0 + qrow) * a.ldo + head * kD;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -488,12 +558,21 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
 
 }  // namespace
 
+template <bool PACKED>
+static hipError_t launch(PrefillArgs a, int64_t tiles, hipStream_t stream) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_prefill_kernel<PACKED>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (attr != hipSuccess) return attr;
+    a.qtiles = (a.S + kBQ - 1) / kBQ;
+    a.nslot = device_info().num_cu;
+    a.lazy = kLazy / a.scale2;
+    hipLaunchKernelGGL(sdpa_prefill_kernel<PACKED>, dim3((uint32_t)(tiles * a.H)), dim3(256), kLds, stream, a);
+    return hipGetLastError();
+}
+
 hipError_t launch_sdpa_prefill(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
                                int64_t ldv, uint16_t* o, int64_t ldo, int S, int H, int H_KV, uint16_t* k_cache,
                                uint16_t* v_cache, int cap, hipStream_t stream) {
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_prefill_kernel),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (attr != hipSuccess) return attr;
     PrefillArgs a{};
     a.q = q;
     a.k = k;
@@ -506,15 +585,35 @@ hipError_t launch_sdpa_prefill(const uint16_t* q, int64_t ldq, const uint16_t* k
     a.S = S;
     a.H = H;
     a.H_KV = H_KV;
-    a.qtiles = (S + kBQ - 1) / kBQ;
-    a.nslot = device_info().num_cu;
     a.scale2 = 1.4426950408889634f / sqrtf((float)kD);
-    a.lazy = kLazy / a.scale2;
     a.k_cache = k_cache;
     a.v_cache = v_cache;
     a.cap = cap;
-    hipLaunchKernelGGL(sdpa_prefill_kernel, dim3(a.qtiles * H), dim3(256), kLds, stream, a);
-    return hipGetLastError();
+    return launch<false>(a, (S + kBQ - 1) / kBQ, stream);
+}
+
+int64_t sdpa_prefill_packed_tiles(int tokens, int batch) { return (int64_t)(tokens / kBQ) + std::min(batch, tokens); }
+
+hipError_t launch_sdpa_prefill_packed(const uint16_t* q, int64_t ldq, const uint16_t* k, int64_t ldk, const uint16_t* v,
+                                      int64_t ldv, uint16_t* o, int64_t ldo, const int32_t* cu, int batch, int tokens,
+                                      int H, int H_KV, float scale, hipStream_t stream) {
+    PrefillArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.o = o;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldo = ldo;
+    a.S = tokens;
+    a.H = H;
+    a.H_KV = H_KV;
+    a.scale2 = 1.4426950408889634f * scale;
+    a.cu = cu;
+    a.batch = batch;
+    a.error = async_error_word(AsyncKind::Paged);
+    return launch<true>(a, sdpa_prefill_packed_tiles(tokens, batch), stream);
 }
 
 }  // namespace nmi
