@@ -287,13 +287,14 @@ struct PagedDecodeArgs {
     uint16_t* o;
     int64_t ldq, ldo;
     const int32_t* lens;        // [batch]
-    float* part_o;              // [slots, H, 128] sums of each split, and
-    float* part_ml;             // [slots, H, 2] its maximum and row sum
+    float* part_o;              // [waves + batch, H, 128] sums of each piece of a sequence, and
+    float2* part_ml;            // [waves + batch, H] its maximum and row sum
+    Pieces* plan;               // [batch] each sequence's pieces
     int batch, H, group;        // group: query heads per KV head
-    int budget;                 // splits beyond one per sequence
+    int waves;                  // waves per KV head (and 16 of its query heads)
     float scale2;               // log2(e) * softmax scale
 };
-int sdpa_decode_paged_budget(int batch, int n_kv, int group);
+int sdpa_decode_paged_waves(int n_kv, int group);
 size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv);
 hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, bool e4m3, void* workspace, hipStream_t stream);
 

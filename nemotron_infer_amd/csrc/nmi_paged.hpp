@@ -62,17 +62,57 @@ NMI_HD int checked_span(int c0, int c1, int tokens, int* first, bool* bad) {
     return e - f;
 }
 
-// Decode attention: tiles per split when `total` tiles of all sequences are to make at most `budget`
-// splits beyond the one that every sequence has; a multiple of `unit`, so that the waves of a
-// workgroup get equal shares.  With n_b = max(1, ceil(tiles_b / result)) the splits of all sequences
-// number at most batch + budget: sum ceil(t_b / c) <= batch + total / c.  Never more than a whole
-// sequence of the most positions.
+// Decode attention: tiles per wave when all sequences' tiles, `total` of them in a row, are dealt to at
+// most `waves` waves, at least `unit` to each.
 constexpr int kPagedMaxPositions = 1 << 30;
-NMI_HD int split_tiles(uint32_t total, int budget, int unit) {
-    const uint32_t c = (total + (uint32_t)budget - 1) / (uint32_t)budget;
-    const uint32_t m = (c + (uint32_t)unit - 1) / (uint32_t)unit;
-    constexpr uint32_t most = kPagedMaxPositions / kPagedTile;
-    return (int)(m < 1 ? (uint32_t)unit : m > most / (uint32_t)unit ? most : m * (uint32_t)unit);
+constexpr int kPagedWaves = 4;          // per workgroup
+NMI_HD int range_tiles(uint32_t total, int waves, int unit) {
+    const uint32_t c = (total + (uint32_t)waves - 1) / (uint32_t)waves;
+    return c > (uint32_t)unit ? (int)c : unit;
+}
+
+// Wave x's tiles [range_first(x), range_first(x + 1)) of that row; none where the row is shorter.
+NMI_HD uint32_t range_first(uint32_t x, int c, uint32_t total) {
+    const uint64_t f = (uint64_t)x * (uint32_t)c;
+    return f < total ? (uint32_t)f : total;
+}
+
+// The pieces of a sequence with tiles [first, first + tiles) of the row, one at least.  A workgroup all
+// of whose tiles are the sequence's takes them together, as one piece; of another, each wave takes a
+// piece.  So there are `head` waves' pieces of the first workgroup (from `wave` on), `joint` workgroups',
+// `tail` waves' of the last.  A piece that wave x, or the workgroup whose first wave is x, has of
+// sequence b is left in slot x + b: going along the row, x or b or both grow from one piece to the
+// next, so no two share a slot, and waves + batch slots are enough.
+struct Pieces {
+    int wave, head, joint, tail;
+    NMI_HD int count() const { return head + joint + tail; }
+    NMI_HD int owner(int i) const {     // x of piece i
+        if (i < head) return wave + i;
+        const int group = wave / kPagedWaves + (head > 0 ? 1 : 0);
+        if (i < head + joint) return (group + i - head) * kPagedWaves;
+        return (group + joint) * kPagedWaves + i - head - joint;
+    }
+};
+// Whether workgroup x has no tiles but the sequence's.
+NMI_HD bool is_joint(uint32_t x, uint32_t first, uint32_t tiles, int c, uint32_t total) {
+    return first <= range_first(x * kPagedWaves, c, total) && first + tiles >= range_first((x + 1) * kPagedWaves, c, total);
+}
+NMI_HD Pieces pieces_of(uint32_t first, uint32_t tiles, int c, uint32_t total) {
+    const uint32_t w0 = first / (uint32_t)c, w1 = (first + tiles - 1) / (uint32_t)c;
+    const uint32_t g0 = w0 / kPagedWaves, g1 = w1 / kPagedWaves;
+    const bool joint0 = is_joint(g0, first, tiles, c, total), joint1 = is_joint(g1, first, tiles, c, total);
+    Pieces p;
+    p.wave = (int)w0;
+    if (g0 == g1) {
+        p.head = joint0 ? 0 : (int)(w1 - w0 + 1);
+        p.joint = joint0 ? 1 : 0;
+        p.tail = 0;
+    } else {
+        p.head = joint0 ? 0 : (int)(kPagedWaves * (g0 + 1) - w0);
+        p.tail = joint1 ? 0 : (int)(w1 - kPagedWaves * g1 + 1);
+        p.joint = (int)(g1 - g0 + 1) - (p.head ? 1 : 0) - (p.tail ? 1 : 0);
+    }
+    return p;
 }
 
 }  // namespace nmi

@@ -159,8 +159,8 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
     if (batch < 1 || n_heads < n_kv || n_heads % n_kv || n_heads > 65535)
         return refuse(NMI_ERR_INVALID_ARG, "%s: batch=%d n_heads=%d n_kv_heads=%d (need batch >= 1, n_heads a multiple)",
                       fn, batch, n_heads, n_kv);
-    // every sequence at its longest, in tiles, summed by the kernel in 32 bits; and the launch's axes
-    if (batch + (int64_t)sdpa_decode_paged_budget(batch, n_kv, n_heads / n_kv) > kMaxGroups256)
+    // the joining launch's axis; and every sequence at its longest, in tiles, summed by the kernel in 32 bits
+    if (batch > kMaxGroups256)
         return refuse(NMI_ERR_INVALID_ARG, "%s: batch=%d is too large for one launch", fn, batch);
     if ((int64_t)batch * (((int64_t)a.kv.max_pages << a.kv.page_shift) / kPagedTile) > INT32_MAX)
         return refuse(NMI_ERR_INVALID_ARG, "%s: batch=%d sequences of up to %lld positions are more than 2^35", fn, batch,

@@ -9,6 +9,7 @@ include/nmi_fp8_linear.h; there is no torch or CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -637,56 +638,84 @@ def mamba_forward_fp8(x: torch.Tensor, norm_w: torch.Tensor, in_w, in_s, conv_w,
     return out
 
 
-def _elsewhere(t: torch.Tensor):
-    """None where t's GPU is the current device, else a context that makes it so (the stream, the
-    launch and the library's per-device state go by the current device)."""
-    if not t.is_cuda or t.get_device() == torch.cuda.current_device():
-        return None
-    return torch.cuda.device(t.device)
+# The operators below are called once per layer and step at sizes where the host bounds the call, so
+# each tensor's properties are asked for once: a helper checks a tensor and returns what the call passes
+# on.  (With a helper per property, a look for the device of all tensors at the end and a ctypes
+# structure for the cache, an eager append took 16.3 us and a decode 17.6 us; so NN and NN.)
+_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
+_PAGED_KV = struct.Struct("@2P3qPq2P5i4x")     # nmi_paged_kv
 
 
-def _check_ints(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 vector of {n} values, got {t.dtype} {tuple(t.shape)}")
-    return t
+def _rows(t: torch.Tensor, T: int, cols: int, name: str, dev: int):
+    """Rows [T, >= cols] of bf16 on GPU `dev`: (address, row stride)."""
+    shape, st = t.shape, t.stride()
+    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] != T or shape[1] < cols or st[1] != 1:
+        raise ValueError(f"{name} must be a bf16 [{T}, >= {cols}] tensor with contiguous rows, got {t.dtype} "
+                         f"{tuple(shape)} strides {st}")
+    if t.get_device() != dev:
+        raise ValueError(f"all tensors must be on one GPU: {name} is on {t.device}")
+    # (torch's stride of a dimension of one element has no meaning)
+    return t.data_ptr(), st[0] if T > 1 else (shape[1] + 7) // 8 * 8
 
 
-def _paged_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, batch: int, k_scale, v_scale):
-    """The cache's descriptor, its tensors checked: pages [n_pages, n_kv_heads, page_size, 128] of any
-    strides with contiguous head vectors, K and V alike."""
-    if k_pages.dim() != 4 or k_pages.shape[3] != 128 or k_pages.stride(3) != 1:
+def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, dev: int) -> int:
+    """A contiguous vector of n values on GPU `dev`: its address."""
+    shape = t.shape
+    if t.dtype is not dtype or len(shape) != 1 or shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} values, got {t.dtype} {tuple(shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"all tensors must be on one GPU: {name} is on {t.device}")
+    return t.data_ptr()
+
+
+def _paged_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, batch: int, k_scale, v_scale,
+              dev: int):
+    """The cache's descriptor (an nmi_paged_kv) and its KV heads: pages [n_pages, n_kv_heads, page_size,
+    128] of any strides with contiguous head vectors, K and V alike."""
+    shape, st, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
+    if len(shape) != 4 or shape[3] != 128 or st[3] != 1:
         raise ValueError(f"k_pages must be [n_pages, n_kv_heads, page_size, 128] with contiguous head vectors, got "
-                         f"{tuple(k_pages.shape)} strides {k_pages.stride()}")
-    if k_pages.dtype == torch.bfloat16:
-        kind = _lib.NMI_KV_BF16
-    elif k_pages.dtype in (torch.float8_e4m3fn, torch.uint8):
-        kind = _lib.NMI_KV_E4M3
-    else:
-        raise TypeError(f"pages must be bfloat16, float8_e4m3fn or uint8 codes, got {k_pages.dtype}")
-    if v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
-        raise ValueError(f"v_pages must be as k_pages ({k_pages.dtype} {tuple(k_pages.shape)} strides "
-                         f"{k_pages.stride()}), got {v_pages.dtype} {tuple(v_pages.shape)} strides {v_pages.stride()}")
-    n_pages, n_kv, page_size, _ = k_pages.shape
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch or (
-            page_table.stride(1) != 1):
+                         f"{tuple(shape)} strides {st}")
+    e4m3 = dtype is not _BF16
+    if e4m3 and dtype is not torch.float8_e4m3fn and dtype is not torch.uint8:
+        raise TypeError(f"pages must be bfloat16, float8_e4m3fn or uint8 codes, got {dtype}")
+    if v_pages.dtype is not dtype or v_pages.shape != shape or v_pages.stride() != st:
+        raise ValueError(f"v_pages must be as k_pages ({dtype} {tuple(shape)} strides {st}), got {v_pages.dtype} "
+                         f"{tuple(v_pages.shape)} strides {v_pages.stride()}")
+    tshape, tst = page_table.shape, page_table.stride()
+    if page_table.dtype is not _I32 or len(tshape) != 2 or tshape[0] != batch or tst[1] != 1:
         raise ValueError(f"page_table must be int32 [batch={batch}, max_pages] with contiguous rows, got "
-                         f"{page_table.dtype} {tuple(page_table.shape)} strides {page_table.stride()}")
-    tensors = [k_pages, v_pages, page_table]
-    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if s is not None:
-            if kind == _lib.NMI_KV_BF16:
-                raise ValueError("a bf16 cache takes no scales")
-            _check_f32(s, (n_kv,), name)
-            tensors.append(s)
-    max_pages = page_table.shape[1]
-    ps, hs, ts, _ = k_pages.stride()
-    # (torch's stride of a dimension of one element is of no meaning)
-    ps, hs, ts = (st if n > 1 else 128 for st, n in zip((ps, hs, ts), (n_pages, n_kv, page_size)))
-    cache = _lib.PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), ps, hs, ts, page_table.data_ptr(),
-                         page_table.stride(0) if batch > 1 else max_pages,
-                         None if k_scale is None else k_scale.data_ptr(),
-                         None if v_scale is None else v_scale.data_ptr(), kind, n_pages, page_size, max_pages, n_kv)
-    return cache, n_kv, tensors
+                         f"{page_table.dtype} {tuple(tshape)} strides {tst}")
+    if k_pages.get_device() != dev or v_pages.get_device() != dev or page_table.get_device() != dev:
+        raise ValueError("all tensors must be on one GPU: the pages and the page table are on "
+                         f"{k_pages.device}, {v_pages.device} and {page_table.device}")
+    n_pages, n_kv, page_size, _ = shape
+    ks = vs = 0
+    if k_scale is not None or v_scale is not None:
+        if not e4m3:
+            raise ValueError("a bf16 cache takes no scales")
+        if k_scale is not None:
+            ks = _vector(k_scale, n_kv, _F32, "k_scale", dev)
+        if v_scale is not None:
+            vs = _vector(v_scale, n_kv, _F32, "v_scale", dev)
+    ps, hs, ts, _ = st
+    if n_pages == 1 or n_kv == 1 or page_size == 1:     # (strides without meaning)
+        ps, hs, ts = (s if n > 1 else 128 for s, n in zip(st, shape[:3]))
+    max_pages = tshape[1]
+    return _PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), ps, hs, ts, page_table.data_ptr(),
+                          tst[0] if batch > 1 else max_pages, ks, vs, int(e4m3), n_pages, page_size, max_pages,
+                          n_kv), n_kv
+
+
+def _check_current(dev: int, t: torch.Tensor) -> bool:
+    """Whether GPU `dev`, t's, is the current device, by which the stream, the launch and the library's
+    per-device state go (torch.cuda.device makes it so)."""
+    if dev < 0:
+        raise ValueError(f"tensors must be on a GPU, got {t.device}")
+    try:
+        return dev == torch._C._cuda_getDevice()
+    except AttributeError:                     # private to torch: another version may lack it
+        return dev == torch.cuda.current_device()
 
 
 def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -701,62 +730,48 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     page_table int32 [batch, max_pages].  With inv_freq (float32 [rotary_dim / 2]) k is rotated by
     position, and q [T, n_heads * 128] too.  Returns (q_out, k_out): the rotated q (None without q)
     and k_out, which receives the rotated k where it is given; either may be its input itself."""
-    context = _elsewhere(k)
-    if context is not None:
-        with context:
-            return kv_append_paged(k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q, inv_freq, interleaved,
-                                   k_scale, v_scale, q_out, k_out)
+    dev = k.get_device()
     if start_pos.dim() != 1:
         raise ValueError(f"start_pos must be an int32 vector [batch], got {tuple(start_pos.shape)}")
-    batch = start_pos.shape[0]
-    _check_ints(start_pos, batch, "start_pos")
-    cache, n_kv, tensors = _paged_kv(k_pages, v_pages, page_table, batch, k_scale, v_scale)
-    T = k.shape[0]
-    _check_rows(k, T, n_kv * 128, "k")
-    _check_rows(v, T, n_kv * 128, "v")
-    tensors += [k, v, start_pos]
+    batch, T = start_pos.shape[0], k.shape[0]
+    start = _vector(start_pos, batch, _I32, "start_pos", dev)
+    cache, n_kv = _paged_kv(k_pages, v_pages, page_table, batch, k_scale, v_scale, dev)
+    kp, ldk = _rows(k, T, n_kv * 128, "k", dev)
+    vp, ldv = _rows(v, T, n_kv * 128, "v", dev)
+    cu = qp = ldq = qop = ldqo = kop = ldko = freq = rotary = H = 0
     if cu_seqlens is not None:
-        tensors.append(_check_ints(cu_seqlens, batch + 1, "cu_seqlens"))
+        cu = _vector(cu_seqlens, batch + 1, _I32, "cu_seqlens", dev)
     elif T != batch:
         raise ValueError(f"{T} rows for {batch} sequences: give cu_seqlens")
-    rotary, H = 0, 0
     if inv_freq is not None:
-        _check_f32(inv_freq, (inv_freq.numel(),), "inv_freq")
         rotary = 2 * inv_freq.numel()
-        tensors.append(inv_freq)
+        freq = _vector(inv_freq, rotary // 2, _F32, "inv_freq", dev)
+        if q is not None:
+            H = q.shape[-1] // 128
+            if q.dim() != 2 or not H or q.shape[1] % (n_kv * 128):
+                raise ValueError(f"q must be [T, n_heads * 128], n_heads a multiple of {n_kv}, got {tuple(q.shape)}")
+            qp, ldq = _rows(q, T, H * 128, "q", dev)
+            if q_out is None:
+                q_out = q.new_empty((T, H * 128))
+                qop, ldqo = q_out.data_ptr(), H * 128
+            else:
+                qop, ldqo = _rows(q_out, T, H * 128, "q_out", dev)
+        if k_out is not None:
+            kop, ldko = _rows(k_out, T, n_kv * 128, "k_out", dev)
     elif q is not None or k_out is not None:
         raise ValueError("q and k_out are for the rotation: give inv_freq")
     if q is None and q_out is not None:
         raise ValueError("q_out without q")
-    if q is not None:
-        if q.dim() != 2 or q.shape[1] % (n_kv * 128):
-            raise ValueError(f"q must be [T, n_heads * 128], n_heads a multiple of {n_kv}, got {tuple(q.shape)}")
-        H = q.shape[1] // 128
-        _check_rows(q, T, H * 128, "q")
-        if q_out is None:
-            q_out = torch.empty((T, H * 128), dtype=torch.bfloat16, device=q.device)
-        _check_rows(q_out, T, H * 128, "q_out")
-        tensors += [q, q_out]
-    if k_out is not None:
-        _check_rows(k_out, T, n_kv * 128, "k_out")
-        tensors.append(k_out)
-    _check_device(*tensors)
-    if T == 0 or batch == 0:
-        return q_out, k_out
-    rc = _lib.lib().nmi_kv_append_paged(
-        ctypes.addressof(cache), None if q is None else q.data_ptr(), 0 if q is None else _row_stride(q),
-        k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v),
-        None if q is None else q_out.data_ptr(), 0 if q is None else _row_stride(q_out),
-        None if k_out is None else k_out.data_ptr(), 0 if k_out is None else _row_stride(k_out),
-        None if cu_seqlens is None else cu_seqlens.data_ptr(), start_pos.data_ptr(), batch, T, H,
-        None if inv_freq is None else inv_freq.data_ptr(), rotary, int(interleaved), _stream())
-    _lib.check(rc, "nmi_kv_append_paged")
+    if not _check_current(dev, k):
+        with torch.cuda.device(dev):
+            return kv_append_paged(k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q, inv_freq, interleaved,
+                                   k_scale, v_scale, q_out, k_out)
+    if T and batch:
+        rc = _lib.lib().nmi_kv_append_paged(cache, qp, ldq, kp, ldk, vp, ldv, qop, ldqo, kop, ldko, cu, start, batch, T, H,
+                                            freq, rotary, 1 if interleaved else 0, _stream())
+        if rc:
+            _lib.check(rc, "nmi_kv_append_paged")
     return q_out, k_out
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor (of one row its width: torch's stride has no meaning there)."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 7) // 8 * 8
 
 
 def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -766,35 +781,35 @@ def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     [batch, n_heads * 128] bf16 against the first kv_lens[b] (int32) positions of sequence b's pages
     (as kv_append_paged takes them); a length of 0 gives zeros.  scale: 1 / sqrt(128) unless given.
     Returns o [batch, n_heads * 128] bf16."""
-    context = _elsewhere(q)
-    if context is not None:
-        with context:
-            return sdpa_decode_paged(q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale, scale, out)
+    dev = q.get_device()
     if q.dim() != 2:
         raise ValueError(f"q must be [batch, n_heads * 128], got {tuple(q.shape)}")
-    batch = q.shape[0]
-    cache, n_kv, tensors = _paged_kv(k_pages, v_pages, page_table, batch, k_scale, v_scale)
-    if q.shape[1] % (n_kv * 128) or not q.shape[1]:
+    batch, cols = q.shape
+    cache, n_kv = _paged_kv(k_pages, v_pages, page_table, batch, k_scale, v_scale, dev)
+    if cols % (n_kv * 128) or not cols:
         raise ValueError(f"q must be [batch, n_heads * 128], n_heads a multiple of {n_kv}, got {tuple(q.shape)}")
-    H = q.shape[1] // 128
-    _check_rows(q, batch, H * 128, "q")
-    _check_ints(kv_lens, batch, "kv_lens")
+    qp, ldq = _rows(q, batch, cols, "q", dev)
+    lens = _vector(kv_lens, batch, _I32, "kv_lens", dev)
     if out is None:
-        out = torch.empty((batch, H * 128), dtype=torch.bfloat16, device=q.device)
-    _check_rows(out, batch, H * 128, "out")
-    _check_device(q, kv_lens, out, *tensors)
-    if batch == 0:
-        return out
-    L = _lib.lib()
-    st = _stream()
-    need = L.nmi_sdpa_decode_paged_workspace_bytes(batch, H, n_kv)
-    ws, key = _workspace(q.device, need, st)
-    rc = L.nmi_sdpa_decode_paged(ctypes.addressof(cache), q.data_ptr(), _row_stride(q), out.data_ptr(), _row_stride(out),
-                                 kv_lens.data_ptr(), batch, H, 128 ** -0.5 if scale is None else scale,
-                                 ws.data_ptr(), need, st)
-    if key is not None:
-        _kept[key] = ws
-    _lib.check(rc, "nmi_sdpa_decode_paged")
+        out = q.new_empty((batch, cols))
+        op, ldo = out.data_ptr(), cols
+    else:
+        op, ldo = _rows(out, batch, cols, "out", dev)
+    if not _check_current(dev, q):
+        with torch.cuda.device(dev):
+            return sdpa_decode_paged(q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale, scale, out)
+    if batch:
+        L = _lib.lib()
+        st = _stream()
+        H = cols // 128
+        need = L.nmi_sdpa_decode_paged_workspace_bytes(batch, H, n_kv)
+        ws, key = _workspace(q.device, need, st)
+        rc = L.nmi_sdpa_decode_paged(cache, qp, ldq, op, ldo, lens, batch, H, 128 ** -0.5 if scale is None else scale,
+                                     ws.data_ptr(), need, st)
+        if key is not None:
+            _kept[key] = ws
+        if rc:
+            _lib.check(rc, "nmi_sdpa_decode_paged")
     return out
 
 
@@ -805,29 +820,27 @@ def sdpa_prefill_packed_bf16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     cu_seqlens[b + 1]) (int32) of the token-major q [T, >= n_heads * 128], k, v [T, >= n_kv_heads * 128]
     are prompt b (row-strided views allowed).  scale: 1 / sqrt(128) unless given.  Returns o
     [T, n_heads * 128] bf16; rows of no prompt are left as they were (in a new o: undefined)."""
-    context = _elsewhere(q)
-    if context is not None:
-        with context:
-            return sdpa_prefill_packed_bf16(q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
-    T = q.shape[0]
-    _check_rows(q, T, n_heads * 128, "q")
-    _check_rows(k, T, n_kv_heads * 128, "k")
-    _check_rows(v, T, n_kv_heads * 128, "v")
+    dev, T = q.get_device(), q.shape[0]
+    qp, ldq = _rows(q, T, n_heads * 128, "q", dev)
+    kp, ldk = _rows(k, T, n_kv_heads * 128, "k", dev)
+    vp, ldv = _rows(v, T, n_kv_heads * 128, "v", dev)
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be an int32 vector [batch + 1], got {tuple(cu_seqlens.shape)}")
     batch = cu_seqlens.shape[0] - 1
-    _check_ints(cu_seqlens, batch + 1, "cu_seqlens")
+    cu = _vector(cu_seqlens, batch + 1, _I32, "cu_seqlens", dev)
     if out is None:
-        out = torch.empty((T, n_heads * 128), dtype=torch.bfloat16, device=q.device)
-    _check_rows(out, T, n_heads * 128, "out")
-    _check_device(q, k, v, cu_seqlens, out)
-    if T == 0 or batch == 0:
-        return out
-    rc = _lib.lib().nmi_sdpa_prefill_packed_bf16(
-        q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), out.data_ptr(),
-        _row_stride(out), cu_seqlens.data_ptr(), batch, T, n_heads, n_kv_heads,
-        128 ** -0.5 if scale is None else scale, _stream())
-    _lib.check(rc, "nmi_sdpa_prefill_packed_bf16")
+        out = q.new_empty((T, n_heads * 128))
+        op, ldo = out.data_ptr(), n_heads * 128
+    else:
+        op, ldo = _rows(out, T, n_heads * 128, "out", dev)
+    if not _check_current(dev, q):
+        with torch.cuda.device(dev):
+            return sdpa_prefill_packed_bf16(q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
+    if T and batch:
+        rc = _lib.lib().nmi_sdpa_prefill_packed_bf16(qp, ldq, kp, ldk, vp, ldv, op, ldo, cu, batch, T, n_heads, n_kv_heads,
+                                                     128 ** -0.5 if scale is None else scale, _stream())
+        if rc:
+            _lib.check(rc, "nmi_sdpa_prefill_packed_bf16")
     return out
 
 

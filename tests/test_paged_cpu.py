@@ -25,7 +25,14 @@ int len(int l, int max_pages, int shift, int* bad) {
 int span(int c0, int c1, int tokens, int* first, int* bad) {
     bool b = false; int r = nmi::checked_span(c0, c1, tokens, first, &b); *bad = b; return r;
 }
-int split(unsigned total, int budget, int unit) { return nmi::split_tiles(total, budget, unit); }
+int share(unsigned total, int waves, int unit) { return nmi::range_tiles(total, waves, unit); }
+unsigned first(unsigned x, int c, unsigned total) { return nmi::range_first(x, c, total); }
+int joint(unsigned x, unsigned first, unsigned tiles, int c, unsigned total) { return nmi::is_joint(x, first, tiles, c, total); }
+int pieces(unsigned first, unsigned tiles, int c, unsigned total, int* owners, int most) {
+    const nmi::Pieces p = nmi::pieces_of(first, tiles, c, total);
+    for (int i = 0; i < p.count() && i < most; ++i) owners[i] = p.owner(i);
+    return p.count();
+}
 }
 """
 
@@ -74,23 +81,59 @@ def test_a_packed_sequence_never_leaves_the_rows(bounds):
                 assert not good or (first.value, n) == (c0, c1 - c0)
 
 
-def test_splits_fit_the_slots_and_cover_the_sequences(bounds):
-    """Whatever the lengths: the splits number at most batch + budget (the launch's grid and the
-    workspace's slots), and a sequence's splits cover its tiles."""
+def test_shares_cover_the_sequences_and_their_pieces_have_slots_of_their_own(bounds):
+    """Whatever the lengths: the waves' shares are the whole row of tiles, each once; the pieces that the
+    waves and workgroups make of a sequence are, in order, those that the joining kernel looks for; no
+    two pieces share a slot, and every slot is in the workspace's waves + batch."""
     rng = random.Random(5)
-    for _ in range(2000):
-        batch, budget, unit = rng.randint(1, 80), rng.randint(1, 600), rng.choice([4, 8])
-        top = int(math.exp(rng.uniform(0, math.log(2 ** 30 // 16 // batch))))
-        tiles = [rng.choice([0, 1, top, rng.randint(0, top)]) for _ in range(batch)]
-        chunk = bounds.split(sum(tiles), budget, unit)
-        n = [max(1, -(-t // chunk)) for t in tiles]
-        assert chunk >= unit and chunk % unit == 0
-        assert sum(n) <= batch + budget
-    # the longest sequence (2^30 positions, 2^26 tiles), and as many of them as a call may have
-    for batch in (1, 2 ** 5 - 1):
-        for budget in (1, 2, 500):
-            chunk = bounds.split(batch * 2 ** 26, budget, 4)
-            assert 0 < chunk <= 2 ** 26 and batch * -(-2 ** 26 // chunk) <= batch + budget
+    bounds.first.restype = ctypes.c_uint
+    owners = (ctypes.c_int * 700)()
+    joints = 0
+    for trial in range(1500):
+        batch, waves, unit = rng.randint(1, 60), 4 * rng.randint(1, 150), rng.choice([1, 2])
+        top = int(math.exp(rng.uniform(0, math.log(2 ** 26 // batch))))
+        tiles = [rng.choice([1, 1, top, rng.randint(1, top)]) for _ in range(batch)]
+        if trial % 3 == 0:                               # ends of shares that are ends of sequences
+            tiles = [rng.choice([1, 2, 4, 8, 16]) for _ in range(batch)]
+        total = sum(tiles)
+        c = bounds.share(total, waves, unit)
+        assert c >= unit and waves * c >= total
+        starts = [sum(tiles[:b]) for b in range(batch)]
+        made = [[] for _ in range(batch)]
+        slots = set()
+
+        def piece(x, b, whole):
+            assert x + b not in slots and x + b < waves + batch
+            slots.add(x + b)
+            made[b].append((x, whole))
+
+        for x in range(waves // 4):                      # as the kernel goes through its share
+            at, end = bounds.first(4 * x, c, total), bounds.first(4 * x + 4, c, total)
+            if at >= end:
+                continue
+            b = max(i for i in range(batch) if starts[i] <= at)
+            if bounds.joint(x, starts[b], tiles[b], c, total):
+                assert end <= starts[b] + tiles[b]
+                piece(4 * x, b, end - at == tiles[b])
+                joints += 1
+                continue
+            for w in range(4 * x, 4 * x + 4):
+                at, end = bounds.first(w, c, total), bounds.first(w + 1, c, total)
+                assert end - at <= c
+                while at < end:
+                    b = max(i for i in range(batch) if starts[i] <= at)
+                    stop = min(end, starts[b] + tiles[b])
+                    piece(w, b, stop - at == tiles[b])
+                    at = stop
+        for b in range(batch):
+            n = bounds.pieces(starts[b], tiles[b], c, total, owners, 700)
+            assert [x for x, _ in made[b]] == owners[:n]
+            assert (n == 1) == made[b][0][1]
+    assert joints > 1000
+    # as many tiles as a call may have
+    c = bounds.share(2 ** 31 - 1, 4, 1)
+    assert c == 2 ** 29 and bounds.first(3, c, 2 ** 31 - 1) == 3 * 2 ** 29
+    assert bounds.first(4, c, 2 ** 31 - 1) == bounds.first(2 ** 24, c, 2 ** 31 - 1) == 2 ** 31 - 1
 
 
 # --- the oracle ------------------------------------------------------------------------------------
@@ -169,18 +212,20 @@ def decode(batch, H, **kw):
 
 
 def test_decode_launches_fit_the_workspace(host):  # noqa: F811
-    """The grid's slots are those that the workspace holds, whatever the batch, the heads and the cache;
-    a cache of one split per sequence is not joined."""
+    """Two resident workgroups per CU (256 CUs) at most, and slots for their waves' pieces in the
+    workspace, whatever the batch, the heads and the cache; the joining launch reaches every head of every
+    sequence."""
     got = host(CACHE + """
-result = [[b, h, n, kind, decode(b, h, n_kv=n, kind=kind)] for b in (1, 3, 64, 1000) for h, n in ((40, 8), (4, 4), (33, 1))
-          for kind in (0, 1)]
-result.append([1, 40, 8, 0, decode(1, 40, max_pages=4)])
+result = [[b, h, n, kind, decode(b, h, n_kv=n, kind=kind)] for b in (1, 3, 8, 9, 64, 1000)
+          for h, n in ((40, 8), (4, 4), (33, 1)) for kind in (0, 1)]
 """)
-    for b, h, n, kind, (need, grids) in got[:-1]:
-        (x, y, z, threads), join = grids
-        assert need == x * h * 130 * 4 and x > b and y == n and z == -(-(h // n) // 16) and threads == 256
-        assert join == [b, h, 1, 256]
-    assert len(got[-1][4][1]) == 1
+    for b, h, n, kind, (need, grids) in got:
+        (x, y, z, threads), (jx, jy, jz, jthreads) = grids
+        x -= 1                                          # (one more, for the join's plan)
+        assert need == (4 * x + b) * h * 130 * 4 + 16 * b and y == n and z == -(-(h // n) // 16) and threads == 256
+        assert 512 - y * z < x * y * z <= 512
+        heads = 1 if b <= 8 else min(8, -(-b * h // 2048))
+        assert jx == b and jy == -(-h // heads) and jz == 1 and jthreads == (1024 if b <= 8 else 256)
 
 
 def test_packed_prefill_launches_enough_workgroups(host):  # noqa: F811
