@@ -26,10 +26,11 @@
 // * S^T = K . Q^T (positions x heads) by 16x16x32 products: a lane then holds 4 positions of one head.
 // * weights in base 2 against a running maximum that is raised only when a score exceeds it by 2^8
 //   in weight, so that the sums are rarely rescaled.
-// * O^T += V^T . P^T: the 32 places of the product's inner dimension are the tile's 16 positions
-//   twice, with the weights' hi and lo parts, so one product does both.  V^T comes from the
-//   token-major tile by transposing LDS reads (for e4m3, of pairs of dims, whose bytes are then
-//   sorted: the even dims of a block go to one product, the odd ones to the next).
+// * O^T += V^T . P^T.  V^T comes from the token-major tile by transposing LDS reads.  bf16: the 32 places
+//   of the product's inner dimension are the tile's 16 positions twice, with the weights' hi and lo
+//   parts.  e4m3: the 16 positions of both tiles of a stage, one product for hi, one for lo; the
+//   reads transpose pairs of dims, whose bytes are then sorted: the even dims of a block go to one
+//   product, the odd ones to the next.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 
@@ -322,36 +323,45 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
             m = mn;
         }
         const float mc = m * sc;
+        uint32_t hi[F::kTiles][2], lo[F::kTiles][2];            // the weights of each tile's 4 positions
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) {
             float p[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) p[k] = fexp2(__builtin_fmaf(st[t][k], sc, -mc));
             l += (p[0] + p[1]) + (p[2] + p[3]);
-            const uint32_t h01 = pack_bf16(p[0], p[1]), h23 = pack_bf16(p[2], p[3]);
-            const uint32_t l01 = pack_bf16(p[0] - bf16lo_to_f32(h01), p[1] - bf16hi_to_f32(h01));
-            const uint32_t l23 = pack_bf16(p[2] - bf16lo_to_f32(h23), p[3] - bf16hi_to_f32(h23));
-            const bf16x8 w = __builtin_bit_cast(bf16x8, uint4{h01, h23, l01, l23});
-            if constexpr (E4M3) {
 #pragma unroll
-                for (int b = 0; b < kFrags; ++b) {
-                    // positions 4 g .. + 3 of dims 32 b + 2 l16, + 1 as pairs of codes
-                    const uint2 p2 = vf[t][b];
-                    const uint2 e = e4m3x4_to_bf16(__builtin_amdgcn_perm(p2.y, p2.x, 0x06040200u));
-                    const uint2 o = e4m3x4_to_bf16(__builtin_amdgcn_perm(p2.y, p2.x, 0x07050301u));
-                    oacc[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, uint4{e.x, e.y, e.x, e.y}), w, oacc[2 * b], 0, 0, 0);
-                    oacc[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, uint4{o.x, o.y, o.x, o.y}), w, oacc[2 * b + 1], 0, 0, 0);
-                }
-            } else {
+            for (int k = 0; k < 2; ++k) {
+                hi[t][k] = pack_bf16(p[2 * k], p[2 * k + 1]);
+                lo[t][k] = pack_bf16(p[2 * k] - bf16lo_to_f32(hi[t][k]), p[2 * k + 1] - bf16hi_to_f32(hi[t][k]));
+            }
+        }
+        auto frag = [](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            return __builtin_bit_cast(bf16x8, uint4{a0, a1, a2, a3});
+        };
+        if constexpr (E4M3) {
+            const bf16x8 wh = frag(hi[0][0], hi[0][1], hi[1][0], hi[1][1]);
+            const bf16x8 wl = frag(lo[0][0], lo[0][1], lo[1][0], lo[1][1]);
 #pragma unroll
-                for (int b = 0; b < kFrags; ++b) {
-                    const uint2 p2 = vf[t][b];
-                    oacc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, uint4{p2.x, p2.y, p2.x, p2.y}), w, oacc[b], 0, 0, 0);
+            for (int b = 0; b < kFrags; ++b) {
+                // positions 4 g .. + 3 of dims 32 b + 2 l16, + 1 of both tiles, as pairs of codes
+#pragma unroll
+                for (int odd = 0; odd < 2; ++odd) {
+                    const uint32_t pick = odd ? 0x07050301u : 0x06040200u;
+                    const uint2 x0 = e4m3x4_to_bf16(__builtin_amdgcn_perm(vf[0][b].y, vf[0][b].x, pick));
+                    const uint2 x1 = e4m3x4_to_bf16(__builtin_amdgcn_perm(vf[1][b].y, vf[1][b].x, pick));
+                    const bf16x8 x = frag(x0.x, x0.y, x1.x, x1.y);
+                    f32x4& acc = oacc[2 * b + odd];
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, wh, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, wl, acc, 0, 0, 0);
                 }
             }
+        } else {
+            const bf16x8 w = frag(hi[0][0], hi[0][1], lo[0][0], lo[0][1]);
+#pragma unroll
+            for (int b = 0; b < kFrags; ++b)
+                oacc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    frag(vf[0][b].x, vf[0][b].y, vf[0][b].x, vf[0][b].y), w, oacc[b], 0, 0, 0);
         }
     };
     // A piece's end.  A lane's sums are its head's dims 16 b + 4 g .. + 3 of block b (bf16), or 32 b + 8 g
