@@ -422,7 +422,7 @@ typedef struct nmi_paged_kv {
  * token per sequence, b = t) and has position start_pos[b] + t - cu_seqlens[b] (start_pos int32
  * [batch]; a negative one marks a sequence that is not in use: nothing of it is read or written).
  * Rows outside [cu_seqlens[0], cu_seqlens[batch]) are left alone.
- *   rotation   rotary_dim > 0 (a multiple of 8, at most 128) with inv_freq float32 [rotary_dim / 2]: the
+ *   rotation   rotary_dim > 0 (a multiple of 16, at most 128) with inv_freq float32 [rotary_dim / 2]: the
  *              angle of pair i is position * inv_freq[i], formed in 64 bits; pairs are dims (i, i +
  *              rotary_dim / 2), or (2i, 2i + 1) where interleaved is not 0; (x, y) becomes
  *              (x cos - y sin, x sin + y cos) in float32; dims from rotary_dim on stay.  rotary_dim = 0

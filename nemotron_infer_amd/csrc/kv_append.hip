@@ -7,15 +7,15 @@
 // is: as bf16, or divided by the head's scale and rounded once to e4m3 (values past +-448 saturate,
 // NaN stays).  q and, when asked for, k are also returned rotated, as bf16.
 //
-// The angle is formed in 64 bits, in turns (p * inv_freq / 2 pi) with its whole turns taken off before
-// it is narrowed: at p = 10^6 a float32 angle would be off by 0.03 rad.  sincospi of the rest, the
-// rotation and the division are float32, each output rounded once.
+// The angle is formed in 64 bits, in turns (p * inv_freq / 2 pi) with its whole turns taken off (at
+// p = 10^6 a float32 angle would be off by 0.03 rad), and so are its sine and cosine (cos_sin), each
+// rounded once; the rotation and the division are float32, each output rounded once.
 //
-// Bound: bytes (every vector is read once and written once) for prompts, latency at decode.  One
-// workgroup of 256 threads takes up to 16 head vectors of a token at a time, 16 lanes of 8 dims each:
-// with halves paired a lane holds dims 4s .. + 3 of both halves, so that a pair never leaves its lane.
-// The token's cosines are computed once per workgroup, one per thread, and shared through LDS; the
-// first vectors are on their way meanwhile.
+// Bound: bytes (every vector is read once and written once) for prompts, latency at decode.  A wave
+// takes a token, or a part of its head vectors where there are few tokens: 8 vectors at a time, 8 lanes
+// of two times 8 dims each, BATCH times that on their way at once.  With halves paired a lane
+// holds the same 8 dims of both halves, so that a pair never leaves its lane.  The token's cosines are
+// computed once per wave, one per lane, while the vectors are on their way, and passed on through LDS.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 
@@ -25,46 +25,32 @@ namespace nmi {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRowsPerPass = kThreads / 16;
+constexpr int kWaves = 4;
+constexpr int kBatch = 7;               // of 8 vectors: 40 query and 8 KV heads, k and v, at once
+enum { kPlain = 0, kHalves = 1, kInterleaved = 2 };
 
-// 8 dims of a head vector: quads at d0 and d1
-struct Dims {
-    int d0, d1;
-};
-
-__device__ __forceinline__ void load8(const uint16_t* p, Dims d, float (&x)[8]) {
-    const uint2 lo = *reinterpret_cast<const uint2*>(p + d.d0), hi = *reinterpret_cast<const uint2*>(p + d.d1);
-    x[0] = bf16lo_to_f32(lo.x), x[1] = bf16hi_to_f32(lo.x), x[2] = bf16lo_to_f32(lo.y), x[3] = bf16hi_to_f32(lo.y);
-    x[4] = bf16lo_to_f32(hi.x), x[5] = bf16hi_to_f32(hi.x), x[6] = bf16lo_to_f32(hi.y), x[7] = bf16hi_to_f32(hi.y);
+__device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
+    const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(d[i]), x[2 * i + 1] = bf16hi_to_f32(d[i]);
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return uint4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
 }
 
-__device__ __forceinline__ void store8(uint16_t* p, Dims d, const float (&x)[8]) {
-    *reinterpret_cast<uint2*>(p + d.d0) = uint2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-    *reinterpret_cast<uint2*>(p + d.d1) = uint2{pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-}
-
-// x / s as an e4m3 code: to the nearest (ties to even), saturating
+// x / s as an e4m3 code: to the nearest (ties to even), saturating; NaN stays
 __device__ __forceinline__ float to_e4m3_range(float x, float s) {
     const float y = x / s;
-    return y > 448.f ? 448.f : (y < -448.f ? -448.f : y);      // (NaN stays)
+    return y > 448.f ? 448.f : (y < -448.f ? -448.f : y);
 }
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-}
-
-template <bool E4M3>
-__device__ __forceinline__ void store_cache(uint8_t* p, Dims d, const float (&x)[8], float s) {
-    if constexpr (E4M3) {
-        float y[8];
+__device__ __forceinline__ uint2 pack8_e4m3(const float (&x)[8], float s) {
+    float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = to_e4m3_range(x[i], s);
-        *reinterpret_cast<uint32_t*>(p + d.d0) = pack_e4m3(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint32_t*>(p + d.d1) = pack_e4m3(y[4], y[5], y[6], y[7]);
-    } else {
-        store8(reinterpret_cast<uint16_t*>(p), d, x);
-    }
+    for (int i = 0; i < 8; ++i) y[i] = to_e4m3_range(x[i], s);
+    int a = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), b = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], a, true);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], b, true);
+    return uint2{(uint32_t)a, (uint32_t)b};
 }
 
 // The sequence of packed row t: the number of ends cu[1 ..] at or before it (64 of them at a time).
@@ -78,110 +64,189 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int t, 
     return batch;
 }
 
-template <bool E4M3, bool INTERLEAVED>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(const AppendArgs a) {
-    __shared__ float2 turn[kPagedHead / 2];         // cos, sin of each frequency
-    const int t = blockIdx.x, tid = threadIdx.x;
+// cos and sin of 2 pi f, |f| <= 1/2: f = q / 4 + y with |y| <= 1/8, the Taylor polynomials of y's angle
+// t, |t| <= pi / 4 (left out: t^13 / 13! < 7e-12, t^12 / 12! < 2e-10), turned by q quarters.
+__device__ __forceinline__ float2 cos_sin(double f) {
+    const double q = rint(4.0 * f), t = 6.283185307179586 * __builtin_fma(q, -0.25, f), z = t * t;
+    double s = __builtin_fma(z, -1.0 / 39916800.0, 1.0 / 362880.0), c = __builtin_fma(z, -1.0 / 3628800.0, 1.0 / 40320.0);
+    s = __builtin_fma(z, s, -1.0 / 5040.0);
+    c = __builtin_fma(z, c, -1.0 / 720.0);
+    s = __builtin_fma(z, s, 1.0 / 120.0);
+    c = __builtin_fma(z, c, 1.0 / 24.0);
+    s = __builtin_fma(z, s, -1.0 / 6.0);
+    c = __builtin_fma(z, c, -0.5);
+    const float sf = (float)__builtin_fma(t * z, s, t), cf = (float)__builtin_fma(z, c, 1.0);
+    const int k = (int)q;                                       // -2 .. 2
+    const float cs = (k & 1) ? sf : cf, sn = (k & 1) ? cf : sf;
+    return float2{((k + 1) & 2) ? -cs : cs, (k & 2) ? -sn : sn};
+}
+
+// parts: waves that share a token, BATCH its vectors (by 8) on their way at once.
+template <bool E4M3, int MODE, int BATCH>
+__global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs a, int parts) {
+    __shared__ float2 turns[kWaves][kPagedHead / 2];            // cos, sin of each frequency
+    const int tid = threadIdx.x, lane = tid & 63, sub = lane & 7;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t job = (int64_t)blockIdx.x * kWaves + wave;
+    const int t = (int)(job / parts), part = (int)(job - (int64_t)t * parts);
+    if (t >= a.tokens) return;
+
+    // the lane's two times 8 dims in a vector that is rotated, and in one that is not
+    const int turning = a.rotary / 16;                          // lanes of a vector that rotate (halves)
+    const int p0 = 16 * sub, p1 = p0 + 8;
+    const bool halves = MODE == kHalves && sub < turning;
+    const int r0 = halves ? 8 * sub : p0, r1 = halves ? a.rotary / 2 + 8 * sub : p1;
+
+    const int nq = a.q ? a.H : 0, n_kv = a.kv.n_kv, rows = nq + 2 * n_kv;
+    uint4 lo[BATCH], hi[BATCH];
+    auto load = [&](int pass0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int row = 8 * (pass0 + i * parts) + (lane >> 3);
+            if (row < rows) {
+                const bool is_q = row < nq, is_v = row >= nq + n_kv;
+                const uint16_t* x = is_q   ? a.q + (int64_t)t * a.ldq + row * kPagedHead
+                                    : is_v ? a.v + (int64_t)t * a.ldv + (row - nq - n_kv) * kPagedHead
+                                           : a.k + (int64_t)t * a.ldk + (row - nq) * kPagedHead;
+                lo[i] = load16(x + (is_v ? p0 : r0));
+                hi[i] = load16(x + (is_v ? p1 : r1));
+            }
+        }
+    };
+    load(part);
+
     int b = t, place = 0;
     if (a.cu) {
-        b = __builtin_amdgcn_readfirstlane(sequence_of(a.cu, a.batch, t, tid & 63));
-        if (b >= a.batch) return;                   // rows behind the last sequence
+        b = __builtin_amdgcn_readfirstlane(sequence_of(a.cu, a.batch, t, lane));
+        if (b >= a.batch) return;                               // rows behind the last sequence
         place = t - a.cu[b];
-        if (place < 0) return;                      // rows before the first
+        if (place < 0) return;                                  // rows before the first
     }
     const int start = a.start[b];
-    if (start < 0) return;                          // a sequence that is not in use
+    if (start < 0) return;                                      // a sequence that is not in use
     const int64_t pos = (int64_t)start + place;
 
-    const int sub = tid & 15;
-    const int nq = a.q ? a.H : 0, n_kv = a.kv.n_kv, rows = nq + 2 * n_kv;
-    const int pairs = a.rotary / 8;                 // lanes of a vector that rotate
-    const bool rotates = sub < pairs;
-    // the lane's dims in a vector that is rotated, and in one that is not
-    const Dims plain{8 * sub, 8 * sub + 4};
-    const Dims turned = (rotates && !INTERLEAVED) ? Dims{4 * sub, a.rotary / 2 + 4 * sub} : plain;
-
-    float x[8];
-    int row = blockIdx.y * kRowsPerPass + (tid >> 4);
-    auto load = [&](int r) {
-        if (r < nq) load8(a.q + (int64_t)t * a.ldq + r * kPagedHead, turned, x);
-        else if (r < nq + n_kv) load8(a.k + (int64_t)t * a.ldk + (r - nq) * kPagedHead, turned, x);
-        else load8(a.v + (int64_t)t * a.ldv + (r - nq - n_kv) * kPagedHead, plain, x);
-    };
-    if (row < rows) load(row);
-
-    if (a.rotary) {
-        if (tid < a.rotary / 2) {
-            const double turns = (double)pos * (double)a.inv_freq[tid] * 0.15915494309189535;   // 1 / (2 pi)
-            float s, c;
-            sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-            turn[tid] = float2{c, s};
-        }
-        __syncthreads();
-    }
     // where the token goes; nowhere if the table has no page for it
     uint8_t *kp = nullptr, *vp = nullptr;
     {
         bool bad = false;
         const int64_t entry = pos >> a.kv.page_shift;
         int page = 0;
-        if (entry < a.kv.max_pages) page = checked_page(a.kv.page_table[b * a.kv.table_stride + entry], a.kv.n_pages, &bad);
-        else bad = true;
+        if (entry < a.kv.max_pages)
+            page = checked_page(a.kv.page_table[b * a.kv.table_stride + entry], a.kv.n_pages, &bad);
+        else
+            bad = true;
         if (!bad) {
             const int64_t off = page * a.kv.page_stride + (pos & ((1 << a.kv.page_shift) - 1)) * a.kv.token_stride;
             kp = a.kv.k_pages + off;
             vp = a.kv.v_pages + off;
-        } else if (tid == 0 && a.kv.error) {
+        } else if (lane == 0 && a.kv.error) {
             __hip_atomic_store(a.kv.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
     }
-    while (row < rows) {
-        if (row < nq + n_kv) {
-            if (rotates) {
-                float c[4], s[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 cs = turn[4 * sub + i];
-                    c[i] = cs.x, s[i] = cs.y;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    constexpr int second = INTERLEAVED ? 1 : 4;
-                    const int i0 = INTERLEAVED ? 2 * i : i;
-                    const float u = x[i0], w = x[i0 + second];
-                    x[i0] = u * c[i] - w * s[i];
-                    x[i0 + second] = u * s[i] + w * c[i];
-                }
-            }
-            if (row < nq) {
-                store8(a.q_out + (int64_t)t * a.ldqo + row * kPagedHead, turned, x);
-            } else {
-                const int h = row - nq;
-                if (a.k_out) store8(a.k_out + (int64_t)t * a.ldko + h * kPagedHead, turned, x);
-                if (kp)
-                    store_cache<E4M3>(kp + h * a.kv.head_stride, turned, x, E4M3 && a.kv.k_scale ? a.kv.k_scale[h] : 1.f);
-            }
-        } else if (vp) {
-            const int h = row - nq - n_kv;
-            store_cache<E4M3>(vp + h * a.kv.head_stride, plain, x, E4M3 && a.kv.v_scale ? a.kv.v_scale[h] : 1.f);
+    float c[8], s[8];                                           // of the lane's pairs
+    if constexpr (MODE != kPlain) {
+        if (lane < a.rotary / 2) {
+            const double turn = (double)pos * (double)a.inv_freq[lane] * 0.15915494309189535;   // 1 / (2 pi)
+            turns[wave][lane] = cos_sin(turn - rint(turn));
         }
-        row += kRowsPerPass * gridDim.y;
-        if (row < rows) load(row);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (a wave's own: no barrier)
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 cs = turns[wave][8 * sub + i];         // (of frequencies past the last: not used)
+            c[i] = cs.x, s[i] = cs.y;
+        }
     }
+
+    const int passes = (rows + 7) / 8;
+    for (int pass0 = part;; load(pass0)) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int row = 8 * (pass0 + i * parts) + (lane >> 3);
+            if (row >= rows) continue;
+            const bool is_q = row < nq, is_v = row >= nq + n_kv;
+            float x[8], y[8];
+            unpack8(lo[i], x);
+            unpack8(hi[i], y);
+            if (!is_v) {
+                if constexpr (MODE == kHalves) {
+                    if (halves) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float u = x[j], w = y[j];
+                            x[j] = __builtin_fmaf(u, c[j], -(w * s[j]));
+                            y[j] = __builtin_fmaf(u, s[j], w * c[j]);
+                        }
+                    }
+                } else if constexpr (MODE == kInterleaved) {
+                    if (p0 < a.rotary) {                        // (rotary a multiple of 16: both times 8 dims, or none)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            float(&z)[8] = j < 4 ? x : y;       // (j is known here: no choice is left)
+                            const int e = 2 * (j & 3);
+                            const float u = z[e], w = z[e + 1];
+                            z[e] = __builtin_fmaf(u, c[j], -(w * s[j]));
+                            z[e + 1] = __builtin_fmaf(u, s[j], w * c[j]);
+                        }
+                    }
+                }
+            }
+            const uint4 xb = pack8(x), yb = pack8(y);
+            if (MODE != kPlain && is_q) {
+                uint16_t* o = a.q_out + (int64_t)t * a.ldqo + row * kPagedHead;
+                *reinterpret_cast<uint4*>(o + r0) = xb;
+                *reinterpret_cast<uint4*>(o + r1) = yb;
+                continue;
+            }
+            const int h = is_v ? row - nq - n_kv : row - nq;
+            const int d0 = is_v ? p0 : r0, d1 = is_v ? p1 : r1;
+            if (MODE != kPlain && !is_v && a.k_out) {
+                uint16_t* o = a.k_out + (int64_t)t * a.ldko + h * kPagedHead;
+                *reinterpret_cast<uint4*>(o + d0) = xb;
+                *reinterpret_cast<uint4*>(o + d1) = yb;
+            }
+            uint8_t* p = is_v ? vp : kp;
+            if (!p) continue;
+            p += h * a.kv.head_stride;
+            if constexpr (E4M3) {
+                const float* scale = is_v ? a.kv.v_scale : a.kv.k_scale;
+                const float sc = scale ? scale[h] : 1.f;
+                *reinterpret_cast<uint2*>(p + d0) = pack8_e4m3(x, sc);
+                *reinterpret_cast<uint2*>(p + d1) = pack8_e4m3(y, sc);
+            } else {
+                *reinterpret_cast<uint4*>(p + 2 * d0) = xb;
+                *reinterpret_cast<uint4*>(p + 2 * d1) = yb;
+            }
+        }
+        pass0 += BATCH * parts;
+        if (pass0 >= passes) break;
+    }
+}
+
+template <bool E4M3, int BATCH>
+void launch(const AppendArgs& a, int parts, hipStream_t stream) {
+    const dim3 grid((uint32_t)(((int64_t)a.tokens * parts + kWaves - 1) / kWaves)), block(64 * kWaves);
+    if (!a.rotary) hipLaunchKernelGGL((kv_append_kernel<E4M3, kPlain, BATCH>), grid, block, 0, stream, a, parts);
+    else if (!a.interleaved) hipLaunchKernelGGL((kv_append_kernel<E4M3, kHalves, BATCH>), grid, block, 0, stream, a, parts);
+    else hipLaunchKernelGGL((kv_append_kernel<E4M3, kInterleaved, BATCH>), grid, block, 0, stream, a, parts);
 }
 
 }  // namespace
 
 hipError_t launch_kv_append(const AppendArgs& a, bool e4m3, hipStream_t stream) {
-    const int rows = (a.q ? a.H : 0) + 2 * a.kv.n_kv;
-    const int passes = (rows + kRowsPerPass - 1) / kRowsPerPass;
-    const dim3 grid(a.tokens, passes);
-    if (e4m3) {
-        if (a.interleaved) hipLaunchKernelGGL((kv_append_kernel<true, true>), grid, dim3(kThreads), 0, stream, a);
-        else hipLaunchKernelGGL((kv_append_kernel<true, false>), grid, dim3(kThreads), 0, stream, a);
+    // Few tokens: their vectors spread over up to 8 waves per CU, since latency is all there is; many: a
+    // wave for a token, whose cosines are then computed once.  Parts 1 / 2 / 4 / 7 (40 / 8 heads, rotated,
+    // bf16): 128 tokens 6.7 / 5.2 / 4.6 / 4.2 us, 512 7.8 / 6.7 / 6.3 / 7.5, 1024 11.0 / 10.2 / 11.1 / 11.9,
+    // 2048 14.4 / 15.9 / 16.3 / 18.5, 8191 51 / 49 / 55 / 67.
+    const int passes = ((a.q ? a.H : 0) + 2 * a.kv.n_kv + 7) / 8;
+    const int parts = std::min(passes, std::max(1, 8 * device_info().num_cu / a.tokens));
+    if (parts == passes) {
+        if (e4m3) launch<true, 1>(a, parts, stream);
+        else launch<false, 1>(a, parts, stream);
     } else {
-        if (a.interleaved) hipLaunchKernelGGL((kv_append_kernel<false, true>), grid, dim3(kThreads), 0, stream, a);
-        else hipLaunchKernelGGL((kv_append_kernel<false, false>), grid, dim3(kThreads), 0, stream, a);
+        if (e4m3) launch<true, kBatch>(a, parts, stream);
+        else launch<false, kBatch>(a, parts, stream);
     }
     return hipGetLastError();
 }

@@ -102,9 +102,9 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
                       "%s: batch=%d tokens=%d (need both >= 1, less than 2^24 tokens, and as many as sequences where "
                       "cu_seqlens is NULL)",
                       fn, batch, tokens);
-    if (rotary_dim < 0 || rotary_dim > kPagedHead || rotary_dim % 8 || (rotary_dim > 0) != (inv_freq != nullptr))
+    if (rotary_dim < 0 || rotary_dim > kPagedHead || rotary_dim % 16 || (rotary_dim > 0) != (inv_freq != nullptr))
         return refuse(NMI_ERR_INVALID_ARG,
-                      "%s: rotary_dim=%d (need a multiple of 8 up to %d, with inv_freq, or 0 without)", fn, rotary_dim,
+                      "%s: rotary_dim=%d (need a multiple of 16 up to %d, with inv_freq, or 0 without)", fn, rotary_dim,
                       kPagedHead);
     if ((q_bf16 != nullptr) != (q_out_bf16 != nullptr) || ((q_bf16 || k_out_bf16) && !rotary_dim))
         return refuse(NMI_ERR_INVALID_ARG,

@@ -221,7 +221,6 @@ result = [[b, h, n, kind, decode(b, h, n_kv=n, kind=kind)] for b in (1, 3, 8, 9,
 """)
     for b, h, n, kind, (need, grids) in got:
         (x, y, z, threads), (jx, jy, jz, jthreads) = grids
-        x -= 1                                          # (one more, for the join's plan)
         assert need == (4 * x + b) * h * 130 * 4 + 16 * b and y == n and z == -(-(h // n) // 16) and threads == 256
         assert 512 - y * z < x * y * z <= 512
         heads = 1 if b <= 8 else min(8, -(-b * h // 2048))
@@ -298,8 +297,8 @@ def test_bad_caches_are_refused(change, code):
     (dict(k=0), _lib.NMI_ERR_INVALID_ARG), (dict(v=0), _lib.NMI_ERR_INVALID_ARG), (dict(start=0), _lib.NMI_ERR_INVALID_ARG),
     (dict(batch=0), _lib.NMI_ERR_INVALID_ARG), (dict(tokens=0), _lib.NMI_ERR_INVALID_ARG),
     (dict(cu=0), _lib.NMI_ERR_INVALID_ARG),                                  # 9 tokens of 2 sequences
-    (dict(rotary=-8), _lib.NMI_ERR_INVALID_ARG), (dict(rotary=60), _lib.NMI_ERR_INVALID_ARG),
-    (dict(rotary=136), _lib.NMI_ERR_INVALID_ARG), (dict(rotary=0), _lib.NMI_ERR_INVALID_ARG),
+    (dict(rotary=-16), _lib.NMI_ERR_INVALID_ARG), (dict(rotary=72), _lib.NMI_ERR_INVALID_ARG),
+    (dict(rotary=144), _lib.NMI_ERR_INVALID_ARG), (dict(rotary=0), _lib.NMI_ERR_INVALID_ARG),
     (dict(inv=0), _lib.NMI_ERR_INVALID_ARG), (dict(q=0), _lib.NMI_ERR_INVALID_ARG), (dict(qo=0), _lib.NMI_ERR_INVALID_ARG),
     (dict(q=0, qo=0, rotary=0, inv=0), _lib.NMI_ERR_INVALID_ARG),           # k_out without a rotation
     (dict(H=41), _lib.NMI_ERR_INVALID_ARG), (dict(H=0), _lib.NMI_ERR_INVALID_ARG),

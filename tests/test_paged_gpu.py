@@ -7,9 +7,9 @@ Bars (derived before the first run):
   rounding (2^-24 per operation, sums of at most some thousand terms) and the softmax weights' 16 bits
   (2^-17 each), far below half a bf16 step (2^-9): a value moves to the neighbouring bf16 only from
   next to a border.
-* rotation: |kernel - exact| <= d = (|x| + |y|) 2^-20 before rounding (x, y the pair): the angle is off
-  by at most 2^-24 turns half = 1.9e-7 and sincospi by 2 ulp = 1.2e-7, 3.1e-7 < 2^-21 on each of the
-  two terms, their products and sum 3 * 2^-24.  Rounding is monotone, so the output must lie between
+* rotation: |kernel - exact| <= d = (|x| + |y|) 2^-20 before rounding (x, y the pair): a float32 angle
+  would be off by at most 2^-24 turns half = 1.9e-7 and its sine by 2 ulp = 1.2e-7, 3.1e-7 < 2^-21 on
+  each of the two terms (the kernel's are better), their products and sum 3 * 2^-24.  Rounding is monotone, so the output must lie between
   the rounded ends of [exact - d, exact + d].  For e4m3 the same with the division's 2^-24 and the
   scale: d / s + |exact / s| 2^-22.
 * what is not rotated and not scaled is copied: bit for bit; what is not addressed stays bit for bit.
@@ -348,7 +348,7 @@ def _check_append(rng, starts, lens, H, n_kv, page, kind, rotary, interleaved, w
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
-@pytest.mark.parametrize("rotary,interleaved", [(0, False), (128, False), (128, True), (64, False), (8, True), (104, False)])
+@pytest.mark.parametrize("rotary,interleaved", [(0, False), (128, False), (128, True), (64, False), (16, True), (112, False), (96, True)])
 def test_append_prompts(kind, rotary, interleaved):
     announce("append", kind, rotary, interleaved)
     rng = np.random.default_rng(rotary)
@@ -420,7 +420,7 @@ def test_append_bad_places_are_skipped_and_reported():
     """A position past the table or a page outside the pool: that token is not stored, its rotated q is
     still right, the others are stored, and NMI_ERR_ASYNC says so once."""
     rng = np.random.default_rng(22)
-    f = _dev(np.ones(4, np.float32))
+    f = _dev(np.ones(8, np.float32))
     for table, starts in (([[0], [-1], [1]], [3, 4, 5]), ([[0], [2], [1]], [3, 4, 5]), ([[0], [0], [1]], [3, 16, 5]),
                           ([[0], [0], [1]], [3, 2 ** 31 - 1, 5])):
         announce("append_bad", table, starts)
