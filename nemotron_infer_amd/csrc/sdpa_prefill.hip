@@ -164,15 +164,24 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
         }
         if (g >= total) return;                                 // the grid holds the most tiles there could be
     }
-    const int n2 = min(2 * a.nslot, total);
-    const int rank = (g >= a.nslot && g < n2) ? a.nslot + (n2 - 1 - g) : g;
-    const int head = rank - rank / a.H * a.H;
-    const int kvh = head / (a.H / a.H_KV);
-    int qt = a.qtiles - 1 - rank / a.H, S = a.S, row0 = 0;
+    int head, qt, S = a.S, row0 = 0;
     if constexpr (PACKED) {
-        qt = packed_find(a, nt0, first0, len0, rank / a.H, lane, &row0, &S);
+        // As below, but within each of the 8 dies by itself where the heads divide by them (workgroups go
+        // to the dies in turn): a die then has the query heads that share KV heads, and its L2 their K and V
+        const int dies = a.H % 8 == 0 ? 8 : 1, heads = a.H / dies;
+        const int die = g % dies, at = g / dies, slots = a.nslot / dies;
+        const int n2 = min(2 * slots, total / dies);
+        const int rank = (at >= slots && at < n2) ? slots + (n2 - 1 - at) : at;
+        head = die * heads + rank % heads;
+        qt = packed_find(a, nt0, first0, len0, rank / heads, lane, &row0, &S);
         if (qt * kBQ >= S) return;                              // (only if cu changes under the launch)
+    } else {
+        const int n2 = min(2 * a.nslot, total);
+        const int rank = (g >= a.nslot && g < n2) ? a.nslot + (n2 - 1 - g) : g;
+        qt = a.qtiles - 1 - rank / a.H;
+        head = rank - rank / a.H * a.H;
     }
+    const int kvh = head / (a.H / a.H_KV);
     const int q0 = qt * kBQ;
     const int qw = q0 + 32 * wave;                              // the wave's first query row
     const int qrow = qw + l32;                                  // this lane's query (B operand column)
