@@ -489,16 +489,20 @@ def test_prefill_heads_scales_and_peaks():
     _check_prefill(rng, [150, 40], 4, 2, scale=0.3)
 
 
-def test_prefill_equals_the_single_prompt_operator():
-    """A packed prompt gets the bytes that nmi_sdpa_prefill_bf16 gives it alone: the same kernel body."""
-    announce("packed_vs_single")
+@pytest.mark.parametrize("H,n_kv", [(16, 4), (40, 8), (16, 2), (48, 16), (8, 8), (32, 1), (40, 4), (10, 2), (7, 1)])
+def test_prefill_equals_the_single_prompt_operator(H, n_kv):
+    """A packed prompt gets the bytes that nmi_sdpa_prefill_bf16 gives it alone, whichever heads its last
+    rows share a workgroup with: the same kernel body."""
+    announce("packed_vs_single", H, n_kv)
     rng = np.random.default_rng(32)
-    H, n_kv, lens = 16, 4, [300, 1, 1000, 129]
+    lens = [300, 1, 1000, 129, 32, 33, 64, 65, 160, 0, 161, 192, 193, 31]
     T = sum(lens)
     q, k, v = _dev(_rand_bits(rng, T, H * 128)), _dev(_rand_bits(rng, T, n_kv * 128)), _dev(_rand_bits(rng, T, n_kv * 128))
     cu = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
     got = ops.sdpa_prefill_packed_bf16(q, k, v, _dev(cu), H, n_kv)
     for a, b in zip(cu, cu[1:]):
+        if a == b:
+            continue
         one = ops.sdpa_prefill_bf16(q[a:b].contiguous(), k[a:b].contiguous(), v[a:b].contiguous(), H, n_kv)
         assert torch.equal(got[a:b].view(torch.int16), one.view(torch.int16)), (a, b)
 
