@@ -151,6 +151,26 @@ __device__ __forceinline__ Tile packed_find(const PrefillArgs& a, Lanes v, int r
     }
 }
 
+// One row of a packed sequence (its first row row0) by one wave, key by key in float32, two dims a lane.
+__device__ __forceinline__ void packed_row(const PrefillArgs& a, int row0, int row, int head, int kvh, int lane) {
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(a.q + (int64_t)(row0 + row) * a.ldq + head * kD + 2 * lane);
+    const uint16_t* k = a.k + row0 * a.ldk + kvh * kD + 2 * lane;
+    const uint16_t* v = a.v + row0 * a.ldv + kvh * kD + 2 * lane;
+    const float q0 = bf16lo_to_f32(q) * a.scale2, q1 = bf16hi_to_f32(q) * a.scale2;
+    float m = -FLT_MAX, l = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int t = 0; t <= row; ++t) {
+        const uint32_t kt = *reinterpret_cast<const uint32_t*>(k + t * a.ldk);
+        const uint32_t vt = *reinterpret_cast<const uint32_t*>(v + t * a.ldv);
+        const float s = wave_sum(__builtin_fmaf(q0, bf16lo_to_f32(kt), q1 * bf16hi_to_f32(kt)));
+        const float mn = fmaxf(m, s), c = fexp2(m - mn), p = fexp2(s - mn);
+        l = __builtin_fmaf(l, c, p);
+        o0 = __builtin_fmaf(o0, c, p * bf16lo_to_f32(vt));
+        o1 = __builtin_fmaf(o1, c, p * bf16hi_to_f32(vt));
+        m = mn;
+    }
+    *reinterpret_cast<uint32_t*>(a.o + (int64_t)(row0 + row) * a.ldo + head * kD + 2 * lane) = pack_bf16(o0 / l, o1 / l);
+}
+
 template <bool PACKED>
 __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs a) {
     typedef __attribute__((address_space(3))) void lds_void;
@@ -564,6 +584,21 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
         finish(std::false_type{}, sb, wa, wb, vstage(t) + 4096 * j0, 0);
     }
     l += __shfl_xor(l, 32);
+    if constexpr (PACKED) {
+        // A value of v that is not finite reaches all rows of its block through the products, the rows before
+        // it too (0 * NaN): such a wave's rows once more, one by one.
+        f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[b] += oacc[b][r];
+        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (__builtin_amdgcn_ballot_w64(!(fabsf(all) < INFINITY) && qrow < S)) {
+            for (int row = qw; row < min(qw + 32, S); ++row)
+                packed_row(a, row0, row, head, kvh, lane);
+            return;
+        }
+    }
 
     // O = O^T / l: register r of block b is dim 32 b + 8 (r / 4) + 4 h + r % 4 of query qrow
     if (qrow < S) {

@@ -80,8 +80,14 @@ def prefill(q: np.ndarray, k: np.ndarray, v: np.ndarray, cu, scale=HEAD ** -0.5)
             e = scale * (q[s, h] @ k[s, h * n_kv // H].T)
             e[np.triu_indices(n, 1)] = -np.inf
             if n:
-                w = np.exp(e - e.max(axis=1, keepdims=True))
-                out[s, h] = (w @ v[s, h * n_kv // H]) / w.sum(axis=1, keepdims=True)
+                vh = v[s, h * n_kv // H]
+                if np.isfinite(vh).all() and np.isfinite(k[s, h * n_kv // H]).all():
+                    w = np.exp(e - e.max(axis=1, keepdims=True))
+                    out[s, h] = (w @ vh) / w.sum(axis=1, keepdims=True)
+                    continue
+                for i in range(n):              # a row takes no part in the keys after it (0 * NaN is NaN)
+                    w = np.exp(e[i, :i + 1] - e[i, :i + 1].max())
+                    out[s.start + i, h] = (w @ vh[:i + 1]) / w.sum()
     return out
 
 

@@ -507,6 +507,34 @@ def test_prefill_equals_the_single_prompt_operator(H, n_kv):
         assert torch.equal(got[a:b].view(torch.int16), one.view(torch.int16)), (a, b)
 
 
+@pytest.mark.parametrize("bad", [NAN_BF16, 0x7F80, 0xFF80])
+def test_prefill_values_that_are_not_finite_stay_with_the_rows_that_see_them(bad):
+    """NaN or an infinity in k and v of some keys: the rows before them, and the other prompts, as without."""
+    announce("packed_not_finite", hex(bad))
+    rng = np.random.default_rng(34)
+    H, n_kv, lens = 10, 2, [200, 40, 33, 300]
+    T, cu = sum(lens), np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    q, k, v = (_rand_bits(rng, T, n * 128) for n in (H, n_kv, n_kv))
+    for at in ([199], [77, 150], [200 + 17], [273 + 128]):
+        k2, v2 = k.copy(), v.copy()
+        for t in at:
+            v2[t, rng.integers(0, 128, 5)] = bad                # some dims of KV head 0
+            k2[t, 128:] = bad                                   # all of KV head 1
+        o = ops.sdpa_prefill_packed_bf16(_dev(q), _dev(k2), _dev(v2), _dev(cu), H, n_kv)
+        torch.cuda.synchronize()
+        with np.errstate(all="ignore"):
+            want = paged.prefill(_f64(q).reshape(T, H, 128), _f64(k2).reshape(T, n_kv, 128), _f64(v2).reshape(T, n_kv, 128), cu)
+        got = _f64(bits(o)).reshape(T, H, 128)
+        seen = np.zeros(T, bool)
+        for t in at:
+            seen[t:cu[np.searchsorted(cu, t, side="right")]] = True
+        # (an infinite weight or one that underflows times an infinity may be NaN on one side: not finite on both)
+        assert np.array_equal(np.isfinite(got[:, :5]), np.isfinite(want[:, :5]))
+        assert np.isfinite(got[~seen]).all()
+        clean = np.isfinite(got) & np.isfinite(want)
+        assert_parity(bits(o).reshape(T, H, 128)[clean], block.bf16_round_exact(want[clean]), f"not finite at {at}")
+
+
 def test_prefill_bad_offsets_are_cut_and_reported():
     """Offsets that fall, or leave the rows: nothing outside the rows is touched, and NMI_ERR_ASYNC."""
     rng = np.random.default_rng(33)
