@@ -162,6 +162,20 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
     v = dpp_add_u32<0x143, 0xC>(v);     // rows 0 and 1's to rows 2 and 3
     return v;
 }
+// The largest of the 64 lanes' values, for all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    v = dpp_max_u32<0x111, 0xF>(v);
+    v = dpp_max_u32<0x112, 0xF>(v);
+    v = dpp_max_u32<0x114, 0xF>(v);
+    v = dpp_max_u32<0x118, 0xF>(v);
+    v = dpp_max_u32<0x142, 0xA>(v);
+    v = dpp_max_u32<0x143, 0xC>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ uint32_t lane_u32(uint32_t v, int lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }

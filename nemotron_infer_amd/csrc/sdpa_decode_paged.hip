@@ -77,6 +77,12 @@ __device__ __forceinline__ Lanes load_lanes(const PagedDecodeArgs& a, int b0, ui
     return v;
 }
 
+__device__ __forceinline__ uint32_t tiles_at(const PagedDecodeArgs& a, int b) {
+    bool bad = false;
+    const int len = a.lens[min(b, a.batch - 1)];
+    return b < a.batch ? (uint32_t)(checked_len(len, a.kv.max_pages, a.kv.page_shift, &bad) + kPagedTile - 1) / kPagedTile : 0u;
+}
+
 typedef short v4i16 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 
@@ -119,8 +125,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
     // this wave's tiles, and the sequence that they begin in
     Lanes v = load_lanes(a, 0, 0, lane);
     uint32_t total = lane_u32(v.upto, 63);
-    if constexpr (MANY)
-        for (int b0 = 64; b0 < a.batch; b0 += 64) total = lane_u32(load_lanes(a, b0, total, lane).upto, 63);
+    if constexpr (MANY) {
+        uint32_t tiles = v.tiles;
+        for (int b0 = 64; b0 < a.batch; b0 += 4 * 64)           // (lengths of four times 64 on their way at once)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tiles += tiles_at(a, b0 + 64 * c + lane);
+        total = lane_u32(wave_scan_u32(tiles), 63);
+    }
     const int c = range_tiles(total, a.waves, F::kTiles);
     if (me + 1 == (uint32_t)a.waves && kvh == 0 && r0 == 0) {
         // for the joining kernel (the last wave: the first to have no tiles)

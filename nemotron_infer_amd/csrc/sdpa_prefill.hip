@@ -100,55 +100,78 @@ typedef __attribute__((address_space(3))) v4i16 lds_v4i16;
 // the heads divide by the 8 dies, each die has heads of its own (workgroups go to the dies in turn), so
 // that its L2 holds the K and V of few KV heads (12 of up to 700: 44.8 -> 42.6; 4 of 1000: 86.8 -> 83.6).
 
-// 64 sequences in the lanes: their rows, their tiles, and the workgroups of a die for the last tile.
-struct Lanes {
+// A sequence: its rows, its tiles, and the workgroups of a die for the last tile.
+struct Seq {
     int first, len, tiles, last;
     bool bad;
 };
-__device__ __forceinline__ Lanes packed_lanes(const PrefillArgs& a, int b) {
-    Lanes v{0, 0, 0, 0, false};
+__device__ __forceinline__ Seq packed_seq(const PrefillArgs& a, int b) {
+    Seq v{0, 0, 0, 0, false};
     if (b < a.batch) v.len = checked_span(a.cu[b], a.cu[b + 1], a.S, &v.first, &v.bad);
     v.tiles = (v.len + kBQ - 1) / kBQ;
     const int rows = v.len - (v.tiles - 1) * kBQ;
     v.last = v.tiles == 0 ? 0 : rows > 64 ? a.wgs4 : rows > 32 ? a.wgs2 : a.wgs1;
     return v;
 }
-// A die's workgroups for all sequences' tiles from number x on, of each sequence; with the first 64
-// sequences at hand.
-__device__ __forceinline__ int packed_from(const PrefillArgs& a, const Lanes& v, int x, int lane) {
-    auto of = [&](const Lanes& w) {
-        return (uint32_t)(w.tiles > x ? (w.tiles - 1 - x) * a.wgs4 + w.last : 0);
-    };
-    uint32_t n = lane_u32(wave_scan_u32(of(v)), 63);
-    for (int b0 = 64; b0 < a.batch; b0 += 64) n += lane_u32(wave_scan_u32(of(packed_lanes(a, b0 + lane))), 63);
-    return (int)n;
+// A die's workgroups for a sequence's tiles from number x on.
+__device__ __forceinline__ uint32_t packed_from(const PrefillArgs& a, const Seq& v, int x) {
+    return v.tiles > x ? (uint32_t)((v.tiles - 1 - x) * a.wgs4 + v.last) : 0u;
 }
-// A die's workgroup `rank`, longest tiles (the latest in their sequences) first: the tile's number in its
-// sequence, that sequence's rows, and which of the tile's workgroups it is.  Every wave finds it by
-// itself: a binary search for the tile number, then a scan over the sequences that have such a tile.
+// The sequences, one in each lane: the first 4 times 64 stay at hand, further ones are read again.
+constexpr int kAtHand = 4;
+struct Seqs {
+    Seq s[kAtHand];
+};
+template <class F>
+__device__ __forceinline__ void packed_each(const PrefillArgs& a, const Seqs& v, int lane, F&& f) {
+#pragma unroll
+    for (int c = 0; c < kAtHand; ++c)
+        if (c == 0 || 64 * c < a.batch) f(v.s[c]);
+    for (int b0 = 64 * kAtHand; b0 < a.batch; b0 += 64 * kAtHand) {
+        Seq s[kAtHand];                                         // (their offsets on their way at once)
+#pragma unroll
+        for (int c = 0; c < kAtHand; ++c) s[c] = packed_seq(a, b0 + 64 * c + lane);
+#pragma unroll
+        for (int c = 0; c < kAtHand; ++c) f(s[c]);
+    }
+}
+__device__ __forceinline__ int packed_from(const PrefillArgs& a, const Seqs& v, int x, int lane) {
+    uint32_t n = 0;
+    packed_each(a, v, lane, [&](const Seq& w) { n += packed_from(a, w, x); });
+    return (int)lane_u32(wave_scan_u32(n), 63);
+}
+// A die's workgroup `rank`, longest tiles (the latest in their sequences, of `most` in the longest one)
+// first: the tile's number in its sequence, that sequence's rows, and which of the tile's workgroups it
+// is.  Every wave finds it by itself: a binary search for the tile number, then a scan over the
+// sequences that have such a tile.
 struct Tile {
     int number, first, len, part;
 };
-__device__ __forceinline__ Tile packed_find(const PrefillArgs& a, Lanes v, int rank, int lane) {
-    int lo = 0, hi = (a.S + kBQ - 1) / kBQ;                     // tiles from lo on: more than rank; from hi: not
+__device__ __forceinline__ Tile packed_find(const PrefillArgs& a, const Seqs& v, int most, int rank, int lane) {
+    int lo = 0, hi = most;                                      // tiles from lo on: more than rank; from hi: not
     while (hi - lo > 1) {
         const int x = (lo + hi) / 2;
         if (packed_from(a, v, x, lane) > rank) lo = x;
         else hi = x;
     }
-    int j = rank - packed_from(a, v, lo + 1, lane);
-    for (int b0 = 0;; b0 += 64) {
-        if (b0) v = packed_lanes(a, b0 + lane);
-        const uint32_t n = v.tiles <= lo ? 0 : v.tiles == lo + 1 ? v.last : a.wgs4;
+    int j = lo + 1 < most ? rank - packed_from(a, v, lo + 1, lane) : rank;
+    Tile tile{lo, 0, 0, 0};
+    bool found = false;
+    packed_each(a, v, lane, [&](const Seq& w) {
+        if (found) return;
+        const uint32_t n = w.tiles <= lo ? 0 : w.tiles == lo + 1 ? w.last : a.wgs4;
         const uint32_t upto = wave_scan_u32(n);
         const int all = (int)lane_u32(upto, 63);
-        if (j < all || b0 + 64 >= a.batch) {
-            const int i = min(63, __popcll(__builtin_amdgcn_ballot_w64(upto <= (uint32_t)j)));
-            return Tile{lo, __builtin_amdgcn_readlane(v.first, i), __builtin_amdgcn_readlane(v.len, i),
-                        j - (int)(lane_u32(upto, i) - lane_u32(n, i))};
+        if (j < all) {
+            const int i = __popcll(__builtin_amdgcn_ballot_w64(upto <= (uint32_t)j));
+            tile.first = __builtin_amdgcn_readlane(w.first, i);
+            tile.len = __builtin_amdgcn_readlane(w.len, i);
+            tile.part = j - (int)(lane_u32(upto, i) - lane_u32(n, i));
+            found = true;
         }
         j -= all;
-    }
+    });
+    return tile;
 }
 
 // One row of a packed sequence (its first row row0) by one wave, key by key in float32, two dims a lane.
@@ -158,14 +181,32 @@ __device__ __forceinline__ void packed_row(const PrefillArgs& a, int row0, int r
     const uint16_t* v = a.v + row0 * a.ldv + kvh * kD + 2 * lane;
     const float q0 = bf16lo_to_f32(q) * a.scale2, q1 = bf16hi_to_f32(q) * a.scale2;
     float m = -FLT_MAX, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int t = 0; t <= row; ++t) {
-        const uint32_t kt = *reinterpret_cast<const uint32_t*>(k + t * a.ldk);
-        const uint32_t vt = *reinterpret_cast<const uint32_t*>(v + t * a.ldv);
-        const float s = wave_sum(__builtin_fmaf(q0, bf16lo_to_f32(kt), q1 * bf16hi_to_f32(kt)));
-        const float mn = fmaxf(m, s), c = fexp2(m - mn), p = fexp2(s - mn);
-        l = __builtin_fmaf(l, c, p);
-        o0 = __builtin_fmaf(o0, c, p * bf16lo_to_f32(vt));
-        o1 = __builtin_fmaf(o1, c, p * bf16hi_to_f32(vt));
+    constexpr int kAtOnce = 8;
+    for (int t0 = 0; t0 <= row; t0 += kAtOnce) {
+        uint32_t kt[kAtOnce], vt[kAtOnce];
+        float s[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int t = min(t0 + i, row);
+            kt[i] = *reinterpret_cast<const uint32_t*>(k + t * a.ldk);
+            vt[i] = *reinterpret_cast<const uint32_t*>(v + t * a.ldv);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            s[i] = wave_sum(__builtin_fmaf(q0, bf16lo_to_f32(kt[i]), q1 * bf16hi_to_f32(kt[i])));
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) mn = fmaxf(mn, s[i]);     // (past the row: the last one's again)
+        const float c = fexp2(m - mn);
+        l *= c, o0 *= c, o1 *= c;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (t0 + i > row) continue;
+            const float p = fexp2(s[i] - mn);
+            l += p;
+            o0 = __builtin_fmaf(p, bf16lo_to_f32(vt[i]), o0);
+            o1 = __builtin_fmaf(p, bf16hi_to_f32(vt[i]), o1);
+        }
         m = mn;
     }
     *reinterpret_cast<uint32_t*>(a.o + (int64_t)(row0 + row) * a.ldo + head * kD + 2 * lane) = pack_bf16(o0 / l, o1 / l);
@@ -186,17 +227,22 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
     const int g = (int)blockIdx.x;
     int qt, kvh, head, waves = 4, S = a.S, row0 = 0;            // waves: per head
     if constexpr (PACKED) {
-        Lanes v = packed_lanes(a, lane);
-        const int total = packed_from(a, v, 0, lane);       // of a die, each the same
-        if (g == 0 && wave == 0 && a.error) {
-            bool bad = v.bad;
-            for (int b0 = 64; b0 < a.batch; b0 += 64) bad |= packed_lanes(a, b0 + lane).bad;
-            if (bad) __hip_atomic_store(a.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-        }
+        Seqs v;
+#pragma unroll
+        for (int c = 0; c < kAtHand; ++c) v.s[c] = c == 0 || 64 * c < a.batch ? packed_seq(a, 64 * c + lane) : Seq{};
+        uint32_t from = 0, most = 0, bad = 0;
+        packed_each(a, v, lane, [&](const Seq& w) {
+            from += packed_from(a, w, 0);
+            most = max(most, (uint32_t)w.tiles);
+            bad |= w.bad;
+        });
+        const int total = (int)lane_u32(wave_scan_u32(from), 63);       // of a die, each the same
+        if (g == 0 && wave == 0 && a.error && bad)
+            __hip_atomic_store(a.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         const int die = g & ((1 << a.die_shift) - 1), at = g >> a.die_shift, slots = a.nslot >> a.die_shift;
         if (at >= total) return;                                // the grid holds the most there could be
         const int n2 = min(2 * slots, total);
-        const Tile tile = packed_find(a, v, (at >= slots && at < n2) ? slots + (n2 - 1 - at) : at, lane);
+        const Tile tile = packed_find(a, v, (int)wave_max_u32(most), (at >= slots && at < n2) ? slots + (n2 - 1 - at) : at, lane);
         qt = tile.number, S = tile.len, row0 = tile.first;
         if (qt * kBQ >= S) return;                              // (only if cu changes under the launch)
         const int rows = S - qt * kBQ;
@@ -618,14 +664,14 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
 }  // namespace
 
 template <bool PACKED>
-static hipError_t launch(PrefillArgs a, int64_t tiles, hipStream_t stream) {
+static hipError_t launch(PrefillArgs a, int64_t wgs, hipStream_t stream) {
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_prefill_kernel<PACKED>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return attr;
     a.qtiles = (a.S + kBQ - 1) / kBQ;
     a.nslot = device_info().num_cu;
     a.lazy = kLazy / a.scale2;
-    hipLaunchKernelGGL(sdpa_prefill_kernel<PACKED>, dim3((uint32_t)(tiles * a.H)), dim3(256), kLds, stream, a);
+    hipLaunchKernelGGL(sdpa_prefill_kernel<PACKED>, dim3((uint32_t)wgs), dim3(256), kLds, stream, a);
     return hipGetLastError();
 }
 
@@ -648,7 +694,7 @@ hipError_t launch_sdpa_prefill(const uint16_t* q, int64_t ldq, const uint16_t* k
     a.k_cache = k_cache;
     a.v_cache = v_cache;
     a.cap = cap;
-    return launch<false>(a, (S + kBQ - 1) / kBQ, stream);
+    return launch<false>(a, (int64_t)((S + kBQ - 1) / kBQ) * H, stream);
 }
 
 int64_t sdpa_prefill_packed_tiles(int tokens, int batch) { return (int64_t)(tokens / kBQ) + std::min(batch, tokens); }
@@ -685,7 +731,13 @@ hipError_t launch_sdpa_prefill_packed(const uint16_t* q, int64_t ldq, const uint
         a.wgs2 = a.per_die / a.run * ((a.run + 1) / 2);
         a.wgs1 = a.per_die / a.run * ((a.run + 3) / 4);
     }
-    return launch<true>(a, sdpa_prefill_packed_tiles(tokens, batch), stream);
+    // The most workgroups there could be, of a die: tiles of four waves per head each; or wgs1 for a
+    // sequence's first row and then at most `rate` / 64 for each row, since 32 more rows make wgs1 into wgs2
+    // and that into wgs4, and 64 more add wgs1.
+    const int64_t used = std::min(batch, tokens), rate = std::max({2 * (a.wgs2 - a.wgs1), 2 * (a.wgs4 - a.wgs2), a.wgs1});
+    const int64_t wgs = std::min(sdpa_prefill_packed_tiles(tokens, batch) * a.per_die,
+                                 used * a.wgs1 + (tokens - used) * rate / 64);
+    return launch<true>(a, wgs << a.die_shift, stream);
 }
 
 }  // namespace nmi

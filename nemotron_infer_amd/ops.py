@@ -690,6 +690,8 @@ def _paged_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Te
         raise ValueError("all tensors must be on one GPU: the pages and the page table are on "
                          f"{k_pages.device}, {v_pages.device} and {page_table.device}")
     n_pages, n_kv, page_size, _ = shape
+    if not n_kv:
+        raise ValueError("pages of no KV heads")
     ks = vs = 0
     if k_scale is not None or v_scale is not None:
         if not e4m3:

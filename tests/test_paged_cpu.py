@@ -228,22 +228,33 @@ result = [[b, h, n, kind, decode(b, h, n_kv=n, kind=kind)] for b in (1, 3, 8, 9,
 
 
 def test_packed_prefill_launches_enough_workgroups(host):  # noqa: F811
-    """As many per head as the most query tiles that `tokens` rows in `batch` sequences can make."""
+    """As many as `tokens` rows in `batch` sequences can need: of a sequence's last tile, one for each head
+    (more than 64 rows, or a launch that is resident at once), two or four heads of a group (fewer rows)."""
     grids = host("""
 W, ST = 1 << 38, 1 << 12
 result = []
-for tokens, batch in ((1, 1), (1, 50), (127, 3), (128, 1), (128, 2), (5000, 7), (300, 1000)):
-    rc = L.nmi_sdpa_prefill_packed_bf16(W, 2048, W, 512, W, 512, W, 2048, W, batch, tokens, 16, 4, 0.1, ST)
-    assert rc == 0, L.nmi_last_error()
-    result.append([tokens, batch, launches()[0][1]])
+for H, n_kv in ((16, 4), (40, 8), (6, 2), (7, 1)):
+    for tokens, batch in ((1, 1), (1, 50), (127, 3), (128, 1), (128, 2), (5000, 7), (300, 1000), (2000, 60), (2000, 30), (9000, 70)):
+        rc = L.nmi_sdpa_prefill_packed_bf16(W, H * 128, W, n_kv * 128, W, n_kv * 128, W, H * 128, W, batch, tokens, H, n_kv, 0.1, ST)
+        assert rc == 0, L.nmi_last_error()
+        result.append([H, n_kv, tokens, batch, launches()[-1][1]])
 """)
-    for tokens, batch, x in grids:
-        n = min(batch, tokens)
-        # n sequences, all of one row but the last: and one whose last tile is a single row as often as can be
-        most = max(sum(-(-v // 128) for v in lens) for lens in (
-            [1] * (n - 1) + [tokens - n + 1],
-            [128 * i + 1 for i in [(tokens - n) // 128 // n] * n]))
-        assert x % 16 == 0 and x // 16 >= most
+    for H, n_kv, tokens, batch, x in grids:
+        n, group = min(batch, tokens), H // n_kv
+        shared = (tokens // 128 + n) * H > 2 * 256
+
+        def workgroups(v):
+            rows = v - v // 128 * 128 or 128
+            heads = 1 if rows > 64 or not shared else 2 if rows > 32 else 4
+            return (-(-v // 128) - 1) * H + n_kv * -(-group // heads) if v else 0
+
+        # n sequences, all of one row but the last; and as many as can be whose last tile just needs more
+        tries = [[1] * (n - 1) + [tokens - n + 1]]
+        for full in (0, 128, 256):
+            for v in (full + 1, full + 33, full + 65):
+                m = min(n, tokens // v)
+                tries.append([v] * m + ([tokens - m * v] if m < n else []))
+        assert x >= max(sum(workgroups(v) for v in lens) for lens in tries if lens), (H, tokens, batch)
 
 
 # --- refusals --------------------------------------------------------------------------------------

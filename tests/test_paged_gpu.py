@@ -171,6 +171,17 @@ def test_decode_ragged_batches(kind):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("batch", [65, 128, 129, 320, 321, 700])
+def test_decode_many_sequences(kind, batch):
+    announce("decode_many", kind, batch)
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(1, 60, batch)
+    lens[rng.integers(0, batch, batch // 4)] = 0
+    lens[[batch // 3, batch - 1]] = 700, 333
+    _check_decode(rng, lens, 4, 2, 16, kind, label=f"{batch} sequences")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 def test_decode_long_peaked_flat_and_scaled(kind):
     rng = np.random.default_rng(8)
     announce("paged_long", kind)
@@ -477,6 +488,15 @@ def test_prefill_one_length(n):
 def test_prefill_ragged(lens):
     announce("packed_ragged", len(lens), sum(lens))
     _check_prefill(np.random.default_rng(sum(lens)), lens, 6, 2, lead=1, tail=2, wide=True)
+
+
+@pytest.mark.parametrize("H,n_kv", [(10, 2), (16, 2)])
+@pytest.mark.parametrize("lens", [[1, 33, 65, 0, 129, 32, 64, 40, 300, 2] * 33, [65] * 257, [33] * 300, [1] * 600],
+                         ids=["ragged", "65", "33", "1"])
+def test_prefill_many_sequences(H, n_kv, lens):
+    """More sequences than stay at hand, and the lengths that need the most workgroups for their rows."""
+    announce("packed_many", H, n_kv, len(lens), sum(lens))
+    _check_prefill(np.random.default_rng(len(lens)), lens, H, n_kv, lead=2, tail=1)
 
 
 def test_prefill_heads_scales_and_peaks():
