@@ -492,12 +492,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
 // The pieces of a sequence's heads joined: O = sum_i c_i o_i / sum_i c_i l_i, c_i = 2^(m_i - max m); a
 // sequence of one piece is done already, one of none gets zeros.  A workgroup takes `heads` heads.  Of
 // few pieces, each wave joins a head by itself, two dims a lane; of many, all waves join one head after
-// another: wave w dims 32 (w % 4) .. + 31 of pieces 8 (w / 4) + lane / 8, + 8 GROUPS, .., four dims a lane.
-constexpr int kFewPieces = 8, kAtOnce = 4;
-template <int GROUPS>
-__global__ __launch_bounds__(256 * GROUPS) void sdpa_decode_paged_join_kernel(const PagedDecodeArgs a, int heads) {
-    __shared__ float2 sm_ml[GROUPS][4];
-    __shared__ f32x4 sm_o[GROUPS][kD / 4];
+// another: wave w dims 32 w .. + 31 of pieces lane / 8, + 8, .., four dims a lane, eight pieces of a lane on
+// their way at once.  (With four at once and 16 waves to a head of few sequences: 777 positions 9.3 us
+// both launches, 8.8 so; 60001 45.5, 46.2 so.)
+constexpr int kFewPieces = 8, kAtOnce = 8;
+__global__ __launch_bounds__(64 * kWaves) void sdpa_decode_paged_join_kernel(const PagedDecodeArgs a, int heads) {
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Pieces plan = a.plan[b];
@@ -507,11 +506,11 @@ __global__ __launch_bounds__(256 * GROUPS) void sdpa_decode_paged_join_kernel(co
     uint32_t* out = reinterpret_cast<uint32_t*>(a.o + (int64_t)b * a.ldo);
     auto slot = [&](int i, int h) { return (int64_t)(plan.owner(i) + b) * a.H + h; };
     if (n == 0) {
-        for (int i = h0 * (kD / 2) + tid; i < h1 * (kD / 2); i += 256 * GROUPS) out[i] = 0u;
+        for (int i = h0 * (kD / 2) + tid; i < h1 * (kD / 2); i += 64 * kWaves) out[i] = 0u;
         return;
     }
     if (n <= kFewPieces) {
-        for (int h = h0 + wave; h < h1; h += 4 * GROUPS) {
+        for (int h = h0 + wave; h < h1; h += kWaves) {
             const float2 ml = a.part_ml[slot(min(lane & (kFewPieces - 1), n - 1), h)];
             float2 o[kFewPieces];
 #pragma unroll
@@ -536,16 +535,16 @@ __global__ __launch_bounds__(256 * GROUPS) void sdpa_decode_paged_join_kernel(co
         }
         return;
     }
-    const int quarter = wave & 3, group = wave >> 2, quad = 8 * quarter + (lane & 7);
+    const int quad = 8 * wave + (lane & 7);
     for (int h = h0; h < h1; ++h) {
         float M = -FLT_MAX, L = 0.f;
         f32x4 o{0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 8 * group + (lane >> 3); i0 < n; i0 += 8 * GROUPS * kAtOnce) {
+        for (int i0 = lane >> 3; i0 < n; i0 += 8 * kAtOnce) {
             float2 ml[kAtOnce];
             f32x4 oi[kAtOnce];
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
-                const int i = i0 + 8 * GROUPS * k;
+                const int i = i0 + 8 * k;
                 ml[k] = float2{-FLT_MAX, 0.f};
                 oi[k] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (i < n) {
@@ -570,33 +569,13 @@ __global__ __launch_bounds__(256 * GROUPS) void sdpa_decode_paged_join_kernel(co
             }
             M = mn;
         }
-        // over the lanes of the same dims (8 apart: the other half of the row, then the rows), then the groups
+        // over the lanes of the same dims (8 apart: the other half of the row, then the rows)
         const float mw = rows_max(fmaxf(M, dpp_f32<0x128>(M)));
         const float c = fexp2(M - mw);
         L = rows_sum(L * c + dpp_f32<0x128>(L * c));
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[d] = rows_sum(o[d] * c + dpp_f32<0x128>(o[d] * c));
-        if constexpr (GROUPS > 1) {
-            if (lane == 0) sm_ml[group][quarter] = float2{mw, L};
-            if (lane < 8) sm_o[group][quad] = o;
-            __syncthreads();
-            if (group == 0 && lane < 8) {
-                float mt = sm_ml[0][quarter].x;
-#pragma unroll
-                for (int k = 1; k < GROUPS; ++k) mt = fmaxf(mt, sm_ml[k][quarter].x);
-                L = 0.f;
-                o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < GROUPS; ++k) {
-                    const float w = fexp2(sm_ml[k][quarter].x - mt);
-                    L = __builtin_fmaf(w, sm_ml[k][quarter].y, L);
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) o[d] = __builtin_fmaf(w, sm_o[k][quad][d], o[d]);
-                }
-            }
-            if (h + 1 < h1) __syncthreads();
-        }
-        if (group == 0 && lane < 8) {
+        if (lane < 8) {
             const float inv = (a.kv.v_scale ? a.kv.v_scale[h / a.group] : 1.f) / L;
             uint32_t* q = out + h * (kD / 2) + 2 * quad;
             q[0] = pack_bf16(o[0] * inv, o[1] * inv);
@@ -614,15 +593,10 @@ hipError_t launch(const PagedDecodeArgs& a, hipStream_t stream) {
     const dim3 grid(a.waves / kWaves, a.kv.n_kv, (a.group + kCols - 1) / kCols);
     hipLaunchKernelGGL((sdpa_decode_paged_kernel<E4M3, MANY>), grid, dim3(64 * kWaves), kLds, stream, a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    // Few sequences are in many pieces: a workgroup of 32 pieces at a time for each head.  Many sequences
-    // are in few pieces each, most in one: workgroups that find nothing to do are what it costs.
-    if (a.batch <= 8) {
-        hipLaunchKernelGGL(sdpa_decode_paged_join_kernel<4>, dim3(a.batch, a.H), dim3(1024), 0, stream, a, 1);
-    } else {
-        const int heads = std::min(8, (int)(((int64_t)a.batch * a.H + 2047) / 2048));
-        hipLaunchKernelGGL(sdpa_decode_paged_join_kernel<1>, dim3(a.batch, (a.H + heads - 1) / heads), dim3(256), 0,
-                           stream, a, heads);
-    }
+    // Many sequences are in few pieces each, most in one: workgroups that find nothing to do are what it costs.
+    const int heads = std::min(8, (int)(((int64_t)a.batch * a.H + 2047) / 2048));
+    hipLaunchKernelGGL(sdpa_decode_paged_join_kernel, dim3(a.batch, (a.H + heads - 1) / heads), dim3(64 * kWaves), 0, stream,
+                       a, heads);
     return hipGetLastError();
 }
 

@@ -223,8 +223,7 @@ result = [[b, h, n, kind, decode(b, h, n_kv=n, kind=kind)] for b in (1, 3, 8, 9,
         (x, y, z, threads), (jx, jy, jz, jthreads) = grids
         assert need == (4 * x + b) * h * 130 * 4 + 16 * b and y == n and z == -(-(h // n) // 16) and threads == 256
         assert 512 - y * z < x * y * z <= 512
-        heads = 1 if b <= 8 else min(8, -(-b * h // 2048))
-        assert jx == b and jy == -(-h // heads) and jz == 1 and jthreads == (1024 if b <= 8 else 256)
+        assert jx == b and jy == -(-h // min(8, -(-b * h // 2048))) and jz == 1 and jthreads == 256
 
 
 def test_packed_prefill_launches_enough_workgroups(host):  # noqa: F811
