@@ -450,7 +450,8 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
  * The work is split by the lengths found on the device: the launch depends on the batch size only.
  * workspace: nmi_sdpa_decode_paged_workspace_bytes(batch, n_heads, n_kv_heads) bytes, 16-byte aligned,
  * no initialisation; NULL takes it from the bump allocator.  Two launches, the second joining the splits
- * in a fixed order: equal calls give the same bytes.
+ * in a fixed order: equal calls give the same bytes.  o overlaps no input.  Pages that are not attended may
+ * hold anything; an attended infinity in v gives an infinity or NaN.
  */
 size_t nmi_sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv_heads);
 int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,
@@ -462,7 +463,8 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
  * cu_seqlens[b + 1]) of q, k, v and o, with softmax(scale * q . k), in one launch whose grid depends on
  * batch and tokens only.  cu_seqlens int32 [batch + 1], ascending (a sequence may be empty); rows of the
  * `tokens` given that belong to no sequence are left as they were.  Layouts, alignment and strides as
- * nmi_sdpa_prefill_bf16, strides at most 2^24; scale positive.  No workspace.
+ * nmi_sdpa_prefill_bf16, strides at most 2^24; scale positive.  No workspace.  o overlaps no input.  A row
+ * of k or v that is not finite reaches the rows of its sequence from its own on, and no others.
  */
 int nmi_sdpa_prefill_packed_bf16(const void* q_bf16, int64_t ldq, const void* k_bf16, int64_t ldk, const void* v_bf16,
                                  int64_t ldv, void* o_bf16, int64_t ldo, const int32_t* cu_seqlens, int batch, int tokens,

@@ -16,6 +16,9 @@
 // of two times 8 dims each, BATCH times that on their way at once.  With halves paired a lane
 // holds the same 8 dims of both halves, so that a pair never leaves its lane.  The token's cosines are
 // computed once per wave, one per lane, while the vectors are on their way, and passed on through LDS.
+// Measured (40 / 8 heads, rotated; graph replays): one token 3.0-3.7 us, 8191 tokens into an e4m3 cache 50
+// us, 4.7 TB/s read and written (a large copy: 4.9); with a workgroup to a token, 8-byte rows and a
+// float32 sine, 71 us.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 

@@ -22,7 +22,8 @@
 //
 // Wave: stages of 8 KiB (16 positions of bf16, 32 of e4m3) brought into the wave's own LDS by DMA, one
 // on its way while another is used, on past the end of a piece into the next sequence; waves wait for
-// one another only to add up their parts.  A tile of 16 positions lies within a page: its address is one scalar.  Per tile:
+// one another only to add up their parts.  A tile of 16 positions lies within a page: its address is one
+// scalar.  Per tile:
 // * S^T = K . Q^T (positions x heads) by 16x16x32 products: a lane then holds 4 positions of one head.
 // * weights in base 2 against a running maximum that is raised only when a score exceeds it by 2^8
 //   in weight, so that the sums are rarely rescaled.
@@ -31,6 +32,15 @@
 //   parts.  e4m3: the 16 positions of both tiles of a stage, one product for hi, one for lo; the
 //   reads transpose pairs of dims, whose bytes are then sorted: the even dims of a block go to one
 //   product, the odd ones to the next.
+//
+// Measured (graph replays, both launches; 40 query, 8 KV heads): one sequence of 777 positions 8.8 us, of
+// 65536 46 (5.8 TB/s of the cache's bytes; a streaming read of as many 6.5); e4m3, 131072 positions 50
+// (5.4); 64 of 90 to 8000 positions, e4m3, 48 (5.0); 128 of 500 50 (5.3).  What is left of a long one is the
+// second launch and the gap before it (5 us), of a short one the two launches and the lengths, the
+// page's id and the tile read one after another.
+// Both sides of the choices, at 268 MB of cache: DMA past the caches 44 us, through them 50; eight waves per
+// CU 44, ten with smaller stages 47; a workgroup's waves at separate shares throughout 44, and in turns over one
+// 44 where the sequences are long but 56 where they are many (hence both, by is_joint).
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 

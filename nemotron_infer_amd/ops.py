@@ -641,7 +641,7 @@ def mamba_forward_fp8(x: torch.Tensor, norm_w: torch.Tensor, in_w, in_s, conv_w,
 # The operators below are called once per layer and step at sizes where the host bounds the call, so
 # each tensor's properties are asked for once: a helper checks a tensor and returns what the call passes
 # on.  (With a helper per property, a look for the device of all tensors at the end and a ctypes
-# structure for the cache, an eager append took 16.3 us and a decode 17.6 us; so NN and NN.)
+# structure for the cache, an eager append took 16.3 us and a decode 17.6 us; so 11.4 and 13.5.)
 _BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
 _PAGED_KV = struct.Struct("@2P3qPq2P5i4x")     # nmi_paged_kv
 
