@@ -14,6 +14,7 @@ Bars (derived before the first run):
   scale: d / s + |exact / s| 2^-22.
 * what is not rotated and not scaled is copied: bit for bit; what is not addressed stays bit for bit.
 """
+import ctypes
 import threading
 
 import numpy as np
@@ -216,6 +217,42 @@ def test_decode_offsets_past_32_bits():
     assert np.array_equal(bits(pages.contiguous()), kb) and np.array_equal(bits(v_pages.contiguous()), vb)
 
 
+def test_decode_of_sequences_that_share_pages():
+    """A page in several sequences' tables, and twice in one: the same positions read by all of them."""
+    announce("decode_shared_pages")
+    rng = np.random.default_rng(12)
+    pool = Pool(rng, [640, 64], 2, 16, "bf16")
+    pool.table = np.stack([pool.table[0], pool.table[0], np.where(np.arange(pool.table.shape[1]) % 2, pool.table[1, 1], pool.table[0, 3])])
+    pool.dtable, pool.lens = _dev(pool.table), np.array([640, 333, 600], np.int32)
+    q = _rand_bits(rng, 3, 8 * 128)
+    o = pool.decode(_dev(q))
+    torch.cuda.synchronize()
+    K, V = pool.values()
+    want = paged.decode(_f64(q).reshape(3, 8, 128), K, V, pool.table, pool.lens)
+    assert_parity(bits(o).reshape(want.shape), block.bf16_round_exact(want), "shared pages")
+
+
+def test_decode_takes_its_workspace_from_the_allocator():
+    """Through the C ABI without a workspace."""
+    announce("decode_bump")
+    rng = np.random.default_rng(13)
+    pool = Pool(rng, [900, 5], 4, 16, "e4m3")
+    q = _dev(_rand_bits(rng, 2, 16 * 128))
+    want, got = pool.decode(q), torch.zeros(2, 16 * 128, dtype=torch.bfloat16, device=DEV)
+    L, lens = _lib.lib(), _dev(pool.lens)
+    c = _lib.PagedKv(pool.dk.data_ptr(), pool.dv.data_ptr(), 4 * 16 * 128, 16 * 128, 128, pool.dtable.data_ptr(),
+                     pool.table.shape[1], pool.dks.data_ptr(), pool.dvs.data_ptr(), 1, pool.dk.shape[0], 16,
+                     pool.table.shape[1], 4)
+    for _ in range(2):
+        got.zero_()
+        rc = L.nmi_sdpa_decode_paged(ctypes.addressof(c), q.data_ptr(), 16 * 128, got.data_ptr(), 16 * 128, lens.data_ptr(), 2,
+                                     16, 128 ** -0.5, None, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, L.nmi_last_error()
+        torch.cuda.synchronize()
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+        assert L.nmi_alloc_rewind() in (0, None)
+
+
 def test_decode_strides_and_outputs():
     """q and o as columns of wider buffers; the rest of o's buffer stays as it was."""
     announce("paged_strides")
@@ -383,6 +420,38 @@ def test_append_many_sequences_of_odd_lengths():
     rng = np.random.default_rng(20)
     lens = [int(n) for n in rng.integers(0, 5, 300)]
     _check_append(rng, [int(s) for s in rng.integers(-2, 40, 300)], lens, 4, 1, 16, "bf16", 32, True, lead=1, tail=70)
+
+
+@pytest.mark.parametrize("kind,rotary,interleaved", [("bf16", 0, False), ("bf16", 128, False), ("e4m3", 96, True)])
+def test_append_more_vectors_than_a_wave_loads_at_once(kind, rotary, interleaved):
+    """A wave for a token, whose head vectors it takes in two turns; in place, too."""
+    announce("append_turns", kind, rotary)
+    rng = np.random.default_rng(23)
+    _check_append(rng, [3, 0, 90], [600, 37, 700], 48, 16, 32, kind, rotary, interleaved, in_place=rotary > 0, lead=1, tail=1)
+
+
+def test_append_offsets_past_32_bits():
+    """Pages whose bytes lie more than 2^32 from the pool's start."""
+    announce("append_large_pool")
+    n_pages, n_kv, page = 70000, 8, 32
+    k_pages = torch.empty(n_pages, n_kv, page, 128, dtype=torch.bfloat16, device=DEV)
+    v_pages = torch.empty_like(k_pages)
+    assert k_pages.numel() * 2 > 1 << 32
+    rng = np.random.default_rng(24)
+    k, v = (_rand_bits(rng, 40, n_kv * 128) for _ in range(2))
+    table = np.array([[n_pages - 1, 66001], [65999, n_pages - 2]], np.int32)
+    for t in table.flat:
+        k_pages[int(t)].zero_(), v_pages[int(t)].zero_()
+    ops.kv_append_paged(_dev(k), _dev(v), k_pages, v_pages, _dev(table), _dev(np.array([20, 31], np.int32)),
+                        cu_seqlens=_dev(np.array([0, 30, 40], np.int32)))
+    torch.cuda.synchronize()
+    for x, pool in ((k, k_pages), (v, v_pages)):
+        want = {int(t): np.zeros((n_kv, page, 128), np.uint16) for t in table.flat}
+        for t in range(40):
+            b, pos = (0, 20 + t) if t < 30 else (1, 31 + t - 30)
+            want[int(table[b, pos // page])][:, pos % page] = x[t].reshape(n_kv, 128)
+        for i, w in want.items():
+            assert np.array_equal(bits(pool[i]), w), i
 
 
 def test_append_at_far_positions():
@@ -553,6 +622,66 @@ def test_prefill_values_that_are_not_finite_stay_with_the_rows_that_see_them(bad
         assert np.isfinite(got[~seen]).all()
         clean = np.isfinite(got) & np.isfinite(want)
         assert_parity(bits(o).reshape(T, H, 128)[clean], block.bf16_round_exact(want[clean]), f"not finite at {at}")
+
+
+def test_prefill_rows_far_apart():
+    """The largest row stride: offsets past 32 bits within a sequence."""
+    announce("packed_far_rows")
+    rng = np.random.default_rng(35)
+    lens, H, n_kv, ld = [150, 40], 2, 1, 1 << 24
+    T, cu = sum(lens), np.array([0, 150, 190], np.int32)
+    buf = torch.empty(T * ld, dtype=torch.bfloat16, device=DEV)
+    views, host = [], []
+    for at, n in ((0, H), (4096, n_kv), (ld - 128, n_kv), (8192, H)):
+        views.append(buf.as_strided((T, n * 128), (ld, 1), at))
+        host.append(_rand_bits(rng, T, n * 128))
+        views[-1].copy_(_dev(host[-1]))
+    ops.sdpa_prefill_packed_bf16(*views[:3], _dev(cu), H, n_kv, out=views[3])
+    torch.cuda.synchronize()
+    q, k, v = (_f64(x).reshape(T, -1, 128) for x in host[:3])
+    want = paged.prefill(q, k, v, cu)
+    assert_parity(bits(views[3].contiguous()).reshape(want.shape), block.bf16_round_exact(want), "far rows")
+
+
+def test_prefill_replays_with_other_offsets():
+    """One graph, replayed with offsets that change on the device, gives the eager bytes each time; rows of
+    no sequence stay."""
+    announce("packed_graph")
+    rng = np.random.default_rng(36)
+    H, n_kv, T = 16, 4, 700
+    q, k, v = (_dev(_rand_bits(rng, T, n * 128)) for n in (H, n_kv, n_kv))
+    cu = _dev(np.array([0, 700, 700, 700, 700], np.int32))
+    out = torch.zeros(T, H * 128, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.sdpa_prefill_packed_bf16(q, k, v, cu, H, n_kv, out=out)
+    for offsets in ([0, 700, 700, 700, 700], [0, 1, 2, 3, 4], [5, 5, 260, 261, 699], [0, 128, 256, 384, 512], [9, 9, 9, 9, 9]):
+        cu.copy_(_dev(np.array(offsets, np.int32)))
+        out.fill_(3.0)
+        g.replay()
+        eager = ops.sdpa_prefill_packed_bf16(q, k, v, cu, H, n_kv, out=torch.full_like(out, 3.0))
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), eager.view(torch.int16)), offsets
+        rest = torch.ones(T, dtype=torch.bool)
+        rest[offsets[0]:offsets[-1]] = False
+        assert (out.cpu()[rest] == 3.0).all()
+    assert _lib.lib().nmi_async_status() == 0
+
+
+def test_nothing_to_do():
+    """No sequences, or no rows: nothing is launched, the outputs are empty."""
+    announce("paged_empty")
+    pool = Pool(np.random.default_rng(37), [3], 2, 16, "bf16")
+    rows = lambda n: torch.empty(0, n * 128, dtype=torch.bfloat16, device=DEV)  # noqa: E731
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    table = torch.empty(0, 4, dtype=torch.int32, device=DEV)
+    assert ops.sdpa_decode_paged(rows(4), pool.dk, pool.dv, table, none).shape == (0, 512)
+    ops.kv_append_paged(rows(2), rows(2), pool.dk, pool.dv, table, none)
+    ops.kv_append_paged(rows(2), rows(2), pool.dk, pool.dv, pool.dtable, _dev(np.zeros(1, np.int32)),
+                        cu_seqlens=_dev(np.zeros(2, np.int32)))
+    assert ops.sdpa_prefill_packed_bf16(rows(4), rows(2), rows(2), _dev(np.zeros(3, np.int32)), 4, 2).shape == (0, 512)
+    torch.cuda.synchronize()
 
 
 def test_prefill_bad_offsets_are_cut_and_reported():
