@@ -5,11 +5,12 @@
 Produces
   nemotron_infer_amd/lib/libnmi.so                 HIP kernels + C ABI (include/nmi_fp8_linear.h)
   nemotron_infer_amd/csrc/binding<EXT_SUFFIX>      pybind11 module `binding` over the C ABI
+  nemotron_infer_amd/csrc/front<EXT_SUFFIX>        torch front end of the batched attention operators
 
 Every HIP translation unit is compiled with ``--offload-arch=gfx950`` and with packed-fp32
 code generation disabled (``-Xclang -target-feature -Xclang -packed-fp32-ops``).  The build
 always recompiles (it is also the "does it build" check) and replaces outputs atomically.
-CMakeLists.txt at the repository root builds the same two artefacts with the same flags
+CMakeLists.txt at the repository root builds the same artefacts with the same flags
 (``cmake -S . -B build -G Ninja && cmake --build build``; tests/test_cmake_build.py checks that
 both builds export the same symbols).
 """
@@ -98,9 +99,31 @@ def build_binding(verbose=False) -> str:
     return out
 
 
+def build_front(verbose=False) -> str:
+    import torch
+
+    at = os.path.dirname(torch.__file__)
+    suffix = sysconfig.get_config_var("EXT_SUFFIX")
+    out = os.path.join(CSRC, "front" + suffix)
+    with tempfile.TemporaryDirectory(prefix="nmi_front_") as tmp:
+        so = os.path.join(tmp, "front" + suffix)
+        # (torch's libraries are in the process when ops.py loads this: no path to them is kept)
+        _run(["g++", "-O2", "-shared", "-fPIC", "-std=c++17", "-Wall",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+              f"-I{sysconfig.get_paths()['include']}", f"-isystem{at}/include", f"-I{INCLUDE}",
+              os.path.join(CSRC, "front.cpp"), "-o", so, f"-L{at}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10"])
+        _atomic_copy(so, out)
+    if verbose:
+        print("built", out)
+    return out
+
+
 def build(verbose=False):
-    lib = build_lib(verbose)
-    bnd = build_binding(verbose)
+    with ThreadPoolExecutor(max_workers=1) as ex:
+        front = ex.submit(build_front, verbose)
+        lib = build_lib(verbose)
+        bnd = build_binding(verbose)
+        front.result()
     return lib, bnd
 
 

@@ -9,7 +9,6 @@ include/nmi_fp8_linear.h; there is no torch or CPU fallback.
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import torch
 
@@ -638,86 +637,37 @@ def mamba_forward_fp8(x: torch.Tensor, norm_w: torch.Tensor, in_w, in_s, conv_w,
     return out
 
 
-# The operators below are called once per layer and step at sizes where the host bounds the call, so
-# each tensor's properties are asked for once: a helper checks a tensor and returns what the call passes
-# on.  (With a helper per property, a look for the device of all tensors at the end and a ctypes
-# structure for the cache, an eager append took 16.3 us and a decode 17.6 us; so 11.4 and 13.5.)
-_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
-_PAGED_KV = struct.Struct("@2P3qPq2P5i4x")     # nmi_paged_kv
+# The operators below are called once per layer and step at sizes where the host bounds an eager call, so
+# their checks, outputs and calls of the C ABI are in C++ (csrc/front.cpp).  (With a Python helper per tensor
+# property and a ctypes call an eager append took 16.3 us and a decode 17.6 us, with one helper per tensor
+# 11.1 and 13.2; so 6.1 and 9.9, the decode's launches alone 8.8.)
+_entries: dict[str, tuple] = {}
 
 
-def _rows(t: torch.Tensor, T: int, cols: int, name: str, dev: int):
-    """Rows [T, >= cols] of bf16 on GPU `dev`: (address, row stride)."""
-    shape, st = t.shape, t.stride()
-    if t.dtype is not _BF16 or len(shape) != 2 or shape[0] != T or shape[1] < cols or st[1] != 1:
-        raise ValueError(f"{name} must be a bf16 [{T}, >= {cols}] tensor with contiguous rows, got {t.dtype} "
-                         f"{tuple(shape)} strides {st}")
-    if t.get_device() != dev:
-        raise ValueError(f"all tensors must be on one GPU: {name} is on {t.device}")
-    # (torch's stride of a dimension of one element has no meaning)
-    return t.data_ptr(), st[0] if T > 1 else (shape[1] + 7) // 8 * 8
+def _front(name: str, *also: str):
+    """The front end's function of that name, and the addresses of the library's nmi_ entries: its own and
+    those of `also`."""
+    got = _entries.get(name)
+    L = _lib.lib()
+    if got is None or got[0] is not L:
+        try:
+            from .csrc import front
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `python -m nemotron_infer_amd.build`") from e
+        addresses = [ctypes.cast(getattr(L, "nmi_" + n), ctypes.c_void_p).value for n in (name, *also)]
+        got = _entries[name] = (L, getattr(front, name), *addresses)
+    return got[1:]
 
 
-def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, name: str, dev: int) -> int:
-    """A contiguous vector of n values on GPU `dev`: its address."""
-    shape = t.shape
-    if t.dtype is not dtype or len(shape) != 1 or shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} values, got {t.dtype} {tuple(shape)}")
-    if t.get_device() != dev:
-        raise ValueError(f"all tensors must be on one GPU: {name} is on {t.device}")
-    return t.data_ptr()
-
-
-def _paged_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, batch: int, k_scale, v_scale,
-              dev: int):
-    """The cache's descriptor (an nmi_paged_kv) and its KV heads: pages [n_pages, n_kv_heads, page_size,
-    128] of any strides with contiguous head vectors, K and V alike."""
-    shape, st, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
-    if len(shape) != 4 or shape[3] != 128 or st[3] != 1:
-        raise ValueError(f"k_pages must be [n_pages, n_kv_heads, page_size, 128] with contiguous head vectors, got "
-                         f"{tuple(shape)} strides {st}")
-    e4m3 = dtype is not _BF16
-    if e4m3 and dtype is not torch.float8_e4m3fn and dtype is not torch.uint8:
-        raise TypeError(f"pages must be bfloat16, float8_e4m3fn or uint8 codes, got {dtype}")
-    if v_pages.dtype is not dtype or v_pages.shape != shape or v_pages.stride() != st:
-        raise ValueError(f"v_pages must be as k_pages ({dtype} {tuple(shape)} strides {st}), got {v_pages.dtype} "
-                         f"{tuple(v_pages.shape)} strides {v_pages.stride()}")
-    tshape, tst = page_table.shape, page_table.stride()
-    if page_table.dtype is not _I32 or len(tshape) != 2 or tshape[0] != batch or tst[1] != 1:
-        raise ValueError(f"page_table must be int32 [batch={batch}, max_pages] with contiguous rows, got "
-                         f"{page_table.dtype} {tuple(tshape)} strides {tst}")
-    if k_pages.get_device() != dev or v_pages.get_device() != dev or page_table.get_device() != dev:
-        raise ValueError("all tensors must be on one GPU: the pages and the page table are on "
-                         f"{k_pages.device}, {v_pages.device} and {page_table.device}")
-    n_pages, n_kv, page_size, _ = shape
-    if not n_kv:
-        raise ValueError("pages of no KV heads")
-    ks = vs = 0
-    if k_scale is not None or v_scale is not None:
-        if not e4m3:
-            raise ValueError("a bf16 cache takes no scales")
-        if k_scale is not None:
-            ks = _vector(k_scale, n_kv, _F32, "k_scale", dev)
-        if v_scale is not None:
-            vs = _vector(v_scale, n_kv, _F32, "v_scale", dev)
-    ps, hs, ts, _ = st
-    if n_pages == 1 or n_kv == 1 or page_size == 1:     # (strides without meaning)
-        ps, hs, ts = (s if n > 1 else 128 for s, n in zip(st, shape[:3]))
-    max_pages = tshape[1]
-    return _PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), ps, hs, ts, page_table.data_ptr(),
-                          tst[0] if batch > 1 else max_pages, ks, vs, int(e4m3), n_pages, page_size, max_pages,
-                          n_kv), n_kv
-
-
-def _check_current(dev: int, t: torch.Tensor) -> bool:
-    """Whether GPU `dev`, t's, is the current device, by which the stream, the launch and the library's
-    per-device state go (torch.cuda.device makes it so)."""
+def _elsewhere(dev: int) -> bool:
+    """Whether `dev` is a GPU other than the current device, by which the stream, the launch and the
+    library's per-device state go (torch.cuda.device makes it so)."""
     if dev < 0:
-        raise ValueError(f"tensors must be on a GPU, got {t.device}")
+        return False                           # (the front end refuses it)
     try:
-        return dev == torch._C._cuda_getDevice()
+        return dev != torch._C._cuda_getDevice()
     except AttributeError:                     # private to torch: another version may lack it
-        return dev == torch.cuda.current_device()
+        return dev != torch.cuda.current_device()
 
 
 def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -733,47 +683,13 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     position, and q [T, n_heads * 128] too.  Returns (q_out, k_out): the rotated q (None without q)
     and k_out, which receives the rotated k where it is given; either may be its input itself."""
     dev = k.get_device()
-    if start_pos.dim() != 1:
-        raise ValueError(f"start_pos must be an int32 vector [batch], got {tuple(start_pos.shape)}")
-    batch, T = start_pos.shape[0], k.shape[0]
-    start = _vector(start_pos, batch, _I32, "start_pos", dev)
-    cache, n_kv = _paged_kv(k_pages, v_pages, page_table, batch, k_scale, v_scale, dev)
-    kp, ldk = _rows(k, T, n_kv * 128, "k", dev)
-    vp, ldv = _rows(v, T, n_kv * 128, "v", dev)
-    cu = qp = ldq = qop = ldqo = kop = ldko = freq = rotary = H = 0
-    if cu_seqlens is not None:
-        cu = _vector(cu_seqlens, batch + 1, _I32, "cu_seqlens", dev)
-    elif T != batch:
-        raise ValueError(f"{T} rows for {batch} sequences: give cu_seqlens")
-    if inv_freq is not None:
-        rotary = 2 * inv_freq.numel()
-        freq = _vector(inv_freq, rotary // 2, _F32, "inv_freq", dev)
-        if q is not None:
-            H = q.shape[-1] // 128
-            if q.dim() != 2 or not H or q.shape[1] % (n_kv * 128):
-                raise ValueError(f"q must be [T, n_heads * 128], n_heads a multiple of {n_kv}, got {tuple(q.shape)}")
-            qp, ldq = _rows(q, T, H * 128, "q", dev)
-            if q_out is None:
-                q_out = q.new_empty((T, H * 128))
-                qop, ldqo = q_out.data_ptr(), H * 128
-            else:
-                qop, ldqo = _rows(q_out, T, H * 128, "q_out", dev)
-        if k_out is not None:
-            kop, ldko = _rows(k_out, T, n_kv * 128, "k_out", dev)
-    elif q is not None or k_out is not None:
-        raise ValueError("q and k_out are for the rotation: give inv_freq")
-    if q is None and q_out is not None:
-        raise ValueError("q_out without q")
-    if not _check_current(dev, k):
+    if _elsewhere(dev):
         with torch.cuda.device(dev):
             return kv_append_paged(k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q, inv_freq, interleaved,
                                    k_scale, v_scale, q_out, k_out)
-    if T and batch:
-        rc = _lib.lib().nmi_kv_append_paged(cache, qp, ldq, kp, ldk, vp, ldv, qop, ldqo, kop, ldko, cu, start, batch, T, H,
-                                            freq, rotary, 1 if interleaved else 0, _stream())
-        if rc:
-            _lib.check(rc, "nmi_kv_append_paged")
-    return q_out, k_out
+    call, entry = _front("kv_append_paged")
+    return call(_lib.check, _stream() if dev >= 0 else 0, entry, k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q,
+                inv_freq, interleaved, k_scale, v_scale, q_out, k_out)
 
 
 def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -784,35 +700,12 @@ def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     (as kv_append_paged takes them); a length of 0 gives zeros.  scale: 1 / sqrt(128) unless given.
     Returns o [batch, n_heads * 128] bf16."""
     dev = q.get_device()
-    if q.dim() != 2:
-        raise ValueError(f"q must be [batch, n_heads * 128], got {tuple(q.shape)}")
-    batch, cols = q.shape
-    cache, n_kv = _paged_kv(k_pages, v_pages, page_table, batch, k_scale, v_scale, dev)
-    if cols % (n_kv * 128) or not cols:
-        raise ValueError(f"q must be [batch, n_heads * 128], n_heads a multiple of {n_kv}, got {tuple(q.shape)}")
-    qp, ldq = _rows(q, batch, cols, "q", dev)
-    lens = _vector(kv_lens, batch, _I32, "kv_lens", dev)
-    if out is None:
-        out = q.new_empty((batch, cols))
-        op, ldo = out.data_ptr(), cols
-    else:
-        op, ldo = _rows(out, batch, cols, "out", dev)
-    if not _check_current(dev, q):
+    if _elsewhere(dev):
         with torch.cuda.device(dev):
             return sdpa_decode_paged(q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale, scale, out)
-    if batch:
-        L = _lib.lib()
-        st = _stream()
-        H = cols // 128
-        need = L.nmi_sdpa_decode_paged_workspace_bytes(batch, H, n_kv)
-        ws, key = _workspace(q.device, need, st)
-        rc = L.nmi_sdpa_decode_paged(cache, qp, ldq, op, ldo, lens, batch, H, 128 ** -0.5 if scale is None else scale,
-                                     ws.data_ptr(), need, st)
-        if key is not None:
-            _kept[key] = ws
-        if rc:
-            _lib.check(rc, "nmi_sdpa_decode_paged")
-    return out
+    call, entry, ws_bytes = _front("sdpa_decode_paged", "sdpa_decode_paged_workspace_bytes")
+    return call(_lib.check, _stream() if dev >= 0 else 0, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
+                kv_lens, k_scale, v_scale, scale, out)
 
 
 def sdpa_prefill_packed_bf16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, n_heads: int,
@@ -822,28 +715,12 @@ def sdpa_prefill_packed_bf16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     cu_seqlens[b + 1]) (int32) of the token-major q [T, >= n_heads * 128], k, v [T, >= n_kv_heads * 128]
     are prompt b (row-strided views allowed).  scale: 1 / sqrt(128) unless given.  Returns o
     [T, n_heads * 128] bf16; rows of no prompt are left as they were (in a new o: undefined)."""
-    dev, T = q.get_device(), q.shape[0]
-    qp, ldq = _rows(q, T, n_heads * 128, "q", dev)
-    kp, ldk = _rows(k, T, n_kv_heads * 128, "k", dev)
-    vp, ldv = _rows(v, T, n_kv_heads * 128, "v", dev)
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        raise ValueError(f"cu_seqlens must be an int32 vector [batch + 1], got {tuple(cu_seqlens.shape)}")
-    batch = cu_seqlens.shape[0] - 1
-    cu = _vector(cu_seqlens, batch + 1, _I32, "cu_seqlens", dev)
-    if out is None:
-        out = q.new_empty((T, n_heads * 128))
-        op, ldo = out.data_ptr(), n_heads * 128
-    else:
-        op, ldo = _rows(out, T, n_heads * 128, "out", dev)
-    if not _check_current(dev, q):
+    dev = q.get_device()
+    if _elsewhere(dev):
         with torch.cuda.device(dev):
             return sdpa_prefill_packed_bf16(q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
-    if T and batch:
-        rc = _lib.lib().nmi_sdpa_prefill_packed_bf16(qp, ldq, kp, ldk, vp, ldv, op, ldo, cu, batch, T, n_heads, n_kv_heads,
-                                                     128 ** -0.5 if scale is None else scale, _stream())
-        if rc:
-            _lib.check(rc, "nmi_sdpa_prefill_packed_bf16")
-    return out
+    call, entry = _front("sdpa_prefill_packed_bf16")
+    return call(_lib.check, _stream() if dev >= 0 else 0, entry, q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
 
 
 class GemvChain:

@@ -6,6 +6,7 @@ import math
 import os
 import random
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -393,10 +394,11 @@ def test_valid_cpu_calls_are_refused_before_the_library():
 def test_front_end_refuses_bad_caches(name, value, exc):
     t = _tensors()
     t[name] = value
-    with pytest.raises(exc):
-        ops.sdpa_decode_paged(t["q"], t["k_pages"], t["v_pages"], t["page_table"], t["kv_lens"])
-    with pytest.raises(exc):
-        ops.kv_append_paged(t["k"], t["v"], t["k_pages"], t["v_pages"], t["page_table"], t["start_pos"])
+    for call in (lambda: ops.sdpa_decode_paged(t["q"], t["k_pages"], t["v_pages"], t["page_table"], t["kv_lens"]),
+                 lambda: ops.kv_append_paged(t["k"], t["v"], t["k_pages"], t["v_pages"], t["page_table"], t["start_pos"])):
+        with pytest.raises(exc) as e:
+            call()
+        assert "on a GPU" not in str(e.value)       # (the last check, which these tensors would fail)
 
 
 def test_front_end_refuses_bad_operands():
@@ -421,8 +423,9 @@ def test_front_end_refuses_bad_operands():
             lambda: ops.sdpa_prefill_packed_bf16(t["q"], t["k"], t["v"], torch.zeros(2), 4, 2),
             lambda: ops.sdpa_prefill_packed_bf16(t["q"], t["k"][:2], t["v"], torch.zeros(2, dtype=torch.int32), 4, 2),
             lambda: ops.sdpa_prefill_packed_bf16(t["q"], t["k"], t["v"], torch.zeros(0, dtype=torch.int32), 4, 2)):
-        with pytest.raises(ValueError):
+        with pytest.raises(ValueError) as e:
             call()
+        assert "on a GPU" not in str(e.value)
     e = _tensors(kind=torch.float8_e4m3fn)
     with pytest.raises(ValueError, match="k_scale"):
         ops.sdpa_decode_paged(e["q"], e["k_pages"], e["v_pages"], e["page_table"], e["kv_lens"], k_scale=torch.ones(3))
@@ -431,3 +434,46 @@ def test_front_end_refuses_bad_operands():
 def test_block_rounding_helper_is_nearest_even():
     assert np.array_equal(_f64(block.bf16_round_exact(np.array([1.0, 1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8]))),
                           [1.0, 1.0, 1 + 2.0 ** -6])
+
+
+def test_front_end_errors_are_exceptions_and_keep_no_references():
+    """Arguments of any kind end in a Python exception, never past it; what was passed is let go."""
+    t = _tensors()
+    cache = (t["k_pages"], t["v_pages"], t["page_table"])
+    odd = [None, 3, "x", object(), torch.zeros(2, 2).to_sparse(), torch.empty(3, 256, dtype=torch.bfloat16, device="meta"),
+           torch.zeros(()), torch.zeros(0)]
+    calls = [
+        lambda x: ops.sdpa_decode_paged(t["q"], x, t["v_pages"], t["page_table"], t["kv_lens"]),
+        lambda x: ops.sdpa_decode_paged(t["q"], t["k_pages"], x, t["page_table"], t["kv_lens"]),
+        lambda x: ops.sdpa_decode_paged(t["q"], t["k_pages"], t["v_pages"], x, t["kv_lens"]),
+        lambda x: ops.sdpa_decode_paged(t["q"], *cache, x),
+        lambda x: ops.sdpa_decode_paged(x, *cache, t["kv_lens"]),
+        lambda x: ops.sdpa_decode_paged(t["q"], *cache, t["kv_lens"], out=x),
+        lambda x: ops.sdpa_decode_paged(t["q"], *cache, t["kv_lens"], scale=x),
+        lambda x: ops.kv_append_paged(x, t["v"], *cache, t["start_pos"]),
+        lambda x: ops.kv_append_paged(t["k"], x, *cache, t["start_pos"]),
+        lambda x: ops.kv_append_paged(t["k"], t["v"], *cache, x),
+        lambda x: ops.kv_append_paged(t["k"], t["v"], *cache, t["start_pos"], cu_seqlens=x),
+        lambda x: ops.kv_append_paged(t["k"], t["v"], *cache, t["start_pos"], q=x, inv_freq=t["inv_freq"]),
+        lambda x: ops.kv_append_paged(t["k"], t["v"], *cache, t["start_pos"], q=t["q"], inv_freq=x),
+        lambda x: ops.sdpa_prefill_packed_bf16(x, t["k"], t["v"], t["start_pos"], 4, 2),
+        lambda x: ops.sdpa_prefill_packed_bf16(t["q"], t["k"], t["v"], x, 4, 2),
+        lambda x: ops.sdpa_prefill_packed_bf16(t["q"], t["k"], t["v"], t["start_pos"], x, 2),
+    ]
+    held = [*odd[3:], *t.values()]
+    before = [sys.getrefcount(x) for x in held]
+    for _ in range(3):
+        for call in calls:
+            for x in odd:
+                with pytest.raises((ValueError, TypeError, RuntimeError, AttributeError)):
+                    call(x)
+    del call, x
+    assert [sys.getrefcount(x) for x in held] == before
+    pages = torch.zeros(4, 0, 16, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no KV heads"):
+        ops.sdpa_decode_paged(t["q"], pages, pages, t["page_table"], t["kv_lens"])
+    from nemotron_infer_amd.csrc import front
+    for f in (front.kv_append_paged, front.sdpa_decode_paged, front.sdpa_prefill_packed_bf16):
+        with pytest.raises(TypeError, match="expected"):
+            f(1, 2)
+

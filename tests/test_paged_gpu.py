@@ -15,6 +15,7 @@ Bars (derived before the first run):
 * what is not rotated and not scaled is copied: bit for bit; what is not addressed stays bit for bit.
 """
 import ctypes
+import sys
 import threading
 
 import numpy as np
@@ -839,3 +840,43 @@ def test_two_streams_and_two_threads():
     for i in range(2):
         assert len(results[i]) == 20
         assert all(torch.equal(o.view(torch.int16), want[i].view(torch.int16)) for o in results[i])
+
+
+def test_the_front_end_keeps_nothing():
+    """References and device memory after many calls as before them; an error of the library is its
+    exception, after which the next call runs."""
+    announce("paged_front")
+    pool = Pool(np.random.default_rng(51), [40, 7], 2, 16, "e4m3")
+    q, k, pos = _dev(_rand_bits(np.random.default_rng(52), 2, 512)), torch.zeros(2, 256, dtype=torch.bfloat16, device=DEV), _dev(
+        np.array([3, 4], np.int32))
+    f, cu = _dev(np.ones(64, np.float32)), _dev(np.array([0, 1, 2], np.int32))
+
+    def all_three():
+        a, none = ops.kv_append_paged(k, k, pool.dk, pool.dv, pool.dtable, pos, q=q, inv_freq=f, k_scale=pool.dks, v_scale=pool.dvs)
+        b = ops.sdpa_prefill_packed_bf16(a, k, k, cu, 4, 2)
+        c = pool.decode(a)
+        assert none is None and sys.getrefcount(a) == sys.getrefcount(b) == sys.getrefcount(c) == 2
+        same = ops.sdpa_decode_paged(q, pool.dk, pool.dv, pool.dtable, pos, k_scale=pool.dks, v_scale=pool.dvs, out=c)
+        assert same is c
+        return c
+
+    want = all_three()
+    torch.cuda.synchronize()
+    held = [q, k, pos, f, cu, pool.dk, pool.dv, pool.dtable, pool.dks, pool.dvs]
+    counts, memory = [sys.getrefcount(x) for x in held], torch.cuda.memory_allocated()
+    nones = sys.getrefcount(None)
+    for _ in range(300):
+        all_three()
+    torch.cuda.synchronize()
+    assert [sys.getrefcount(x) for x in held] == counts and torch.cuda.memory_allocated() == memory
+    assert abs(sys.getrefcount(None) - nones) < 100
+    small = torch.zeros(4, 2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    for _ in range(3):
+        with pytest.raises(_lib.NmiError, match="page_size=8"):
+            ops.sdpa_decode_paged(q, small, small, pool.dtable, pos)
+        with pytest.raises(_lib.NmiError, match="page_size=8"):
+            ops.kv_append_paged(k, k, small, small, pool.dtable, pos)
+        with pytest.raises(_lib.NmiError, match="scale"):
+            ops.sdpa_prefill_packed_bf16(q, k, k, cu, 4, 2, scale=-1.0)
+    assert [sys.getrefcount(x) for x in held] == counts
+    assert torch.equal(all_three().view(torch.int16), want.view(torch.int16))
