@@ -157,8 +157,8 @@ void* stream_of(PyObject* o) {
     return p;
 }
 // What the library reports, raised by _lib.check.
-void check(PyObject* checker, int rc, const char* name) {
-    if (rc != NMI_OK) Owned(PyObject_CallFunction(checker, "is", rc, name));
+void check(PyObject* raise_error, int rc, const char* name) {
+    if (rc != NMI_OK) Owned(PyObject_CallFunction(raise_error, "is", rc, name));
 }
 float scale_of(PyObject* o) {
     if (o == Py_None) return 0.08838834764831845f;              // 1 / sqrt(128)
@@ -181,7 +181,7 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
 }
 
-// checker, stream, entry, k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q, inv_freq, interleaved, k_scale,
+// _lib.check, stream, entry, k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q, inv_freq, interleaved, k_scale,
 // v_scale, q_out, k_out -> (q_out, k_out)
 PyObject* kv_append_paged(PyObject* const* a) {
     const at::Tensor &k = tensor(a[3], "k"), &start = tensor(a[8], "start_pos");
@@ -230,7 +230,7 @@ PyObject* kv_append_paged(PyObject* const* a) {
     return PyTuple_Pack(2, out.p, k_out);
 }
 
-// checker, stream, entry, its workspace's size, workspace, kept, q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale,
+// _lib.check, stream, entry, its workspace's size, workspace, kept, q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale,
 // scale, out -> out.  workspace(device, bytes, stream) -> (tensor, key), kept[key] = tensor after the launch.
 PyObject* sdpa_decode_paged(PyObject* const* a) {
     const at::Tensor& q = tensor(a[6], "q");
@@ -270,7 +270,7 @@ PyObject* sdpa_decode_paged(PyObject* const* a) {
     return new_ref(out.p);
 }
 
-// checker, stream, entry, q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out -> out
+// _lib.check, stream, entry, q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out -> out
 PyObject* sdpa_prefill_packed_bf16(PyObject* const* a) {
     const at::Tensor& q = tensor(a[3], "q");
     const int64_t dev = q.get_device(), T = q.dim() ? q.size(0) : -1;
