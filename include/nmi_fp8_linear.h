@@ -396,8 +396,9 @@ int nmi_attn_forward_fp8(const void* input_bf16, const float* norm_w, const void
  * as the sequences grow) and are not seen by the host.  The kernels never follow one that is out of
  * range -- a page id outside [0, n_pages), a position or length that a row of the table does not
  * hold, offsets that do not ascend within the rows given --: the token is not stored, or the
- * sequence's output of that KV head is NaN, or the rows are cut to those given, and NMI_ERR_ASYNC
- * reports it as described at the top of this file.
+ * sequence's output of that KV head is NaN, or a sequence's rows are cut to those given (none where its
+ * offsets fall; a row that falling offsets give to several sequences is the first one's in the append and
+ * any one's in the attention), and NMI_ERR_ASYNC reports it as described at the top of this file.
  */
 enum { NMI_KV_BF16 = 0, NMI_KV_E4M3 = 1 };
 typedef struct nmi_paged_kv {

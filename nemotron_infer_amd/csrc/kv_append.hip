@@ -56,15 +56,27 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&x)[8], float s) {
     return uint2{(uint32_t)a, (uint32_t)b};
 }
 
-// The sequence of packed row t: the number of ends cu[1 ..] at or before it (64 of them at a time).
-__device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int t, int lane) {
-    for (int b0 = 0; b0 < batch; b0 += 64) {
+// The sequence of packed row t and t's place in it, 64 sequences at a time; *b = -1 where no sequence has
+// the row, the first of several that do (offsets that fall).  `all`: look through every sequence's
+// offsets, also behind the row's.  Whether any looked at were out of order or range.
+__device__ __forceinline__ bool find_sequence(const AppendArgs& a, int t, bool all, int lane, int* b, int* place) {
+    uint64_t bad = 0;
+    *b = -1;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const int i = b0 + lane;
-        const bool before = i < batch && cu[i + 1] <= t;
-        const int n = __popcll(__builtin_amdgcn_ballot_w64(before));
-        if (n < 64) return b0 + n;
+        int at = 0;
+        bool off = false;
+        const bool mine = i < a.batch && span_holds(a.cu[i], a.cu[i + 1], a.tokens, t, &at, &off);
+        bad |= __builtin_amdgcn_ballot_w64(off);
+        const uint64_t holds = __builtin_amdgcn_ballot_w64(mine);
+        if (holds && *b < 0) {
+            const int who = __builtin_ctzll(holds);
+            *b = b0 + who;
+            *place = __builtin_amdgcn_readlane(at, who);
+        }
+        if (*b >= 0 && !all) break;
     }
-    return batch;
+    return bad != 0;
 }
 
 // cos and sin of 2 pi f, |f| <= 1/2: f = q / 4 + y with |y| <= 1/8, the Taylor polynomials of y's angle
@@ -119,33 +131,39 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs
     load(part);
 
     int b = t, place = 0;
+    bool bad = false;                                           // device data out of range
+    auto report = [&]() {
+        if (bad && lane == 0 && a.kv.error)
+            __hip_atomic_store(a.kv.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+    };
+    // (not before the page's id is here: behind a store the compiler takes no more uniform values through
+    // the scalar cache, and an eager call of 8191 tokens takes 55.1 us instead of 52.4)
     if (a.cu) {
-        b = __builtin_amdgcn_readfirstlane(sequence_of(a.cu, a.batch, t, lane));
-        if (b >= a.batch) return;                               // rows behind the last sequence
-        place = t - a.cu[b];
-        if (place < 0) return;                                  // rows before the first
+        // (the last row's wave looks through all offsets: it goes the farthest anyway)
+        bad = find_sequence(a, t, part == 0 && t == a.tokens - 1, lane, &b, &place);
+        if (b < 0) return report();                             // rows of no sequence
     }
     const int start = a.start[b];
-    if (start < 0) return;                                      // a sequence that is not in use
+    if (start < 0) return report();                             // a sequence that is not in use
     const int64_t pos = (int64_t)start + place;
 
     // where the token goes; nowhere if the table has no page for it
     uint8_t *kp = nullptr, *vp = nullptr;
     {
-        bool bad = false;
+        bool nowhere = false;
         const int64_t entry = pos >> a.kv.page_shift;
         int page = 0;
         if (entry < a.kv.max_pages)
-            page = checked_page(a.kv.page_table[b * a.kv.table_stride + entry], a.kv.n_pages, &bad);
+            page = checked_page(a.kv.page_table[b * a.kv.table_stride + entry], a.kv.n_pages, &nowhere);
         else
-            bad = true;
-        if (!bad) {
+            nowhere = true;
+        if (!nowhere) {
             const int64_t off = page * a.kv.page_stride + (pos & ((1 << a.kv.page_shift) - 1)) * a.kv.token_stride;
             kp = a.kv.k_pages + off;
             vp = a.kv.v_pages + off;
-        } else if (lane == 0 && a.kv.error) {
-            __hip_atomic_store(a.kv.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
+        bad |= nowhere;
+        report();
     }
     float c[8], s[8];                                           // of the lane's pairs
     if constexpr (MODE != kPlain) {

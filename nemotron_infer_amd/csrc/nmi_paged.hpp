@@ -62,6 +62,14 @@ NMI_HD int checked_span(int c0, int c1, int tokens, int* first, bool* bad) {
     return e - f;
 }
 
+// Whether packed row t is one of those of the sequence with offsets c0, c1, and then its place there.
+NMI_HD bool span_holds(int c0, int c1, int tokens, int t, int* place, bool* bad) {
+    int first = 0;
+    const int n = checked_span(c0, c1, tokens, &first, bad);
+    *place = t - first;
+    return *place >= 0 && *place < n;
+}
+
 // Decode attention: tiles per wave when all sequences' tiles, `total` of them in a row, are dealt to at
 // most `waves` waves, at least `unit` to each.
 constexpr int kPagedMaxPositions = 1 << 30;

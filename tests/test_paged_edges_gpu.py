@@ -1,0 +1,91 @@
+"""GPU tests of batched attention serving where its device data is out of order or range, and where values
+are not finite.  Bars as in test_paged_gpu.py: what is copied is bit for bit, attention goes by the parity
+gate of oracle.linear.parity against float64 rounded once."""
+import numpy as np
+import pytest
+import torch
+
+from nemotron_infer_amd import _lib, ops
+from oracle import block, paged
+from tests.gpu_util import announce, assert_parity, bits
+from tests.test_paged_gpu import LUT, NAN_BF16, Pool, _bf16, _between, _dev, _f64, _rand_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_pending_error():
+    _lib.lib().nmi_async_status()
+    yield
+    torch.cuda.synchronize()
+    _lib.lib().nmi_async_status()
+
+
+def _cut(cu, T):
+    """[(first, end)] of the sequences, cut to the T rows; (0, 0) for offsets that fall."""
+    return [(min(max(int(a), 0), T), max(min(max(int(a), 0), T), min(max(int(b), 0), T))) for a, b in zip(cu, cu[1:])]
+
+
+BAD_OFFSETS = [
+    (50, [0, 20, 51]), (50, [-1, 20, 50]), (50, [0, 30, 20]), (50, [0, 20, 10, 50]), (12, [0, 8, 2, 4, 12]),
+    (50, [2 ** 31 - 1] * 3), (50, [-5, -5, -5]), (50, [-2 ** 31, 50]), (50, [60, 70]),
+    (50, [3, 20, 40, 2 ** 31 - 1, 40]),
+    # more sequences than lanes: behind the rows' own, before them, and between
+    (10, [0, 5, 10] + [10] * 100 + [11]), (10, [0, 5, 10] + [10] * 100 + [9]), (10, [0, -1] + [0] * 100 + [4, 10]),
+    (300, [*range(0, 150), 100, *range(150, 301)]),
+]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rotary", [0, 128])
+@pytest.mark.parametrize("T,cu", BAD_OFFSETS, ids=[str(i) for i in range(len(BAD_OFFSETS))])
+def test_append_bad_offsets_are_cut_and_reported(kind, rotary, T, cu):
+    """Offsets that fall or leave the rows are cut to them, as for the attention over packed prompts: the rows of
+    each sequence from its first on, a row that several have as the first one's; rows of none are not
+    stored or returned, and NMI_ERR_ASYNC says so once."""
+    announce("append_bad_offsets", kind, rotary, T, cu[:8])
+    rng = np.random.default_rng(T + len(cu))
+    n_kv, H, page, batch = 2, 4, 16, len(cu) - 1
+    starts = rng.integers(0, 40, batch).astype(np.int32)
+    spans = _cut(cu, T)
+    pool = Pool(rng, [int(s) for s in starts], n_kv, page, kind,
+                hold=[int(s) + b - a for s, (a, b) in zip(starts, spans)])
+    q, k, v = (_rand_bits(rng, T, n * 128) for n in (H, n_kv, n_kv))
+    before = [pool.host(pool.dk).copy(), pool.host(pool.dv).copy()]
+    f = (10000.0 ** (-np.arange(64) / 64)).astype(np.float32) if rotary else None
+    qo = torch.full((T, H * 128), 5.0, dtype=torch.bfloat16, device="cuda") if rotary else None
+    ko = torch.full((T, n_kv * 128), 5.0, dtype=torch.bfloat16, device="cuda") if rotary else None
+    ops.kv_append_paged(_dev(k), _dev(v), pool.dk, pool.dv, pool.dtable, _dev(starts), cu_seqlens=_dev(np.array(cu)),
+                        q=_dev(q) if rotary else None, inv_freq=_dev(f) if rotary else None, k_scale=pool.dks,
+                        v_scale=pool.dvs, q_out=qo, k_out=ko)
+    torch.cuda.synchronize()
+    assert _lib.lib().nmi_async_status() == _lib.NMI_ERR_ASYNC
+    assert _lib.lib().nmi_async_status() == 0
+    rows = [(t, b, int(starts[b]) + t - spans[b][0]) for t in range(T)
+            for b in [next((i for i, (x, y) in enumerate(spans) if x <= t < y), -1)] if b >= 0]
+    after = [pool.host(pool.dk), pool.host(pool.dv)]
+    stored = np.zeros(before[0].shape, bool)
+    if rows:
+        r, seq, pos = (np.array(x) for x in zip(*rows))
+        at = (pool.table[seq, pos // page], slice(None), pos % page)
+        stored[at] = True
+        vals = [_f64(x[r]).reshape(len(r), n_kv, 128) for x in (k, v)]
+        slack = [0 * x for x in vals]
+        if rotary:
+            slack[0] = paged.partner_sum(vals[0], rotary, False) * 2.0 ** -20
+            vals[0] = paged.rotate(vals[0], pos.astype(np.float64), f, False)
+            x = _f64(q[r]).reshape(len(r), H, 128)
+            _between(_f64(bits(qo)[r]).reshape(x.shape), paged.rotate(x, pos.astype(np.float64), f, False),
+                     paged.partner_sum(x, rotary, False) * 2.0 ** -20, _bf16)
+            _between(_f64(bits(ko)[r]).reshape(vals[0].shape), vals[0], slack[0], _bf16)
+        for new, want, d, s in zip(after, vals, slack, (pool.ks, pool.vs)):
+            if kind == "bf16":
+                _between(_f64(new[at]), want, d, _bf16)
+            else:
+                sc = s.astype(np.float64)[:, None]
+                _between(LUT[new[at]], want / sc, d / sc + np.abs(want / sc) * 2.0 ** -22, paged.round_e4m3)
+    for new, old in zip(after, before):
+        assert np.array_equal(new[~stored], old[~stored])
+    if rotary:
+        rest = np.setdiff1d(np.arange(T), [t for t, _, _ in rows])
+        assert (qo.cpu()[rest] == 5).all() and (ko.cpu()[rest] == 5).all()
