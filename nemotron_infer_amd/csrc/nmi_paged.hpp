@@ -85,6 +85,11 @@ NMI_HD uint32_t range_first(uint32_t x, int c, uint32_t total) {
     return f < total ? (uint32_t)f : total;
 }
 
+// Whether tile `at` of that row is to be looked for among the 64 sequences after those from b0 on, up to
+// whose last the row has `upto` tiles.  Never past the batch, whatever the lengths: they are read again on
+// the way, and may by then be less than those that `at` was dealt by.
+NMI_HD bool look_on(uint32_t at, uint32_t upto, int b0, int batch) { return at >= upto && b0 + 64 < batch; }
+
 // The pieces of a sequence with tiles [first, first + tiles) of the row, one at least.  A workgroup all
 // of whose tiles are the sequence's takes them together, as one piece; of another, each wave takes a
 // piece.  So there are `head` waves' pieces of the first workgroup (from `wave` on), `joint` workgroups',

@@ -151,21 +151,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
             if (!MANY || w.b0 + 64 >= a.batch) break;
         }
     }
-    // the first sequence with tiles past `at`: its lane
+    // the first sequence with tiles past `at`: its lane; 64 where there is none (only if the lengths change
+    // under the launch)
     auto seek = [&](uint32_t at) {
         if constexpr (MANY)
-            while (at >= lane_u32(v.upto, 63)) v = load_lanes(a, v.b0 + 64, lane_u32(v.upto, 63), lane);
+            while (look_on(at, lane_u32(v.upto, 63), v.b0, a.batch))
+                v = load_lanes(a, v.b0 + 64, lane_u32(v.upto, 63), lane);
         return __popcll(__builtin_amdgcn_ballot_w64(v.upto <= at));
     };
     uint32_t at = range_first(blockIdx.x * kWaves, c, total), end = range_first((blockIdx.x + 1) * kWaves, c, total);
     if (at >= end) return;
     int i = seek(at);
+    if (MANY && i == 64) return;
     const bool joint = is_joint(blockIdx.x, lane_u32(v.upto - v.tiles, i), lane_u32(v.tiles, i), c, total);
     if (!joint) {
         at = range_first(me, c, total);
         end = range_first(me + 1, c, total);
         if (at >= end) return;
         i = seek(at);
+        if (MANY && i == 64) return;
     }
     constexpr int kStep = F::kTiles * kPagedTile;               // positions of a stage
     const int stride = joint ? kWaves * kStep : kStep;          // from one of a wave's stages to its next
@@ -225,6 +229,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         }
         if (at >= end) return false;
         i = seek(at);
+        if (MANY && i == 64) return false;
         open_piece();
         return true;
     };
