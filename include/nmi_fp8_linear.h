@@ -17,10 +17,12 @@
  * nmi_last_error() describes the last failure of the calling thread.
  * NMI_ERR_ASYNC reports a failure of an earlier launch on the device that the host learnt of
  * since (a stream-K GEMM that gave up waiting for a partial tile, see nmi_linear_fp8_w8a16_ws):
- * every entry point that launches a linear, a GEMM or a block, or works on a paged cache or packed
- * prompts (whose kernels report device data out of range the same way), returns it, launching nothing, at
+ * every entry point that launches a linear, a GEMM or a block returns it, launching nothing, at
  * its first call after that launch has finished; nmi_sync after synchronising, nmi_async_status
- * without synchronising.  Each such failure is reported once.
+ * without synchronising.  Each such failure is reported once.  Device data out of range that a call on
+ * a paged cache or on packed prompts met is reported the same way, by the entries that work on those and by
+ * nmi_sync and nmi_async_status; linears, GEMMs and blocks do not return it, nor those entries a
+ * GEMM's.
  *
  * Layouts: x row m starts at x + m*ldx elements; W row n at W + n*ldw bytes; y row m at
  * y + m*ldy elements.  Row-sliced calls pass offset pointers (W + r0*ldw, s + r0, y + r0)

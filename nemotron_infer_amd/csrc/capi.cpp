@@ -123,27 +123,25 @@ uint32_t* async_error_word(AsyncKind kind) {
     return (w && dev >= 0 && dev < kAsyncMaxDevices) ? w + (int)kind * kAsyncMaxDevices + dev : nullptr;
 }
 
-bool take_async_error(const char* fn) {
+bool take_async_error(const char* fn, AsyncKind kind) {
     uint32_t* w = g_async_words.load(std::memory_order_acquire);
     if (!w) return false;                           // no launch yet that could have one
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kAsyncMaxDevices) return false;
-    uint32_t* paged = w + (int)AsyncKind::Paged * kAsyncMaxDevices + dev;
-    if (__atomic_load_n(paged, __ATOMIC_ACQUIRE) != 0u) {
-        __atomic_store_n(paged, 0u, __ATOMIC_RELAXED);
+    w += (int)kind * kAsyncMaxDevices + dev;
+    if (__atomic_load_n(w, __ATOMIC_ACQUIRE) == 0u) return false;
+    __atomic_store_n(w, 0u, __ATOMIC_RELAXED);
+    if (kind == AsyncKind::Paged)
         set_last_error("%s: a call on a paged KV cache or on packed prompts launched earlier on device %d met device "
                        "data out of range: a page id outside the pool, a length or position that its row of the page "
                        "table does not hold, or sequence offsets that do not ascend within the rows given; nothing was "
                        "launched by this call",
                        fn, dev);
-        return true;
-    }
-    if (__atomic_load_n(w + dev, __ATOMIC_ACQUIRE) == 0u) return false;
-    __atomic_store_n(w + dev, 0u, __ATOMIC_RELAXED);
-    set_last_error("%s: a stream-K GEMM launched earlier on device %d gave up waiting for a partial tile, so that "
-                   "launch's output is wrong (the error word of its workspace, byte %d, is set; its flags were left "
-                   "re-armed); nothing was launched by this call",
-                   fn, dev, NMI_WS_ERROR_OFFSET);
+    else
+        set_last_error("%s: a stream-K GEMM launched earlier on device %d gave up waiting for a partial tile, so that "
+                       "launch's output is wrong (the error word of its workspace, byte %d, is set; its flags were left "
+                       "re-armed); nothing was launched by this call",
+                       fn, dev, NMI_WS_ERROR_OFFSET);
     return true;
 }
 
@@ -220,6 +218,11 @@ namespace {
 int dispatch(const uint16_t* x, int64_t ldx, int M, int K, GemvGroup* g, int ng, void* ws,
              size_t ws_bytes, hipStream_t st, const char* fn) {
     return hip_status(dispatch_linear(x, ldx, M, K, g, ng, ws, ws_bytes, st), fn);
+}
+
+// The status entries' own: of either kind, one at a time.
+bool take_any_async_error(const char* fn) {
+    return take_async_error(fn, AsyncKind::StreamK) || take_async_error(fn, AsyncKind::Paged);
 }
 
 int64_t total_rows(const nmi_linear_group* groups, int ngroups) {
@@ -539,9 +542,9 @@ int nmi_tuning_set(const char* knob, int value) {
 int nmi_sync(void) {
     const int rc = hip_status(hipDeviceSynchronize(), "hipDeviceSynchronize");
     if (rc) return rc;
-    return take_async_error("nmi_sync") ? NMI_ERR_ASYNC : NMI_OK;
+    return take_any_async_error("nmi_sync") ? NMI_ERR_ASYNC : NMI_OK;
 }
 
-int nmi_async_status(void) { return take_async_error("nmi_async_status") ? NMI_ERR_ASYNC : NMI_OK; }
+int nmi_async_status(void) { return take_any_async_error("nmi_async_status") ? NMI_ERR_ASYNC : NMI_OK; }
 
 }  // extern "C"

@@ -30,12 +30,14 @@ const DeviceInfo& device_info();
 // memory that it must not follow (nmi_paged.hpp).  async_error_word() returns the device's word of a
 // kind (allocated on first use, one array for the process; nullptr if that fails, and then the GEMM
 // does not use stream-K and the paged kernels report nothing).
-// take_async_error(fn) reads and clears one without synchronising the GPU; when one was set it
-// records a message naming fn and returns true (the caller returns NMI_ERR_ASYNC).
+// take_async_error(fn, kind) reads and clears one without synchronising the GPU; when it was set it
+// records a message naming fn and returns true (the caller returns NMI_ERR_ASYNC).  An entry takes the
+// kind that its own launches can set: another operator's error is no reason to refuse its call, and
+// would be lost to the caller that it concerns.
 enum class AsyncKind { StreamK = 0, Paged = 1 };
 constexpr int kAsyncKinds = 2;
 uint32_t* async_error_word(AsyncKind kind = AsyncKind::StreamK);
-bool take_async_error(const char* fn);
+bool take_async_error(const char* fn, AsyncKind kind = AsyncKind::StreamK);
 
 // Tuning knobs (0 = automatic).  Set through nmi_tuning_set() for sweeps; never needed for
 // correctness.

@@ -93,7 +93,7 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
                         const int32_t* cu_seqlens, const int32_t* start_pos, int batch, int tokens, int n_heads,
                         const float* inv_freq, int rotary_dim, int interleaved, void* stream) {
     const char* fn = "nmi_kv_append_paged";
-    if (take_async_error(fn)) return NMI_ERR_ASYNC;
+    if (take_async_error(fn, AsyncKind::Paged)) return NMI_ERR_ASYNC;
     AppendArgs a{};
     if (const int rc = check_cache(fn, cache, &a.kv)) return rc;
     if (!k_bf16 || !v_bf16 || !start_pos) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL k, v or start_pos", fn);
@@ -151,7 +151,7 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
                           const int32_t* kv_lens, int batch, int n_heads, float scale, void* workspace,
                           size_t workspace_bytes, void* stream) {
     const char* fn = "nmi_sdpa_decode_paged";
-    if (take_async_error(fn)) return NMI_ERR_ASYNC;
+    if (take_async_error(fn, AsyncKind::Paged)) return NMI_ERR_ASYNC;
     PagedDecodeArgs a{};
     if (const int rc = check_cache(fn, cache, &a.kv)) return rc;
     if (!q_bf16 || !o_bf16 || !kv_lens) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL q, o or kv_lens", fn);
@@ -199,7 +199,7 @@ int nmi_sdpa_prefill_packed_bf16(const void* q_bf16, int64_t ldq, const void* k_
                                  int64_t ldv, void* o_bf16, int64_t ldo, const int32_t* cu_seqlens, int batch, int tokens,
                                  int n_heads, int n_kv_heads, float scale, void* stream) {
     const char* fn = "nmi_sdpa_prefill_packed_bf16";
-    if (take_async_error(fn)) return NMI_ERR_ASYNC;
+    if (take_async_error(fn, AsyncKind::Paged)) return NMI_ERR_ASYNC;
     if (!q_bf16 || !k_bf16 || !v_bf16 || !o_bf16 || !cu_seqlens)
         return refuse(NMI_ERR_INVALID_ARG, "%s: NULL pointer argument", fn);
     if (batch < 1 || tokens < 1 || n_kv_heads < 1 || n_heads < n_kv_heads || n_heads % n_kv_heads)

@@ -1,11 +1,16 @@
 """Batched attention serving at its edges, without a GPU: the arithmetic that the kernels share with this
 host (nmi_paged.hpp), and the host code of the C ABI and of the torch front end."""
 import ctypes
+import json
+import os
 import subprocess
+import sys
 
 import pytest
 
 from nemotron_infer_amd import build
+from tests.conftest import ROOT
+from tests.test_host_runtime_cpu import PRELUDE
 
 SHIM = """
 #include "nmi_paged.hpp"
@@ -62,3 +67,79 @@ def test_the_search_for_a_tile_ends_within_the_batch(shared, batch):
                 assert upto - sum(now[b0:b0 + 64]) <= at < upto
             else:
                 assert b0 == (batch - 1) // 64 * 64
+
+
+# The stand-in for the HIP runtime of test_host_runtime_cpu.py, which also says where the library's host
+# memory is: one allocation, of an error word for each kind (a GEMM's, a paged call's) and device (64).
+WORDS_STUB = """
+#define hipHostMalloc plain_hipHostMalloc
+#include "hip_host_stub.cpp"
+#undef hipHostMalloc
+static void* g_host = nullptr;
+extern "C" int hipHostMalloc(void** p, size_t bytes, unsigned flags) {
+    if (g_host || bytes != 2 * 64 * 4) std::abort();
+    const int rc = plain_hipHostMalloc(p, bytes, flags);
+    g_host = *p;
+    return rc;
+}
+extern "C" uint32_t* stub_host_memory() { return static_cast<uint32_t*>(g_host); }
+"""
+
+WORDS_BODY = """
+hip.stub_host_memory.restype = ctypes.POINTER(ctypes.c_uint32)
+W, ST = 1 << 38, 1 << 12
+c = _lib.PagedKv(W, W, 8 * 16 * 128, 16 * 128, 128, W, 64, None, None, 0, 100, 16, 64, 8)
+def decode():
+    return L.nmi_sdpa_decode_paged(ctypes.addressof(c), W, 5120, W, 5120, W, 2, 40, 0.1, W, 1 << 30, ST)
+def append():
+    return L.nmi_kv_append_paged(ctypes.addressof(c), None, 0, W, 1024, W, 1024, None, 0, None, 0, None, W, 2, 2, 0, None, 0, 0, ST)
+def prefill():
+    return L.nmi_sdpa_prefill_packed_bf16(W, 5120, W, 1024, W, 1024, W, 5120, W, 2, 300, 40, 8, 0.1, ST)
+def linear():
+    return L.nmi_linear_fp8_w8a16(W, 3136, W, 3136, W, W, 3136, 1, 3136, 3136, ST)
+def gemv():
+    return L.nmi_gemv_fp8(W, W, W, W, 3136, 3136, ST)
+def mlp():
+    return L.nmi_mlp_forward_fp8(W, W, W, W, W, W, W, 1, 3136, 12544, 1e-5, W, 1 << 30, ST)
+def attn():
+    return L.nmi_attn_forward_fp8(W, W, W, W, W, W, W, W, W, W, W, 520, W, W, 520, 3136, 40, 8, 1e-5, W, 1 << 32, ST)
+gemm_side, paged_side = [linear, gemv, mlp, attn], [append, decode, prefill]
+for f in gemm_side + paged_side:
+    assert f() == 0, L.nmi_last_error()
+words = hip.stub_host_memory()
+GEMM, PAGED = 0, 64
+result = []
+for kind, mine, others in ((GEMM, gemm_side, paged_side), (PAGED, paged_side, gemm_side)):
+    for f in mine:
+        words[kind] = 1
+        hip.stub_take_log()
+        other = [g() for g in others]
+        ran = len(launches())
+        got = [f(), len(launches()), L.nmi_last_error().decode(), f()]
+        result.append([kind, other, ran, got])
+    for status in (L.nmi_async_status, L.nmi_sync):
+        words[kind] = 1
+        result.append([kind, [0], 1, [status(), 0, L.nmi_last_error().decode(), status()]])
+words[GEMM] = words[PAGED] = 1
+result.append([sorted([L.nmi_async_status(), L.nmi_async_status()]), L.nmi_async_status(), words[GEMM], words[PAGED]])
+"""
+
+
+def test_an_operators_error_is_returned_to_calls_of_its_kind(tmp_path):
+    """Bad device data of a paged call is reported to the next call on a paged cache or packed prompts and by
+    the status entries, once; linears and blocks are not refused for it, and a GEMM's error not taken
+    by the paged entries."""
+    (tmp_path / "words.cpp").write_text(WORDS_STUB)
+    stub = str(tmp_path / "libwords.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-shared", "-fPIC", f"-I{os.path.join(ROOT, 'tests')}",
+                    str(tmp_path / "words.cpp"), "-o", stub], check=True, timeout=120)
+    code = PRELUDE.format(stub=stub) + WORDS_BODY + "\nprint(json.dumps(result))\n"
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    *cases, both = json.loads(r.stdout.splitlines()[-1])
+    assert len(cases) == 4 + 3 + 4
+    for kind, other, ran, (rc, launched, why, again) in cases:
+        assert other == [0] * len(other) and ran >= len(other), (kind, other, ran)
+        assert rc == -6 and launched == 0 and again == 0
+        assert ("page" in why) == (kind == 64) and ("stream-K" in why) == (kind == 0)
+    assert both == [[-6, -6], 0, 0, 0]
