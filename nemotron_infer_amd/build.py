@@ -6,6 +6,7 @@ Produces
   nemotron_infer_amd/lib/libnmi.so                 HIP kernels + C ABI (include/nmi_fp8_linear.h)
   nemotron_infer_amd/csrc/binding<EXT_SUFFIX>      pybind11 module `binding` over the C ABI
   nemotron_infer_amd/csrc/front<EXT_SUFFIX>        torch front end of the batched attention operators
+                                                   (only where torch can be imported)
 
 Every HIP translation unit is compiled with ``--offload-arch=gfx950`` and with packed-fp32
 code generation disabled (``-Xclang -target-feature -Xclang -packed-fp32-ops``).  The build
@@ -99,8 +100,15 @@ def build_binding(verbose=False) -> str:
     return out
 
 
-def build_front(verbose=False) -> str:
-    import torch
+def build_front(verbose=False) -> str | None:
+    """The torch front end; None, and nothing built, where torch cannot be imported (the library and the
+    binding need none)."""
+    try:
+        import torch
+    except ImportError as e:
+        if verbose:
+            print(f"no torch ({e}): its front end is left out")
+        return None
 
     at = os.path.dirname(torch.__file__)
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
