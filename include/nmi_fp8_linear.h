@@ -454,7 +454,8 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
  * workspace: nmi_sdpa_decode_paged_workspace_bytes(batch, n_heads, n_kv_heads) bytes, 16-byte aligned,
  * no initialisation; NULL takes it from the bump allocator.  Two launches, the second joining the splits
  * in a fixed order: equal calls give the same bytes.  o overlaps no input.  Pages that are not attended may
- * hold anything; an attended infinity in v gives an infinity or NaN.
+ * hold anything; an attended infinity in v gives that infinity in its dim, or NaN beside one of the other
+ * sign (or where its weight underflows).
  */
 size_t nmi_sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv_heads);
 int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,

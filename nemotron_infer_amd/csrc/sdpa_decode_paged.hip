@@ -234,7 +234,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         return true;
     };
     open_piece();
-    const int piece_b = nx.b;           // (of a joint one)
+    const int piece_b = nx.b, piece_pos = nx.pos, piece_stop = nx.stop;    // (of a joint one)
     const bool piece_whole = nx.whole;
     bool bad = nx.bad;
     bool more = nx.pos < nx.stop;       // (a joint piece may have no stage for this wave)
@@ -290,6 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(tile + vrow * F::kRow + 16 * ch + 8 * (l16 & 1)));
     };
     bf16x8 qf[4];
+    int from = 0;                                   // the piece's first position
     float m = -FLT_MAX, l = 0.f;                    // of head l16 (l: this lane's positions)
     f32x4 oacc[8];                                  // O^T: 8 blocks of 16 dims x 16 heads
 #pragma unroll
@@ -407,11 +408,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         const float L = rows_sum(l);
         return bad ? NAN : L;
     };
+    // A value of v that is not finite makes NaN of its dim's sums by the weights' low parts (0 or negative), and
+    // by the rows past the last position.  Its weight is positive, so that a dim's values that are not
+    // finite, added up by themselves (an infinity, or NaN), are its sum: two dims a lane, over what the wave's
+    // stages from `pos` to `stop` have of sequence b; 0 for other dims.  It takes the place of what was stored.
+    // (The test of the sums costs 0.1 to 0.3 us of 8 to 50; an amended oacc in place of what was stored, which
+    // the compiler keeps twice, cost 0.5.)
+    auto odd_sums = [&]() __attribute__((always_inline)) -> bool {
+        if constexpr (E4M3) return false;
+        f32x4 sum = oacc[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) sum += oacc[i];
+        const bool odd = !(fabsf((sum[0] + sum[1]) + (sum[2] + sum[3])) < INFINITY);
+        return __builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0);
+    };
+    auto odd_values = [&](int b, int pos, int stop) __attribute__((always_inline)) {
+        const int32_t* row = a.kv.page_table + b * a.kv.table_stride;
+        float2 x{0.f, 0.f};
+        for (; pos < stop; pos += stride) {
+            bool none = false;          // (reported by the stage that met it)
+            const int page = checked_page(load_const(row + (pos >> a.kv.page_shift)), a.kv.n_pages, &none);
+            const uint8_t* vp = a.kv.v_pages + page * a.kv.page_stride + head_off + 4 * lane +
+                                (int64_t)(pos & page_mask) * a.kv.token_stride;
+#pragma unroll 4
+            for (int r = min(kPagedTile, stop - pos); r > 0; --r, vp += a.kv.token_stride) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(vp);
+                if ((w & 0x7F80u) == 0x7F80u) x.x += bf16lo_to_f32(w);
+                if ((w & 0x7F800000u) == 0x7F800000u) x.y += bf16hi_to_f32(w);
+            }
+        }
+        return x;
+    };
     auto finish = [&](const Stage& s) __attribute__((always_inline)) {
         const float L = row_sum();
-        if (l16 >= nrow) return;
         const int h = head0 + l16;
-        if (s.whole) {
+        if (l16 >= nrow) {
+        } else if (s.whole) {
             const float inv = vs / L;
             uint16_t* o = a.o + (int64_t)s.b * a.ldo + (int64_t)h * kD;
 #pragma unroll
@@ -426,6 +458,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
 #pragma unroll
             for (int b = 0; b < 8; ++b) *reinterpret_cast<f32x4*>(a.part_o + slot * kD + dim(b)) = four(b);
             if (g == 0) a.part_ml[slot] = float2{m * sc, L};
+        }
+        if (odd_sums()) {
+            const float2 x = odd_values(s.b, from, s.stop);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // the stores above, by other lanes
+#pragma unroll 1
+            for (int r = 0; r < nrow; ++r) {
+                const float Lr = __uint_as_float(lane_u32(__float_as_uint(L), r));
+                if (s.whole) {
+                    uint16_t* o = a.o + (int64_t)s.b * a.ldo + (int64_t)(head0 + r) * kD + 2 * lane;
+                    if (x.x != 0.f && Lr == Lr) o[0] = (uint16_t)(__float_as_uint(x.x) >> 16);
+                    if (x.y != 0.f && Lr == Lr) o[1] = (uint16_t)(__float_as_uint(x.y) >> 16);
+                } else {
+                    float* o = a.part_o + ((int64_t)(me + s.b) * a.H + head0 + r) * kD + 2 * lane;
+                    if (x.x != 0.f) o[0] = x.x;
+                    if (x.y != 0.f) o[1] = x.y;
+                }
+            }
         }
     };
 
@@ -445,6 +494,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
                 m = -FLT_MAX;
                 l = 0.f;
                 bad = s.overlong;
+                from = s.pos;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) qf[j] = s.q[j];
 #pragma unroll
@@ -475,6 +525,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         if (g == 0) {
             sm_m[wave * kCols + l16] = m;
             sm_l[wave * kCols + l16] = L;
+        }
+    }
+    if (odd_sums()) {
+        const float2 x = odd_values(piece_b, piece_pos, piece_stop);
+        __builtin_amdgcn_wave_barrier();        // (LDS writes of one wave are in order)
+#pragma unroll 1
+        for (int r = 0; r < nrow; ++r) {
+            float* o = sm_o + (wave * kCols + r) * kD + 2 * lane;
+            if (x.x != 0.f) o[0] = x.x;
+            if (x.y != 0.f) o[1] = x.y;
         }
     }
     __syncthreads();

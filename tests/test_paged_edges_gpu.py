@@ -89,3 +89,47 @@ def test_append_bad_offsets_are_cut_and_reported(kind, rotary, T, cu):
     if rotary:
         rest = np.setdiff1d(np.arange(T), [t for t, _, _ in rows])
         assert (qo.cpu()[rest] == 5).all() and (ko.cpu()[rest] == 5).all()
+
+
+INF, NINF = 0x7F80, 0xFF80
+
+
+@pytest.mark.parametrize("lens,H,n_kv,page", [([777], 40, 8, 16), ([1], 8, 2, 16), ([20, 33, 5], 6, 2, 16), ([20000, 33], 10, 2, 128),
+                                              ([5] * 70 + [900] + [17] * 9, 8, 2, 32), ([40] * 300, 17, 1, 16),
+                                              ([130] * 8, 8, 8, 64)],
+                         ids=["777", "1", "3 short", "20000", "80", "300", "8"])
+def test_decode_of_values_that_are_not_finite(lens, H, n_kv, page):
+    """Infinities and NaN in single dims of v, in the first, the last and other positions that are attended: those
+    dims' outputs are that infinity (of both signs: NaN) or NaN, as in the formula, since every weight is
+    positive; all others as without."""
+    announce("decode_not_finite", len(lens), max(lens), H, n_kv)
+    rng = np.random.default_rng(sum(lens))
+    pool = Pool(rng, lens, n_kv, page, "bf16")
+
+    def put(b, pos, head, dims, value):
+        pool.v[pool.table[b, pos // page], head, pos % page, dims] = value
+
+    for b, n in enumerate(lens):
+        if b % 3 == 1:
+            continue                                       # (sequences without)
+        put(b, n - 1, 0, [0, 127], INF)                     # whose row is read again for the rows past the end
+        put(b, 0, n_kv - 1, [1, 64], NINF)
+        put(b, n // 2, 0, [5, 6, 77], NINF)
+        put(b, n // 3, 0, [77], INF)                        # with the one before: NaN (but for one position)
+        put(b, int(rng.integers(0, n)), 0, [90], NAN_BF16)
+        put(b, int(rng.integers(0, n)), n_kv - 1, [33, 34], 0x7F7F)     # the largest finite value: stays as it is
+    pool.dv = pool._to_dev(pool.v)
+    q = _rand_bits(rng, len(lens), H * 128, scale=0.5)
+    o = pool.decode(_dev(q))
+    torch.cuda.synchronize()
+    K, V = pool.values()
+    with np.errstate(all="ignore"):
+        want = paged.decode(_f64(q).reshape(len(lens), H, 128), K, V, pool.table, pool.lens)
+        rounded = block.bf16_round_exact(np.where(np.isfinite(want), want, 0))
+    got = bits(o).reshape(want.shape)
+    assert np.array_equal(np.isnan(_f64(got)), np.isnan(want))
+    assert np.array_equal(np.isposinf(_f64(got)), np.isposinf(want)) and np.array_equal(np.isneginf(_f64(got)), np.isneginf(want))
+    assert (np.isinf(want).sum() > 0) and np.isfinite(want).mean() > 0.8
+    clean = np.isfinite(want)
+    assert_parity(got[clean], rounded[clean], "the others")
+    assert _lib.lib().nmi_async_status() == 0
