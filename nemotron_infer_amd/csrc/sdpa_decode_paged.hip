@@ -177,6 +177,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
     const float sc = a.scale2 * (E4M3 && a.kv.k_scale ? load_const(a.kv.k_scale + kvh) : 1.f);
     const float vs = E4M3 && a.kv.v_scale ? load_const(a.kv.v_scale + kvh) : 1.f;
     const float lazy = kLazy / sc;
+    // the maximum of nothing: times sc still finite
+    const float lowest = sc > 1.f ? -0x1p127f * __builtin_amdgcn_rcpf(sc) : -FLT_MAX;
     const int page_mask = (1 << a.kv.page_shift) - 1;
     const int64_t head_off = kvh * a.kv.head_stride;
 
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
     };
     bf16x8 qf[4];
     int from = 0;                                   // the piece's first position
-    float m = -FLT_MAX, l = 0.f;                    // of head l16 (l: this lane's positions)
+    float m = lowest, l = 0.f;                      // of head l16 (l: this lane's positions)
     f32x4 oacc[8];                                  // O^T: 8 blocks of 16 dims x 16 heads
 #pragma unroll
     for (int b = 0; b < 8; ++b) oacc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
             if (stage[k ^ 1].valid) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             if (s.first) {
-                m = -FLT_MAX;
+                m = lowest;
                 l = 0.f;
                 bad = s.overlong;
                 from = s.pos;

@@ -133,3 +133,28 @@ def test_decode_of_values_that_are_not_finite(lens, H, n_kv, page):
     clean = np.isfinite(want)
     assert_parity(got[clean], rounded[clean], "the others")
     assert _lib.lib().nmi_async_status() == 0
+
+
+@pytest.mark.parametrize("scale", [0.09, 0.5, 1.0, 2.5])
+@pytest.mark.parametrize("lens", [[777], [64, 300, 33], [2000, 5]], ids=["777", "3", "2000"])
+def test_decode_of_scores_of_minus_infinity(lens, scale):
+    """Positions whose score is minus infinity have no weight, also where a tile, or all that a wave has of a
+    sequence, holds no other, whatever the scale."""
+    announce("decode_minus_infinity", lens, scale)
+    rng = np.random.default_rng(60)
+    H, n_kv, page = 8, 2, 16
+    pool = Pool(rng, lens, n_kv, page, "bf16")
+    for b, n in enumerate(lens):
+        for pos in {*range(0, min(40, n - 1)), *range(96, min(260, n - 1)), *range(600, max(600, n - 1))}:
+            pool.k[pool.table[b, pos // page], :, pos % page] = 0
+            pool.k[pool.table[b, pos // page], :, pos % page, 0] = NINF
+    pool.dk = pool._to_dev(pool.k)
+    q = _rand_bits(rng, len(lens), H * 128, scale=0.3)
+    q.reshape(len(lens), H, 128)[:, :, 0] = block.bf16_round_exact(np.array([0.5]))[0]
+    o = pool.decode(_dev(q), scale=scale)
+    torch.cuda.synchronize()
+    K, V = pool.values()
+    with np.errstate(all="ignore"):
+        want = paged.decode(_f64(q).reshape(len(lens), H, 128), K, V, pool.table, pool.lens, scale=scale)
+    assert np.isfinite(want).all()
+    assert_parity(bits(o).reshape(want.shape), block.bf16_round_exact(want), f"scale {scale}")
