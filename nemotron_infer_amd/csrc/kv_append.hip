@@ -79,23 +79,6 @@ __device__ __forceinline__ bool find_sequence(const AppendArgs& a, int t, bool a
     return bad != 0;
 }
 
-// cos and sin of 2 pi f, |f| <= 1/2: f = q / 4 + y with |y| <= 1/8, the Taylor polynomials of y's angle
-// t, |t| <= pi / 4 (left out: t^13 / 13! < 7e-12, t^12 / 12! < 2e-10), turned by q quarters.
-__device__ __forceinline__ float2 cos_sin(double f) {
-    const double q = rint(4.0 * f), t = 6.283185307179586 * __builtin_fma(q, -0.25, f), z = t * t;
-    double s = __builtin_fma(z, -1.0 / 39916800.0, 1.0 / 362880.0), c = __builtin_fma(z, -1.0 / 3628800.0, 1.0 / 40320.0);
-    s = __builtin_fma(z, s, -1.0 / 5040.0);
-    c = __builtin_fma(z, c, -1.0 / 720.0);
-    s = __builtin_fma(z, s, 1.0 / 120.0);
-    c = __builtin_fma(z, c, 1.0 / 24.0);
-    s = __builtin_fma(z, s, -1.0 / 6.0);
-    c = __builtin_fma(z, c, -0.5);
-    const float sf = (float)__builtin_fma(t * z, s, t), cf = (float)__builtin_fma(z, c, 1.0);
-    const int k = (int)q;                                       // -2 .. 2
-    const float cs = (k & 1) ? sf : cf, sn = (k & 1) ? cf : sf;
-    return float2{((k + 1) & 2) ? -cs : cs, (k & 2) ? -sn : sn};
-}
-
 // parts: waves that share a token, BATCH its vectors (by 8) on their way at once.
 template <bool E4M3, int MODE, int BATCH>
 __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs a, int parts) {
@@ -169,7 +152,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs
     if constexpr (MODE != kPlain) {
         if (lane < a.rotary / 2) {
             const double turn = (double)pos * (double)a.inv_freq[lane] * 0.15915494309189535;   // 1 / (2 pi)
-            turns[wave][lane] = cos_sin(turn - rint(turn));
+            cos_sin(turn - rint(turn), &turns[wave][lane].x, &turns[wave][lane].y);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (a wave's own: no barrier)
         __builtin_amdgcn_wave_barrier();

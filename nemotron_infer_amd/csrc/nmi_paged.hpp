@@ -3,7 +3,7 @@
 //
 // The functions marked NMI_HD are plain arithmetic, also compiled for the host by the tests: every
 // address the kernels form from a value in device memory (a page id, a length, a sequence's offset)
-// goes through one of them.
+// goes through one of them.  So is the rotation's sine.
 #pragma once
 
 #include <stdint.h>
@@ -68,6 +68,31 @@ NMI_HD bool span_holds(int c0, int c1, int tokens, int t, int* place, bool* bad)
     const int n = checked_span(c0, c1, tokens, &first, bad);
     *place = t - first;
     return *place >= 0 && *place < n;
+}
+
+// cos and sin of 2 pi f, |f| <= 1/2: f = q / 4 + y with |y| <= 1/8, the Taylor polynomials of y's angle
+// t, |t| <= pi / 4, turned by q quarters.  In 64 bits, each rounded once at the end: what the polynomials leave
+// out (t^17 / 17! < 5e-17, t^16 / 16! < 2e-15) is less than 2^-48 of the value, so a result is the nearest
+// float but for values as close as that to the middle of two.
+NMI_HD void cos_sin(double f, float* cos_f, float* sin_f) {
+    const double q = __builtin_rint(4.0 * f), t = 6.283185307179586 * __builtin_fma(q, -0.25, f), z = t * t;
+    double s = __builtin_fma(z, -1.0 / 1307674368000.0, 1.0 / 6227020800.0);
+    double c = __builtin_fma(z, -1.0 / 87178291200.0, 1.0 / 479001600.0);
+    s = __builtin_fma(z, s, -1.0 / 39916800.0);
+    c = __builtin_fma(z, c, -1.0 / 3628800.0);
+    s = __builtin_fma(z, s, 1.0 / 362880.0);
+    c = __builtin_fma(z, c, 1.0 / 40320.0);
+    s = __builtin_fma(z, s, -1.0 / 5040.0);
+    c = __builtin_fma(z, c, -1.0 / 720.0);
+    s = __builtin_fma(z, s, 1.0 / 120.0);
+    c = __builtin_fma(z, c, 1.0 / 24.0);
+    s = __builtin_fma(z, s, -1.0 / 6.0);
+    c = __builtin_fma(z, c, -0.5);
+    const float sf = (float)__builtin_fma(t * z, s, t), cf = (float)__builtin_fma(z, c, 1.0);
+    const int k = (int)q;                                       // -2 .. 2
+    const float cs = (k & 1) ? sf : cf, sn = (k & 1) ? cf : sf;
+    *cos_f = ((k + 1) & 2) ? -cs : cs;
+    *sin_f = (k & 2) ? -sn : sn;
 }
 
 // Decode attention: tiles per wave when all sequences' tiles, `total` of them in a row, are dealt to at

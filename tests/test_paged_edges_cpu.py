@@ -6,6 +6,7 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 
 from nemotron_infer_amd import build
@@ -13,10 +14,18 @@ from tests.conftest import ROOT
 from tests.test_host_runtime_cpu import PRELUDE
 
 SHIM = """
+#include <cmath>
 #include "nmi_paged.hpp"
 extern "C" {
 int holds(int c0, int c1, int tokens, int t, int* place, int* bad) {
     bool b = false; int r = nmi::span_holds(c0, c1, tokens, t, place, &b); *bad = b; return r;
+}
+void turns(const double* f, long n, float* got, float* want) {
+    for (long i = 0; i < n; ++i) {
+        nmi::cos_sin(f[i], &got[2 * i], &got[2 * i + 1]);
+        const long double a = 6.283185307179586476925286766559L * f[i];
+        want[2 * i] = (float)cosl(a), want[2 * i + 1] = (float)sinl(a);
+    }
 }
 int look_on(unsigned at, unsigned upto, int b0, int batch) { return nmi::look_on(at, upto, b0, batch); }
 }
@@ -143,3 +152,22 @@ def test_an_operators_error_is_returned_to_calls_of_its_kind(tmp_path):
         assert rc == -6 and launched == 0 and again == 0
         assert ("page" in why) == (kind == 64) and ("stream-K" in why) == (kind == 0)
     assert both == [[-6, -6], 0, 0, 0]
+
+
+def test_the_rotations_sine_and_cosine_are_rounded_once(shared):
+    """Against the long double functions rounded to float32.  An error of up to 2^-48 before the rounding (the
+    polynomials' 2e-15 and some 64-bit roundings), to either side, crosses the middle of two floats, which are
+    2^-24 of the value apart at least, for 2^-23 of the values: 0.5 of the 4 million here."""
+    rng = np.random.default_rng(70)
+    f = np.concatenate([rng.uniform(-0.5, 0.5, 2_000_000), rng.uniform(-1, 1, 1000) * 2.0 ** rng.integers(-60, -2, 1000)])
+    f = np.concatenate([f, [0.0, -0.0]])
+    got, want = np.empty((len(f), 2), np.float32), np.empty((len(f), 2), np.float32)
+    at = lambda x: x.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    shared.turns(at(f), ctypes.c_long(len(f)), at(got), at(want))
+    off = got != want
+    assert off.sum() <= 3 and np.array_equal(got[off], np.nextafter(want[off], got[off]))
+    # the quarters and eighths of a turn, whose small sine or cosine is what 64 bits of 2 pi make of it
+    f = np.arange(-4, 5) / 8
+    got, want = got[:9], want[:9]
+    shared.turns(at(f), ctypes.c_long(9), at(got), at(want))
+    assert np.abs(got.astype(np.float64) - want).max() <= 2.0 ** -24
