@@ -82,6 +82,14 @@ int as_int(int64_t n, const char* name) {
     return (int)n;
 }
 
+// Whether two tensors of one shape lie alike: their strides, but for dimensions of one element, whose strides have
+// no meaning.
+bool lie_alike(const at::Tensor& a, const at::Tensor& b) {
+    for (int64_t i = 0; i < a.dim(); ++i)
+        if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+    return true;
+}
+
 // Pages [n_pages, n_kv_heads, page_size, 128] of any strides with contiguous head vectors, K and V alike.
 nmi_paged_kv paged_kv(PyObject* k_o, PyObject* v_o, PyObject* table_o, int64_t batch, PyObject* k_scale, PyObject* v_scale,
                       int64_t dev) {
@@ -92,9 +100,10 @@ nmi_paged_kv paged_kv(PyObject* k_o, PyObject* v_o, PyObject* table_o, int64_t b
     if (!e4m3 && k.scalar_type() != at::kBFloat16)
         refuse(PyExc_TypeError, std::string("pages must be bfloat16, float8_e4m3fn or uint8 codes, got ") +
                                     c10::toString(k.scalar_type()));
-    if (v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || v.strides() != k.strides())
+    if (v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || !lie_alike(k, v))
         bad_value("v_pages must be as k_pages (" + show(k) + "), got " + show(v));
-    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch || table.stride(1) != 1)
+    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch ||
+        (table.size(1) > 1 && table.stride(1) != 1))
         bad_value("page_table must be int32 [batch=" + num(batch) + ", max_pages] with contiguous rows, got " + show(table));
     on_device(k, "k_pages", dev);
     on_device(v, "v_pages", dev);

@@ -8,8 +8,9 @@ import sys
 
 import numpy as np
 import pytest
+import torch
 
-from nemotron_infer_amd import build
+from nemotron_infer_amd import build, ops
 from tests.conftest import ROOT
 from tests.test_host_runtime_cpu import PRELUDE
 
@@ -171,3 +172,25 @@ def test_the_rotations_sine_and_cosine_are_rounded_once(shared):
     got, want = got[:9], want[:9]
     shared.turns(at(f), ctypes.c_long(9), at(got), at(want))
     assert np.abs(got.astype(np.float64) - want).max() <= 2.0 ** -24
+
+
+def test_strides_of_dimensions_of_one_element_have_no_meaning():
+    """K and V of one KV head made in either order of heads and positions, and a page table of one page per
+    sequence whatever its column stride: valid (here refused only for not being on a GPU); strides that do
+    mean something still have to agree."""
+    k = torch.zeros(5, 1, 16, 128, dtype=torch.bfloat16)
+    v = torch.zeros(5, 16, 1, 128, dtype=torch.bfloat16).transpose(1, 2)
+    assert k.shape == v.shape and k.stride() != v.stride()
+    rows = torch.zeros(3, 128, dtype=torch.bfloat16)
+    lens = torch.zeros(3, dtype=torch.int32)
+    wide = torch.zeros(3, 4, dtype=torch.int32)
+    one = torch.zeros(3, dtype=torch.int32).as_strided((3, 1), (1, 3))
+    for pages in ((k, v), (v, k)):
+        for table in (wide, one):
+            with pytest.raises(ValueError, match="must be on a GPU"):
+                ops.sdpa_decode_paged(rows, *pages, table, lens)
+            with pytest.raises(ValueError, match="must be on a GPU"):
+                ops.kv_append_paged(rows, rows, *pages, table, lens)
+    other = torch.zeros(5, 2, 16, 128, dtype=torch.bfloat16)[:, :1]
+    with pytest.raises(ValueError, match="v_pages must be as k_pages"):
+        ops.sdpa_decode_paged(rows, k, other, wide, lens)

@@ -158,3 +158,24 @@ def test_decode_of_scores_of_minus_infinity(lens, scale):
         want = paged.decode(_f64(q).reshape(len(lens), H, 128), K, V, pool.table, pool.lens, scale=scale)
     assert np.isfinite(want).all()
     assert_parity(bits(o).reshape(want.shape), block.bf16_round_exact(want), f"scale {scale}")
+
+
+def test_one_kv_head_in_either_order_of_heads_and_positions():
+    """K and V whose strides differ only in the dimension of one KV head, a page table of one column with a
+    column stride of its own: the bytes of the plain layout."""
+    announce("one_kv_head")
+    rng = np.random.default_rng(61)
+    pool = Pool(rng, [40, 64, 7], 1, 64, "bf16")
+    q = _dev(_rand_bits(rng, 3, 6 * 128))
+    lens = _dev(pool.lens)
+    want = pool.decode(q)
+    other = pool.dv.transpose(1, 2).contiguous().transpose(1, 2)
+    other = other.as_strided(other.shape, (64 * 128, 128, 128, 1))
+    assert other.stride() != pool.dk.stride()
+    table = pool.dtable[:, 0].contiguous().as_strided((3, 1), (1, 3))
+    assert torch.equal(ops.sdpa_decode_paged(q, pool.dk, other, table, lens).view(torch.int16), want.view(torch.int16))
+    k, v = (_dev(_rand_bits(rng, 3, 128)) for _ in range(2))
+    at = _dev(np.array([40, 5, 7], np.int32))
+    ops.kv_append_paged(k, v, pool.dk, other, table, at)
+    ids = pool.dtable[:, 0].long()
+    assert torch.equal(pool.dk[ids, 0, at.long()], k) and torch.equal(other[ids, 0, at.long()], v)
