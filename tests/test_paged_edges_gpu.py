@@ -179,3 +179,63 @@ def test_one_kv_head_in_either_order_of_heads_and_positions():
     ops.kv_append_paged(k, v, pool.dk, other, table, at)
     ids = pool.dtable[:, 0].long()
     assert torch.equal(pool.dk[ids, 0, at.long()], k) and torch.equal(other[ids, 0, at.long()], v)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("batch", [65, 200, 700])
+def test_decode_bad_pages_and_lengths_of_many_sequences(kind, batch):
+    """More sequences than lanes: pages outside the pool and lengths past the table give NaN in their own
+    sequences, wherever those are, the others the same bytes, and one report."""
+    announce("decode_many_bad", kind, batch)
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(1, 90, batch)
+    lens[[0, batch // 2, batch - 1]] = 150, 400, 95
+    width = 30
+    pool = Pool(rng, lens, 2, 16, kind, width=width)
+    q = _dev(_rand_bits(rng, batch, 8 * 128))
+    good = bits(pool.decode(q))
+    assert _lib.lib().nmi_async_status() == 0
+    for pages, longs in (([0], []), ([batch - 1], []), ([], [batch - 1]), ([3, 64, batch // 2], [1, batch - 2])):
+        table, now = pool.table.copy(), pool.lens.copy()
+        for i, b in enumerate(pages):
+            table[b, (lens[b] - 1) // 16] = pool.k.shape[0] + i if i % 2 == 0 else -5
+        for b in longs:
+            now[b] = width * 16 + 1 if b % 2 else 2 ** 31 - 1
+            table[b] = table[b, 0]                          # (the whole of its row is read)
+        keep, pool.dtable = pool.dtable, _dev(table)
+        got = bits(pool.decode(q, lens=now))
+        pool.dtable = keep
+        torch.cuda.synchronize()
+        assert _lib.lib().nmi_async_status() == _lib.NMI_ERR_ASYNC and _lib.lib().nmi_async_status() == 0
+        bad = np.zeros(batch, bool)
+        bad[pages + longs] = True
+        assert np.isnan(_f64(got[bad])).all()
+        if longs:                                          # (a longer row deals the tiles out anew)
+            assert_parity(got[~bad], good[~bad], f"{pages} {longs}")
+        else:
+            assert np.array_equal(got[~bad], good[~bad])
+    assert np.array_equal(bits(pool.decode(q)), good)
+
+
+@pytest.mark.parametrize("T,cu", [(T, cu) for T, cu in BAD_OFFSETS], ids=[str(i) for i in range(len(BAD_OFFSETS))])
+def test_prefill_bad_offsets_leave_right_rows(T, cu):
+    """What is left of offsets cut to the rows is attended as prompts of that length; the rows of no sequence
+    stay as they were.  A row that falling offsets give to several sequences is one of theirs: not compared."""
+    announce("packed_bad_rows", T, cu[:8])
+    rng = np.random.default_rng(T + len(cu))
+    H, n_kv = 4, 2
+    q, k, v = (_rand_bits(rng, T, n * 128) for n in (H, n_kv, n_kv))
+    out = torch.full((T, H * 128), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.sdpa_prefill_packed_bf16(_dev(q), _dev(k), _dev(v), _dev(np.array(cu)), H, n_kv, out=out)
+    torch.cuda.synchronize()
+    assert _lib.lib().nmi_async_status() == _lib.NMI_ERR_ASYNC and _lib.lib().nmi_async_status() == 0
+    spans = _cut(cu, T)
+    of = np.array([sum(a <= t < b for a, b in spans) for t in range(T)])
+    got = bits(out).reshape(T, H, 128)
+    assert (out.cpu()[of == 0] == 3).all()
+    for a, b in spans:
+        if b > a:
+            want = paged.prefill(*(_f64(x[a:b]).reshape(b - a, -1, 128) for x in (q, k, v)), [0, b - a])
+            mine = of[a:b] == 1
+            if mine.any():
+                assert_parity(got[a:b][mine], block.bf16_round_exact(want[mine]), f"{cu[:8]} {a}:{b}")
