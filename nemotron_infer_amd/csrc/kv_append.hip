@@ -56,27 +56,34 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float (&x)[8], float s) {
     return uint2{(uint32_t)a, (uint32_t)b};
 }
 
-// The sequence of packed row t and t's place in it, 64 sequences at a time; *b = -1 where no sequence has
-// the row, the first of several that do (offsets that fall).  `all`: look through every sequence's
-// offsets, also behind the row's.  Whether any looked at were out of order or range.
-__device__ __forceinline__ bool find_sequence(const AppendArgs& a, int t, bool all, int lane, int* b, int* place) {
-    uint64_t bad = 0;
-    *b = -1;
+// The sequence of packed row t and t's place in it, 64 sequences at a time: the first of several that have the
+// row (offsets that fall), -1 where none has.
+__device__ __forceinline__ int find_sequence(const AppendArgs& a, int t, int lane, int* place) {
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const int i = b0 + lane;
-        int at = 0;
-        bool off = false;
-        const bool mine = i < a.batch && span_holds(a.cu[i], a.cu[i + 1], a.tokens, t, &at, &off);
-        bad |= __builtin_amdgcn_ballot_w64(off);
-        const uint64_t holds = __builtin_amdgcn_ballot_w64(mine);
-        if (holds && *b < 0) {
-            const int who = __builtin_ctzll(holds);
-            *b = b0 + who;
-            *place = __builtin_amdgcn_readlane(at, who);
+        int c0 = 0;
+        bool mine = false;
+        if (i < a.batch) {
+            c0 = a.cu[i];
+            mine = span_holds(c0, a.cu[i + 1], t);
         }
-        if (*b >= 0 && !all) break;
+        if (const uint64_t holds = __builtin_amdgcn_ballot_w64(mine)) {
+            const int who = __builtin_ctzll(holds);
+            *place = span_place(__builtin_amdgcn_readlane(c0, who), t);
+            return b0 + who;
+        }
     }
-    return bad != 0;
+    return -1;
+}
+// Reports offsets out of order or range.  The work of a wave of its own, behind those of the tokens: in theirs
+// the checks cost 150 to 600 tokens 0.2 us of 4 to 7.
+__device__ __forceinline__ void check_offsets(const AppendArgs& a, int lane) {
+    bool bad = false;
+    for (int i = lane; i < a.batch; i += 64) {
+        int first;
+        checked_span(a.cu[i], a.cu[i + 1], a.tokens, &first, &bad);
+    }
+    if (bad && a.kv.error) __hip_atomic_store(a.kv.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 // parts: waves that share a token, BATCH its vectors (by 8) on their way at once.
@@ -87,7 +94,10 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t job = (int64_t)blockIdx.x * kWaves + wave;
     const int t = (int)(job / parts), part = (int)(job - (int64_t)t * parts);
-    if (t >= a.tokens) return;
+    if (t >= a.tokens) {
+        if (a.cu && t == a.tokens && part == 0) check_offsets(a, lane);
+        return;
+    }
 
     // the lane's two times 8 dims in a vector that is rotated, and in one that is not
     const int turning = a.rotary / 16;                          // lanes of a vector that rotate (halves)
@@ -114,39 +124,31 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs
     load(part);
 
     int b = t, place = 0;
-    bool bad = false;                                           // device data out of range
-    auto report = [&]() {
-        if (bad && lane == 0 && a.kv.error)
-            __hip_atomic_store(a.kv.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-    };
-    // (not before the page's id is here: behind a store the compiler takes no more uniform values through
-    // the scalar cache, and an eager call of 8191 tokens takes 55.1 us instead of 52.4)
     if (a.cu) {
-        // (the last row's wave looks through all offsets: it goes the farthest anyway)
-        bad = find_sequence(a, t, part == 0 && t == a.tokens - 1, lane, &b, &place);
-        if (b < 0) return report();                             // rows of no sequence
+        b = find_sequence(a, t, lane, &place);
+        if (b < 0) return;                                      // rows of no sequence
     }
-    const int start = a.start[b];
-    if (start < 0) return report();                             // a sequence that is not in use
+    const int start = load_const(a.start + b);
+    if (start < 0) return;                                      // a sequence that is not in use
     const int64_t pos = (int64_t)start + place;
 
     // where the token goes; nowhere if the table has no page for it
     uint8_t *kp = nullptr, *vp = nullptr;
     {
-        bool nowhere = false;
+        bool bad = false;
         const int64_t entry = pos >> a.kv.page_shift;
         int page = 0;
         if (entry < a.kv.max_pages)
-            page = checked_page(a.kv.page_table[b * a.kv.table_stride + entry], a.kv.n_pages, &nowhere);
+            page = checked_page(load_const(a.kv.page_table + b * a.kv.table_stride + entry), a.kv.n_pages, &bad);
         else
-            nowhere = true;
-        if (!nowhere) {
+            bad = true;
+        if (!bad) {
             const int64_t off = page * a.kv.page_stride + (pos & ((1 << a.kv.page_shift) - 1)) * a.kv.token_stride;
             kp = a.kv.k_pages + off;
             vp = a.kv.v_pages + off;
+        } else if (lane == 0 && a.kv.error) {
+            __hip_atomic_store(a.kv.error, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
-        bad |= nowhere;
-        report();
     }
     float c[8], s[8];                                           // of the lane's pairs
     if constexpr (MODE != kPlain) {
@@ -230,7 +232,8 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_kernel(const AppendArgs
 
 template <bool E4M3, int BATCH>
 void launch(const AppendArgs& a, int parts, hipStream_t stream) {
-    const dim3 grid((uint32_t)(((int64_t)a.tokens * parts + kWaves - 1) / kWaves)), block(64 * kWaves);
+    const int64_t jobs = (int64_t)a.tokens * parts + (a.cu ? 1 : 0);         // and the offsets' check
+    const dim3 grid((uint32_t)((jobs + kWaves - 1) / kWaves)), block(64 * kWaves);
     if (!a.rotary) hipLaunchKernelGGL((kv_append_kernel<E4M3, kPlain, BATCH>), grid, block, 0, stream, a, parts);
     else if (!a.interleaved) hipLaunchKernelGGL((kv_append_kernel<E4M3, kHalves, BATCH>), grid, block, 0, stream, a, parts);
     else hipLaunchKernelGGL((kv_append_kernel<E4M3, kInterleaved, BATCH>), grid, block, 0, stream, a, parts);

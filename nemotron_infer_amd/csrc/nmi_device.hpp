@@ -194,6 +194,12 @@ __device__ __forceinline__ float rows_sum(float v) {
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// Uniform values through the scalar cache, whatever the code around them writes.
+template <class T>
+__device__ __forceinline__ T load_const(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
+
 // 16-byte global load that bypasses the caches' retention policy (streamed weights).
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 load_stream16(const uint8_t* p) {

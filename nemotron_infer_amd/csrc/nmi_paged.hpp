@@ -62,13 +62,10 @@ NMI_HD int checked_span(int c0, int c1, int tokens, int* first, bool* bad) {
     return e - f;
 }
 
-// Whether packed row t is one of those of the sequence with offsets c0, c1, and then its place there.
-NMI_HD bool span_holds(int c0, int c1, int tokens, int t, int* place, bool* bad) {
-    int first = 0;
-    const int n = checked_span(c0, c1, tokens, &first, bad);
-    *place = t - first;
-    return *place >= 0 && *place < n;
-}
+// Whether packed row t, of the rows given, is one of those of the sequence with offsets c0, c1 so cut, and its
+// place there.
+NMI_HD bool span_holds(int c0, int c1, int t) { return c0 <= t && t < c1; }
+NMI_HD int span_place(int c0, int t) { return t - (c0 < 0 ? 0 : c0); }
 
 // cos and sin of 2 pi f, |f| <= 1/2: f = q / 4 + y with |y| <= 1/8, the Taylor polynomials of y's angle
 // t, |t| <= pi / 4, turned by q quarters.  In 64 bits, each rounded once at the end: what the polynomials leave

@@ -64,12 +64,6 @@ constexpr float kLazy = 8.f;                    // log2 of the largest unnormali
 
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Uniform values through the scalar cache, whatever the code around them writes.
-template <class T>
-__device__ __forceinline__ T load_const(const T* p) {
-    return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
-}
-
 // The row of all sequences' tiles, 64 sequences at a time in the lanes: those from b0 on, and the tiles
 // of theirs and of all before them, up to each.
 struct Lanes {

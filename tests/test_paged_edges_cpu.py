@@ -18,9 +18,9 @@ SHIM = """
 #include <cmath>
 #include "nmi_paged.hpp"
 extern "C" {
-int holds(int c0, int c1, int tokens, int t, int* place, int* bad) {
-    bool b = false; int r = nmi::span_holds(c0, c1, tokens, t, place, &b); *bad = b; return r;
-}
+int holds(int c0, int c1, int t) { return nmi::span_holds(c0, c1, t); }
+int place(int c0, int t) { return nmi::span_place(c0, t); }
+int span(int c0, int c1, int tokens, int* first) { bool b = false; return nmi::checked_span(c0, c1, tokens, first, &b); }
 void turns(const double* f, long n, float* got, float* want) {
     for (long i = 0; i < n; ++i) {
         nmi::cos_sin(f[i], &got[2 * i], &got[2 * i + 1]);
@@ -47,16 +47,15 @@ EDGES = [-2 ** 31, -2 ** 31 + 1, -5, -1, 0, 1, 2, 8, 9, 10, 11, 2 ** 30, 2 ** 31
 
 
 def test_a_row_is_only_of_a_sequence_whose_cut_offsets_hold_it(shared):
-    place, bad = ctypes.c_int(), ctypes.c_int()
+    first = ctypes.c_int()
     for tokens in (1, 10, 2 ** 31 - 1):
         for c0 in EDGES:
             for c1 in EDGES:
-                first, end = min(max(c0, 0), tokens), min(max(c1, 0), tokens)
+                n = shared.span(c0, c1, tokens, ctypes.byref(first))
                 for t in sorted({0, min(8, tokens - 1), min(9, tokens - 1), tokens - 1}):
-                    got = shared.holds(c0, c1, tokens, t, ctypes.byref(place), ctypes.byref(bad))
-                    assert bool(got) == (first <= t < end), (c0, c1, tokens, t)
-                    assert not got or place.value == t - first
-                    assert bool(bad.value) == (not 0 <= c0 <= c1 <= tokens)
+                    got = shared.holds(c0, c1, t)
+                    assert bool(got) == (first.value <= t < first.value + n), (c0, c1, tokens, t)
+                    assert not got or shared.place(c0, t) == t - first.value
 
 
 @pytest.mark.parametrize("batch", [1, 64, 65, 128, 129, 1000])
