@@ -16,8 +16,8 @@
 // of two times 8 dims each, BATCH times that on their way at once.  With halves paired a lane
 // holds the same 8 dims of both halves, so that a pair never leaves its lane.  The token's cosines are
 // computed once per wave, one per lane, while the vectors are on their way, and passed on through LDS.
-// Measured (40 / 8 heads, rotated; graph replays): one token 3.0-3.7 us, 8191 tokens into an e4m3 cache 50
-// us, 4.7 TB/s read and written (a large copy: 4.9); with a workgroup to a token, 8-byte rows and a
+// Measured (40 / 8 heads, rotated; graph replays): one token 3.0-3.7 us, 8191 tokens into an e4m3 cache 48
+// us, 4.9 TB/s read and written (a large copy: 4.9); with a workgroup to a token, 8-byte rows and a
 // float32 sine, 71 us.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
@@ -29,7 +29,11 @@ namespace nmi {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kBatch = 7;               // of 8 vectors: 40 query and 8 KV heads, k and v, at once
+// Times 8 vectors that a wave that takes several asks for at once: few registers and so more waves, which hide
+// more than longer batches do.  2 / 4 / 7 (graph replays, rotated): 8191 tokens of 40 / 8 heads into bf16
+// 51.0 / 50.9 / 54.6 us, into e4m3 48.2 / 48.8 / 52.1, of 32 / 8 44.4 / 45.4 / 49.1, of 16 / 4 24.8 / 25.8 / 25.9, 64
+// interleaved dims 59.3 / 59.9 / 59.4; k and v alone 14.3 / 14.2 / 15.0; 600 tokens 6.5 / 6.75 / 6.8.
+constexpr int kBatch = 2;
 enum { kPlain = 0, kHalves = 1, kInterleaved = 2 };
 
 __device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
@@ -244,8 +248,8 @@ void launch(const AppendArgs& a, int parts, hipStream_t stream) {
 hipError_t launch_kv_append(const AppendArgs& a, bool e4m3, hipStream_t stream) {
     // Few tokens: their vectors spread over up to 8 waves per CU, since latency is all there is; many: a
     // wave for a token, whose cosines are then computed once.  Parts 1 / 2 / 4 / 7 (40 / 8 heads, rotated,
-    // bf16): 128 tokens 6.7 / 5.2 / 4.6 / 4.2 us, 512 7.8 / 6.7 / 6.3 / 7.5, 1024 11.0 / 10.2 / 11.1 / 11.9,
-    // 2048 14.4 / 15.9 / 16.3 / 18.5, 8191 51 / 49 / 55 / 67.
+    // bf16): 128 tokens 6.0 / 4.7 / 3.9 / 3.6 us, 512 7.7 / 6.2 / 5.9 / 5.7, 1024 9.2 / 8.1 / 9.0 / 9.2,
+    // 2048 12.9 / 13.1 / 15.1 / 13.9, 8191 51.0 / 49.7 / 49.1 / 48.2 (into e4m3 47.4 / 46.5 / 48.0 / 51.1).
     const int passes = ((a.q ? a.H : 0) + 2 * a.kv.n_kv + 7) / 8;
     const int parts = std::min(passes, std::max(1, 8 * device_info().num_cu / a.tokens));
     if (parts == passes) {
