@@ -239,3 +239,52 @@ def test_prefill_bad_offsets_leave_right_rows(T, cu):
             mine = of[a:b] == 1
             if mine.any():
                 assert_parity(got[a:b][mine], block.bf16_round_exact(want[mine]), f"{cu[:8]} {a}:{b}")
+
+
+@pytest.mark.parametrize("lens", [[200, 40, 33, 300], [1], [129, 1000], [31] * 40], ids=["4", "1", "1000", "40"])
+def test_prefill_of_values_that_are_not_finite(lens):
+    """Infinities and NaN in single dims of v: the outputs of those dims are that infinity (of both signs: NaN) or
+    NaN from the value's row on, as in the formula, all others as without; early and late in a prompt, in
+    the first and the last rows of a wave's 32."""
+    announce("packed_not_finite_values", lens[:4])
+    rng = np.random.default_rng(sum(lens))
+    H, n_kv = 10, 2
+    T, cu = sum(lens), np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    q, k, v = (_rand_bits(rng, T, n * 128, scale=0.5 if n == H else 1.0) for n in (H, n_kv, n_kv))
+    for a, n in zip(cu, lens):
+        for at, dims, value in ((0, [0], INF), (n // 3, [127, 3], NINF), (n // 2, [3], INF), (min(31, n - 1), [8, 9], INF),
+                                (min(64, n - 1), [40], NAN_BF16), (n - 1, [128 + 5], NINF), (n // 4 // 32 * 32, [128 + 6], INF)):
+            v[a + at, dims] = value
+    o = ops.sdpa_prefill_packed_bf16(_dev(q), _dev(k), _dev(v), _dev(cu), H, n_kv)
+    torch.cuda.synchronize()
+    with np.errstate(all="ignore"):
+        want = paged.prefill(*(_f64(x).reshape(T, -1, 128) for x in (q, k, v)), cu)
+        rounded = block.bf16_round_exact(np.where(np.isfinite(want), want, 0))
+    got = bits(o).reshape(want.shape)
+    assert np.array_equal(np.isnan(_f64(got)), np.isnan(want))
+    assert np.array_equal(np.isposinf(_f64(got)), np.isposinf(want)) and np.array_equal(np.isneginf(_f64(got)), np.isneginf(want))
+    clean = np.isfinite(want)
+    assert_parity(got[clean], rounded[clean], "the others")
+
+
+@pytest.mark.parametrize("scale", [0.09, 1.0, 2.5])
+def test_prefill_of_scores_of_minus_infinity(scale):
+    """Keys whose score is minus infinity have no weight, also where all of a block's are; rows that see no
+    other key are NaN, as in the formula."""
+    announce("packed_minus_infinity", scale)
+    rng = np.random.default_rng(62)
+    H, n_kv, lens = 4, 2, [300, 70, 40]
+    T, cu = sum(lens), np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    q, k, v = (_rand_bits(rng, T, n * 128, scale=0.3 if n == H else 1.0) for n in (H, n_kv, n_kv))
+    q.reshape(T, H, 128)[:, :, 0] = block.bf16_round_exact(np.array([0.5]))[0]
+    for t in (*range(0, 40), *range(64, 200), 305, 380, 381, 409):
+        k[t] = 0
+        k[t, [0, 128]] = NINF
+    o = ops.sdpa_prefill_packed_bf16(_dev(q), _dev(k), _dev(v), _dev(cu), H, n_kv, scale=scale)
+    torch.cuda.synchronize()
+    with np.errstate(all="ignore"):
+        want = paged.prefill(*(_f64(x).reshape(T, -1, 128) for x in (q, k, v)), cu, scale=scale)
+    got = bits(o).reshape(want.shape)
+    assert np.isnan(want[:40]).all() and np.isfinite(want[40:]).all()
+    assert np.isnan(_f64(got[:40])).all()
+    assert_parity(got[40:], block.bf16_round_exact(want[40:]), f"scale {scale}")
