@@ -423,8 +423,9 @@ typedef struct nmi_paged_kv {
  * q [tokens, >= n_heads * 128], k and v [tokens, >= n_kv_heads * 128] (bf16, row strides ldq, ldk, ldv)
  * belongs to the sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1] (int32 [batch + 1]; NULL: one
  * token per sequence, b = t) and has position start_pos[b] + t - cu_seqlens[b] (start_pos int32
- * [batch]; a negative one marks a sequence that is not in use: nothing of it is read or written).
- * Rows outside [cu_seqlens[0], cu_seqlens[batch]) are left alone.
+ * [batch]; a negative one marks a sequence that is not in use).  Rows of sequences not in use and rows
+ * outside [cu_seqlens[0], cu_seqlens[batch]) may be read, but are not stored, and q_out and k_out are left as
+ * they were there.
  *   rotation   rotary_dim > 0 (a multiple of 16, at most 128) with inv_freq float32 [rotary_dim / 2]: the
  *              angle of pair i is position * inv_freq[i], formed in 64 bits; pairs are dims (i, i +
  *              rotary_dim / 2), or (2i, 2i + 1) where interleaved is not 0; (x, y) becomes
@@ -444,7 +445,8 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
 /*
  * Decode attention over a paged cache, one query token per sequence:
  *   o[b, h] = bf16( softmax_s(scale * q[b, h] . k_s) . v_s ),  s < kv_lens[b],
- * KV head h / (n_heads / n_kv_heads); float32 arithmetic.  Every length counts the positions attended,
+ * KV head h / (n_heads / n_kv_heads); sums, maxima and exponentials in float32, the softmax's weights rounded to
+ * 16 significant bits (two bf16 parts) for their product with v.  Every length counts the positions attended,
  * so a token just appended is included by a length that counts it (nmi_sdpa_decode_bf16 attends the
  * positions before the new one).  A length of 0 (or below) gives o = 0: the unused rows of a padded batch.
  * q [batch, >= n_heads * 128], o [batch, >= n_heads * 128] bf16, row strides ldq (multiple of 8) and
@@ -464,8 +466,8 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
 
 /*
  * Causal attention over packed prompts: nmi_sdpa_prefill_bf16 for each sequence b on rows [cu_seqlens[b],
- * cu_seqlens[b + 1]) of q, k, v and o, with softmax(scale * q . k), in one launch whose grid depends on
- * batch and tokens only.  cu_seqlens int32 [batch + 1], ascending (a sequence may be empty); rows of the
+ * cu_seqlens[b + 1]) of q, k, v and o, with softmax(scale * q . k) and weights rounded as above, in one
+ * launch whose grid depends on batch and tokens only.  cu_seqlens int32 [batch + 1], ascending (a sequence may be empty); rows of the
  * `tokens` given that belong to no sequence are left as they were.  Layouts, alignment and strides as
  * nmi_sdpa_prefill_bf16, strides at most 2^24; scale positive.  No workspace.  o overlaps no input.  A row
  * of k or v that is not finite reaches the rows of its sequence from its own on, and no others.

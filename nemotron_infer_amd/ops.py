@@ -681,7 +681,8 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     page_size, 128] bf16, or e4m3 (float8_e4m3fn or uint8 codes) with float32 scales per head;
     page_table int32 [batch, max_pages].  With inv_freq (float32 [rotary_dim / 2]) k is rotated by
     position, and q [T, n_heads * 128] too.  Returns (q_out, k_out): the rotated q (None without q)
-    and k_out, which receives the rotated k where it is given; either may be its input itself."""
+    and k_out, which receives the rotated k where it is given; either may be its input itself.  Rows of
+    no sequence, or of one that is not in use, are left as they were in both (in a new q_out: undefined)."""
     dev = k.get_device()
     if _elsewhere(dev):
         with torch.cuda.device(dev):
