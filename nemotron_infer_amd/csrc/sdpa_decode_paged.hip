@@ -33,9 +33,9 @@
 //   reads transpose pairs of dims, whose bytes are then sorted: the even dims of a block go to one
 //   product, the odd ones to the next.
 //
-// Measured (graph replays, both launches; 40 query, 8 KV heads): one sequence of 777 positions 8.8 us, of
-// 65536 46 (5.8 TB/s of the cache's bytes; a streaming read of as many 6.5); e4m3, 131072 positions 50
-// (5.4); 64 of 90 to 8000 positions, e4m3, 48 (5.0); 128 of 500 50 (5.3).  What is left of a long one is the
+// Measured (graph replays, both launches; 40 query, 8 KV heads): one sequence of 777 positions 8.4 us, of
+// 65536 45 (6.0 TB/s of the cache's bytes; a streaming read of as many 6.5); e4m3, 131072 positions 48.5
+// (5.5); 64 of 90 to 8000 positions, e4m3, 48.6 (4.9); 128 of 500 48.4 (5.4).  What is left of a long one is the
 // second launch and the gap before it (5 us), of a short one the two launches and the lengths, the
 // page's id and the tile read one after another.
 // Both sides of the choices, at 268 MB of cache: DMA past the caches 44 us, through them 50; eight waves per

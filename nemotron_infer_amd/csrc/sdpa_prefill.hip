@@ -48,9 +48,10 @@
 //
 // Packed prompts (the second instance of the kernel): the same body on the rows of one sequence, which
 // every wave looks up from the sequences' offsets on the device.  Measured (graph replays, 40 / 8 heads):
-// prompts of 8200 and 5000 tokens 1156 us (817 TFLOP/s; alone, one after the other 1184), 12 of up to 700 37
-// (alone 129), one of 33 6.7 (alone 6.0: the look-up).  Bounded as the single prompt is: power where they
-// are long; where they are short the first loads of q, K and V, 4 to 8 us, with few products beside them.
+// prompts of 8200 and 5000 tokens 1156 to 1318 us by the card and its clock (817 to 717 TFLOP/s; alone, one after
+// the other, 1184 where packed 1156), 12 of 33 to 700 37 to 39.5 (alone 129).  Bounded as the single prompt is:
+// power where they are long; where they are short the look-up and the first loads of q, K and V, 4 to 8 us, with
+// few products beside them.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 
@@ -662,7 +663,7 @@ __global__ __launch_bounds__(256, 2) void sdpa_prefill_kernel(const PrefillArgs 
         // attend all such values, their dims take the sum of those alone (an infinity, or NaN: the weights are
         // positive); where not, in the wave's last block of keys, its rows are done once more, one by one.  A row
         // whose scores are not finite, or are all minus infinity, has NaN by its sum l, and no others.
-        // 8200 and 5000 tokens, 40 / 8 heads: 1160 us, 2280 with a NaN in an early v, 5650 in a late one, 1180 in
+        // 8200 and 5000 tokens, 40 / 8 heads: 1180 us, 2280 with a NaN in an early v, 5650 in a late one, 1180 in
         // a k (with all rows of such waves one by one 91000, 5700, 91000).
         f32x4 sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
