@@ -384,7 +384,9 @@ int nmi_attn_forward_fp8(const void* input_bf16, const float* norm_w, const void
  *
  * A paged KV cache: k_pages and v_pages hold n_pages pages of page_size positions of n_kv_heads head
  * vectors of 128, as bf16 (NMI_KV_BF16) or OCP e4m3 codes (NMI_KV_E4M3, one byte) that stand for code *
- * k_scale[head], code * v_scale[head] (float32 [n_kv_heads], positive; NULL: 1; NULL for bf16).  Head h
+ * k_scale[head], code * v_scale[head] (float32 [n_kv_heads], positive; NULL: 1; NULL for bf16), or codes under a
+ * scale for each head and block of 16 positions (NMI_KV_E4M3_BLOCK): code * k_scale[page][head][(p % page_size) / 16]
+ * (float32 [n_pages, n_kv_heads, page_size / 16], positive; written by the append).  Head h
  * of position p of sequence b is at element
  *     page_table[b * page_table_stride + p / page_size] * page_stride + h * head_stride
  *         + (p % page_size) * token_stride
@@ -402,7 +404,7 @@ int nmi_attn_forward_fp8(const void* input_bf16, const float* norm_w, const void
  * offsets fall; a row that falling offsets give to several sequences is the first one's in the append and
  * any one's in the attention), and NMI_ERR_ASYNC reports it as described at the top of this file.
  */
-enum { NMI_KV_BF16 = 0, NMI_KV_E4M3 = 1 };
+enum { NMI_KV_BF16 = 0, NMI_KV_E4M3 = 1, NMI_KV_E4M3_BLOCK = 2 };
 typedef struct nmi_paged_kv {
     void* k_pages;
     void* v_pages;
@@ -433,14 +435,66 @@ typedef struct nmi_paged_kv {
  *              and inv_freq NULL: none (the framework's own model has none).
  *   cache      k rotated, v as it is: rounded once, to bf16, or divided by the head's scale (float32) to
  *              e4m3, to nearest even, values past +-448 as +-448, NaN as NaN.
+ *              NMI_KV_E4M3_BLOCK: k rotated is the float32 nearest to the rotation by the float32 sine and cosine.
+ *              A block's scale becomes the smallest power of two s, 2^-126 at least, with |x| <= 448 s for the
+ *              call's finite values x of the block, and no less than it was where places of the block before the
+ *              call's are in it (they hold earlier positions; a block whose first place is the call's begins
+ *              anew; a scale that was no power of two counts as the next one).  Codes are x / s to the nearest
+ *              even, NaN and infinities as NaN; where s grew the block's earlier codes become code * s_old / s to
+ *              the nearest even.  Bytes of places after the call's last one stay.
  *   q_out, k_out  the rotated q and k as bf16 (q and q_out both or neither; k_out for the attention over
  *              the prompt itself); each may be its input, else must not overlap anything.
- * No two tokens of a call may have the same place in the pool.  One launch, no workspace.
+ * No two tokens of a call may have the same place in the pool, nor, of NMI_KV_E4M3_BLOCK, two sequences of a call
+ * places in the same block of it.  (There, of offsets that fall, a row that precedes an earlier sequence's end is not
+ * stored.)  One launch, no workspace.
  */
 int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, const void* k_bf16, int64_t ldk,
                         const void* v_bf16, int64_t ldv, void* q_out_bf16, int64_t ldqo, void* k_out_bf16, int64_t ldko,
                         const int32_t* cu_seqlens, const int32_t* start_pos, int batch, int tokens, int n_heads,
                         const float* inv_freq, int rotary_dim, int interleaved, void* stream);
+
+/*
+ * Pages of a pool handed out on the device, so that a captured step goes on as sequences grow, start and end: those
+ * that a step's new tokens need, and those that come back from sequences that have ended.
+ *   lens [batch]        positions stored so far; negative: not in use
+ *   new_lens [batch]    new tokens of the step: 0 none; negative: the sequence has ended; NULL: one each
+ *   page_table          [batch, max_pages], the entries before ceil(lens / page_size) in use; those of the new
+ *                       pages are written, no others
+ *   free_pages [n_pages], free_count [1]   a stack of the pool's free pages: its first free_count entries
+ * The pages of ended sequences are pushed, in ascending order of the sequences and of their positions; then the pages
+ * for new tokens are popped in the same order.  A sequence in use with new tokens is granted all of them, or none: if
+ * they do not fit its row of the table, or if it needs pages and those needed up to it, by all that fit, are more than
+ * the stack holds.  What is not granted leaves the sequence as it was, for the caller to see (start_pos -1 in spite of
+ * new tokens); it is no error.
+ *   start_pos [batch]   lens where granted, -1 elsewhere: for nmi_kv_append_paged
+ *   kv_lens [batch]     lens + new_lens where granted, 0 elsewhere: for the decode attention
+ *   lens_out [batch]    lens + new_lens where granted, -1 where ended, lens elsewhere: lens of the next step (may be
+ *                       lens itself)
+ *   cu_seqlens [batch + 1]  packed offsets, max(new_lens, 0) rows each whether granted or not; NULL: one row per
+ *                       sequence (tokens = batch, and more than one new token is out of range)
+ *   slots [tokens]      of each row page * page_size + place, -1 where not granted and behind the last row
+ *   free_count_out [1]  the stack's new height (may be free_count itself)
+ * All int32 but slots (int64).  Out of range, and reported (NMI_ERR_ASYNC) by this entry's next call or another of the
+ * paged ones: free_count outside [0, n_pages] (cut), a length that the row cannot hold (cut where it has ended, else not
+ * granted), page ids outside [0, n_pages) where they are met (moved as they are; slot -1), more pages pushed than the
+ * stack holds (dropped), rows past `tokens` (cut, and not granted).  Outputs overlap each other and the inputs in no
+ * other way.  One launch, no workspace.
+ */
+int nmi_kv_assign_paged(const int32_t* lens, const int32_t* new_lens, int32_t* page_table, int64_t page_table_stride,
+                        int max_pages, int page_size, int32_t* free_pages, const int32_t* free_count, int n_pages, int batch,
+                        int tokens, int32_t* start_pos, int32_t* kv_lens, int32_t* cu_seqlens, int64_t* slots,
+                        int32_t* lens_out, int32_t* free_count_out, void* stream);
+
+/*
+ * The smallest and largest keys of pages: for every page that the new positions complete (start_pos, cu_seqlens and
+ * tokens as nmi_kv_append_paged takes them, whose call stores them before),
+ *   k_bounds[page][head][0][d] = min over the page's positions of k[d],  k_bounds[page][head][1][d] = max,
+ * bf16 [n_pages, n_kv_heads, 2, 128], 16-byte aligned, of the keys that the cache holds (code * scale in float32)
+ * rounded to nearest even; NaN in both where one of the keys has NaN.  Other pages' bounds stay.  The cache's v_pages
+ * and v_scale are not read.  One launch, no workspace.
+ */
+int nmi_kv_bounds_paged(const nmi_paged_kv* cache, void* k_bounds_bf16, const int32_t* cu_seqlens, const int32_t* start_pos,
+                        int batch, int tokens, void* stream);
 
 /*
  * Decode attention over a paged cache, one query token per sequence:
@@ -457,12 +511,32 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
  * no initialisation; NULL takes it from the bump allocator.  Two launches, the second joining the splits
  * in a fixed order: equal calls give the same bytes.  o overlaps no input.  Pages that are not attended may
  * hold anything; an attended infinity in v gives that infinity in its dim, or NaN beside one of the other
- * sign (or where its weight underflows).
+ * sign (or where its weight underflows).  Of NMI_KV_E4M3_BLOCK, scores and weights times their block's scale are rounded
+ * to float32 once more, and weights times v's scale have to lie within its range: magnitudes of v between 2^-100 and
+ * 2^110 do.
  */
 size_t nmi_sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv_heads);
 int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,
                           const int32_t* kv_lens, int batch, int n_heads, float scale, void* workspace,
                           size_t workspace_bytes, void* stream);
+
+/*
+ * The same over the pages of each sequence that a score selects, for each query token and KV head: of P pages all where
+ * P <= n_select, else the newest one and the n_select - 1 of the others with the largest
+ *   score[p] = max over the KV head's query heads h of f32( sum_d max(q_hd, 0) hi_d + min(q_hd, 0) lo_d ),
+ * lo and hi page p's k_bounds (nmi_kv_bounds_paged): the largest product that a key of the page can have with one of
+ * them.  Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds are not
+ * read.  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places in the sequence of the pages
+ * attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type; scale does not change the
+ * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first.
+ * workspace: nmi_sdpa_decode_paged_sparse_workspace_bytes(batch, n_heads, n_kv_heads, max_pages, n_select) bytes,
+ * 16-byte aligned, no initialisation; NULL takes it from the bump allocator.  Four launches; two where n_select >=
+ * max_pages.
+ */
+size_t nmi_sdpa_decode_paged_sparse_workspace_bytes(int batch, int n_heads, int n_kv_heads, int max_pages, int n_select);
+int nmi_sdpa_decode_paged_sparse(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,
+                                 const int32_t* kv_lens, const void* k_bounds_bf16, int n_select, int32_t* selected, int batch,
+                                 int n_heads, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Causal attention over packed prompts: nmi_sdpa_prefill_bf16 for each sequence b on rows [cu_seqlens[b],

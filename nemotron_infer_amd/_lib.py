@@ -54,6 +54,10 @@ SIGNATURES = {
     "nmi_kv_append_paged": ([_vp] + [_vp, _i64] * 5 + [_vp, _vp, _i, _i, _i, _vp, _i, _i, _vp], _i),
     "nmi_sdpa_decode_paged_workspace_bytes": ([_i] * 3, _sz),
     "nmi_sdpa_decode_paged": ([_vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _f, _vp, _sz, _vp], _i),
+    "nmi_kv_assign_paged": ([_vp, _vp, _vp, _i64, _i, _i, _vp, _vp, _i, _i, _i] + [_vp] * 7, _i),
+    "nmi_kv_bounds_paged": ([_vp, _vp, _vp, _vp, _i, _i, _vp], _i),
+    "nmi_sdpa_decode_paged_sparse_workspace_bytes": ([_i] * 5, _sz),
+    "nmi_sdpa_decode_paged_sparse": ([_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i, _vp, _i, _i, _f, _vp, _sz, _vp], _i),
     "nmi_sdpa_prefill_packed_bf16": ([_vp, _i64] * 4 + [_vp] + [_i] * 4 + [_f, _vp], _i),
     "nmi_tuning_set": ([ctypes.c_char_p, _i], _i),
     "nmi_alloc": ([_sz, ctypes.POINTER(_vp)], _i),
@@ -92,7 +96,7 @@ class GemvPhase(ctypes.Structure):
                 ("groups", LinearGroup * MAX_GROUPS)]
 
 
-NMI_KV_BF16, NMI_KV_E4M3 = 0, 1
+NMI_KV_BF16, NMI_KV_E4M3, NMI_KV_E4M3_BLOCK = 0, 1, 2
 
 
 class PagedKv(ctypes.Structure):

@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 
+#include <algorithm>
 #include <string>
 
 #include "nmi_fp8_linear.h"
@@ -90,6 +91,19 @@ bool lie_alike(const at::Tensor& a, const at::Tensor& b) {
     return true;
 }
 
+// Scales of blocks [n_pages, n_kv_heads, page_size / 16], contiguous.
+const float* block_scale(PyObject* o, const at::Tensor& pages, const char* name, int64_t dev) {
+    const at::Tensor& t = tensor(o, name);
+    const int64_t n = pages.size(0), heads = pages.size(1), blocks = pages.size(2) / 16;
+    if (t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(0) != n || t.size(1) != heads || t.size(2) != blocks ||
+        !t.is_contiguous())
+        bad_value(std::string(name) + " must be a contiguous float32 [n_pages=" + num(n) + ", n_kv_heads=" + num(heads) +
+                  ", page_size / 16=" + num(blocks) + "] tensor as the other scale, got " + show(t));
+    on_device(t, name, dev);
+    return static_cast<const float*>(t.data_ptr());
+}
+bool of_blocks(PyObject* scale) { return THPVariable_Check(scale) && THPVariable_Unpack(scale).dim() == 3; }
+
 // Pages [n_pages, n_kv_heads, page_size, 128] of any strides with contiguous head vectors, K and V alike.
 nmi_paged_kv paged_kv(PyObject* k_o, PyObject* v_o, PyObject* table_o, int64_t batch, PyObject* k_scale, PyObject* v_scale,
                       int64_t dev) {
@@ -119,9 +133,15 @@ nmi_paged_kv paged_kv(PyObject* k_o, PyObject* v_o, PyObject* table_o, int64_t b
     c.token_stride = k.size(2) > 1 ? k.stride(2) : 128;
     c.page_table = static_cast<const int32_t*>(table.data_ptr());
     c.page_table_stride = batch > 1 ? table.stride(0) : table.size(1);
-    c.k_scale = vector<float>(k_scale, k.size(1), at::kFloat, "k_scale", dev);
-    c.v_scale = vector<float>(v_scale, k.size(1), at::kFloat, "v_scale", dev);
-    c.kv_type = e4m3 ? NMI_KV_E4M3 : NMI_KV_BF16;
+    const bool blocks = of_blocks(k_scale) || of_blocks(v_scale);
+    if (blocks) {
+        c.k_scale = block_scale(k_scale, k, "k_scale", dev);
+        c.v_scale = block_scale(v_scale, k, "v_scale", dev);
+    } else {
+        c.k_scale = vector<float>(k_scale, k.size(1), at::kFloat, "k_scale", dev);
+        c.v_scale = vector<float>(v_scale, k.size(1), at::kFloat, "v_scale", dev);
+    }
+    c.kv_type = blocks ? NMI_KV_E4M3_BLOCK : e4m3 ? NMI_KV_E4M3 : NMI_KV_BF16;
     c.n_pages = as_int(k.size(0), "n_pages");
     c.page_size = as_int(k.size(2), "page_size");
     c.max_pages = as_int(table.size(1), "max_pages");
@@ -239,44 +259,230 @@ PyObject* kv_append_paged(PyObject* const* a) {
     return PyTuple_Pack(2, out.p, k_out);
 }
 
-// _lib.check, stream, entry, its workspace's size, workspace, kept, q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale,
-// scale, out -> out.  workspace(device, bytes, stream) -> (tensor, key), kept[key] = tensor after the launch.
-PyObject* sdpa_decode_paged(PyObject* const* a) {
-    const at::Tensor& q = tensor(a[6], "q");
-    const int64_t dev = q.get_device();
+// A call's transient device memory by ops.py's workspace(device, bytes, stream) -> (tensor, key); put back, kept[key] =
+// tensor, after the launch.
+struct Workspace {
+    Owned device, bytes, taken;
+    PyObject* kept;
+    static PyObject* take(PyObject* workspace, PyObject* device, PyObject* n, PyObject* stream) {
+        PyObject* argv[] = {device, n, stream};
+        return PyObject_Vectorcall(workspace, argv, 3, nullptr);
+    }
+    Workspace(PyObject* like, size_t need, PyObject* workspace, PyObject* kept, PyObject* stream)
+        : device(PyObject_GetAttrString(like, "device")), bytes(PyLong_FromSize_t(need)),
+          taken(take(workspace, device.p, bytes.p, stream)), kept(kept) {
+        if (!PyTuple_Check(taken.p) || PyTuple_GET_SIZE(taken.p) != 2) bad_value("workspace: (tensor, key) expected");
+    }
+    void* data() const { return tensor(PyTuple_GET_ITEM(taken.p, 0), "workspace").data_ptr(); }
+    void put_back() const {
+        PyObject* key = PyTuple_GET_ITEM(taken.p, 1);
+        if (key != Py_None && PyDict_SetItem(kept, key, PyTuple_GET_ITEM(taken.p, 0))) throw Raised{};
+    }
+};
+
+// The operands that the decode operators share.
+struct Decode {
+    nmi_paged_kv cache;
+    Rows q, o;
+    const int32_t* lens;
+    int batch, heads;
+    int64_t dev, cols;
+};
+Decode decode_operands(PyObject* q_o, PyObject* k, PyObject* v, PyObject* table, PyObject* lens, PyObject* k_scale,
+                       PyObject* v_scale, PyObject* out) {
+    const at::Tensor& q = tensor(q_o, "q");
+    Decode d;
+    d.dev = q.get_device();
     if (q.dim() != 2) bad_value("q must be [batch, n_heads * 128], got " + list(q.sizes()));
-    const int64_t batch = q.size(0), cols = q.size(1);
-    const nmi_paged_kv cache = paged_kv(a[7], a[8], a[9], batch, a[11], a[12], dev);
-    const int64_t H = query_heads(q, cache.n_kv_heads);
-    const Rows qr = rows(q, batch, cols, "q", dev);
-    tensor(a[10], "kv_lens");
-    const int32_t* lens = vector<int32_t>(a[10], batch, at::kInt, "kv_lens", dev);
-    Rows orow;
-    if (a[14] != Py_None) orow = rows(a[14], batch, cols, "out", dev);
+    const int64_t batch = q.size(0);
+    d.cols = q.size(1);
+    d.cache = paged_kv(k, v, table, batch, k_scale, v_scale, d.dev);
+    const int64_t H = query_heads(q, d.cache.n_kv_heads);
+    d.q = rows(q, batch, d.cols, "q", d.dev);
+    tensor(lens, "kv_lens");
+    d.lens = vector<int32_t>(lens, batch, at::kInt, "kv_lens", d.dev);
+    if (out != Py_None) d.o = rows(out, batch, d.cols, "out", d.dev);
+    d.batch = as_int(batch, "batch");
+    d.heads = as_int(H, "n_heads");
+    return d;
+}
+
+// _lib.check, stream, entry, its workspace's size, workspace, kept, q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale,
+// scale, out -> out
+PyObject* sdpa_decode_paged(PyObject* const* a) {
+    Decode d = decode_operands(a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[14]);
+    const at::Tensor& q = THPVariable_Unpack(a[6]);
     on_gpu(q);
     const float scale = scale_of(a[13]);
-    Owned out(output(a[14], q, batch, cols));
-    if (a[14] == Py_None) orow = {THPVariable_Unpack(out.p).data_ptr(), cols};
-    if (batch) {
+    Owned out(output(a[14], q, d.batch, d.cols));
+    if (a[14] == Py_None) d.o = {THPVariable_Unpack(out.p).data_ptr(), d.cols};
+    if (d.batch) {
         auto call = entry<decltype(&nmi_sdpa_decode_paged)>(a[2]);
         auto bytes = entry<decltype(&nmi_sdpa_decode_paged_workspace_bytes)>(a[3]);
         void* stream = stream_of(a[1]);
-        const int b = as_int(batch, "batch"), h = as_int(H, "n_heads");
-        const size_t need = bytes(b, h, cache.n_kv_heads);
-        Owned device(PyObject_GetAttrString(a[6], "device")), n(PyLong_FromSize_t(need));
-        PyObject* argv[] = {device.p, n.p, a[1]};
-        Owned taken(PyObject_Vectorcall(a[4], argv, 3, nullptr));
-        if (!PyTuple_Check(taken.p) || PyTuple_GET_SIZE(taken.p) != 2) bad_value("workspace: (tensor, key) expected");
-        PyObject *ws = PyTuple_GET_ITEM(taken.p, 0), *key = PyTuple_GET_ITEM(taken.p, 1);
-        void* ws_p = tensor(ws, "workspace").data_ptr();
+        const size_t need = bytes(d.batch, d.heads, d.cache.n_kv_heads);
+        const Workspace ws(a[6], need, a[4], a[5], a[1]);
+        void* ws_p = ws.data();
         int rc;
         Py_BEGIN_ALLOW_THREADS;
-        rc = call(&cache, qr.p, qr.ld, orow.p, orow.ld, lens, b, h, scale, ws_p, need, stream);
+        rc = call(&d.cache, d.q.p, d.q.ld, d.o.p, d.o.ld, d.lens, d.batch, d.heads, scale, ws_p, need, stream);
         Py_END_ALLOW_THREADS;
-        if (key != Py_None && PyDict_SetItem(a[5], key, ws)) throw Raised{};
+        ws.put_back();
         check(a[0], rc, "nmi_sdpa_decode_paged");
     }
     return new_ref(out.p);
+}
+
+// Bounds of keys [n_pages, n_kv_heads, 2, 128] bf16, contiguous.
+void* key_bounds(PyObject* o, const nmi_paged_kv& c, int64_t dev) {
+    const at::Tensor& t = tensor(o, "k_bounds");
+    if (t.scalar_type() != at::kBFloat16 || t.dim() != 4 || t.size(0) != c.n_pages || t.size(1) != c.n_kv_heads ||
+        t.size(2) != 2 || t.size(3) != 128 || !t.is_contiguous())
+        bad_value("k_bounds must be a contiguous bf16 [n_pages=" + num(c.n_pages) + ", n_kv_heads=" + num(c.n_kv_heads) +
+                  ", 2, 128] tensor, got " + show(t));
+    on_device(t, "k_bounds", dev);
+    return t.data_ptr();
+}
+// A Python whole number.
+int64_t whole(PyObject* o, const char* name) {
+    const long long n = PyLong_AsLongLong(o);
+    if (n == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        refuse(PyExc_TypeError, std::string(name) + " must be a whole number, got " + Py_TYPE(o)->tp_name);
+    }
+    return n;
+}
+
+// _lib.check, stream, entry, its workspace's size, workspace, kept, q, k_pages, v_pages, page_table, kv_lens, k_bounds, n_select,
+// k_scale, v_scale, scale, out, selected -> out
+PyObject* sdpa_decode_paged_sparse(PyObject* const* a) {
+    Decode d = decode_operands(a[6], a[7], a[8], a[9], a[10], a[13], a[14], a[16]);
+    const at::Tensor& q = THPVariable_Unpack(a[6]);
+    void* bounds = key_bounds(a[11], d.cache, d.dev);
+    const int64_t select = whole(a[12], "n_select");
+    if (select < 1 || select > INT32_MAX) bad_value("n_select=" + num(select) + " must be at least 1");
+    int32_t* selected = nullptr;
+    if (a[17] != Py_None) {
+        const at::Tensor& t = tensor(a[17], "selected");
+        if (t.scalar_type() != at::kInt || t.dim() != 3 || t.size(0) != d.batch || t.size(1) != d.cache.n_kv_heads ||
+            t.size(2) != select || !t.is_contiguous())
+            bad_value("selected must be a contiguous int32 [batch=" + num(d.batch) + ", n_kv_heads=" + num(d.cache.n_kv_heads) +
+                      ", n_select=" + num(select) + "] tensor, got " + show(t));
+        on_device(t, "selected", d.dev);
+        selected = static_cast<int32_t*>(t.data_ptr());
+    }
+    on_gpu(q);
+    const float scale = scale_of(a[15]);
+    Owned out(output(a[16], q, d.batch, d.cols));
+    if (a[16] == Py_None) d.o = {THPVariable_Unpack(out.p).data_ptr(), d.cols};
+    if (d.batch) {
+        auto call = entry<decltype(&nmi_sdpa_decode_paged_sparse)>(a[2]);
+        auto bytes = entry<decltype(&nmi_sdpa_decode_paged_sparse_workspace_bytes)>(a[3]);
+        void* stream = stream_of(a[1]);
+        const size_t need = bytes(d.batch, d.heads, d.cache.n_kv_heads, d.cache.max_pages, (int)select);
+        const Workspace ws(a[6], need, a[4], a[5], a[1]);
+        void* ws_p = ws.data();
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = call(&d.cache, d.q.p, d.q.ld, d.o.p, d.o.ld, d.lens, bounds, (int)select, selected, d.batch, d.heads, scale, ws_p,
+                  need, stream);
+        Py_END_ALLOW_THREADS;
+        ws.put_back();
+        check(a[0], rc, "nmi_sdpa_decode_paged_sparse");
+    }
+    return new_ref(out.p);
+}
+
+// _lib.check, stream, entry, k_pages, page_table, start_pos, k_bounds, cu_seqlens, tokens, k_scale -> k_bounds
+PyObject* kv_bounds_paged(PyObject* const* a) {
+    const at::Tensor &k = tensor(a[3], "k_pages"), &start = tensor(a[5], "start_pos");
+    const int64_t dev = k.get_device();
+    if (start.dim() != 1) bad_value("start_pos must be an int32 vector [batch], got " + list(start.sizes()));
+    const int64_t batch = start.size(0);
+    const int32_t* start_p = vector<int32_t>(a[5], batch, at::kInt, "start_pos", dev);
+    const nmi_paged_kv cache = paged_kv(a[3], a[3], a[4], batch, a[9], a[9], dev);
+    void* bounds = key_bounds(a[6], cache, dev);
+    const int32_t* cu = vector<int32_t>(a[7], batch + 1, at::kInt, "cu_seqlens", dev);
+    if ((a[7] == Py_None) != (a[8] == Py_None)) bad_value("cu_seqlens and tokens (its rows) go together");
+    const int64_t tokens = a[8] == Py_None ? batch : whole(a[8], "tokens");
+    if (tokens < 0) bad_value("tokens=" + num(tokens) + " is out of range");
+    on_gpu(k);
+    if (batch && tokens) {
+        auto call = entry<decltype(&nmi_kv_bounds_paged)>(a[2]);
+        void* stream = stream_of(a[1]);
+        const int b = as_int(batch, "batch"), n = as_int(tokens, "tokens");
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = call(&cache, bounds, cu, start_p, b, n, stream);
+        Py_END_ALLOW_THREADS;
+        check(a[0], rc, "nmi_kv_bounds_paged");
+    }
+    return new_ref(a[6]);
+}
+
+// _lib.check, stream, entry, lens, new_lens, page_table, free_pages, free_count, page_size, tokens, lens_out, free_count_out
+// -> (start_pos, kv_lens, cu_seqlens, slots, lens_out, free_count_out)
+PyObject* kv_assign_paged(PyObject* const* a) {
+    const at::Tensor &lens = tensor(a[3], "lens"), &table = tensor(a[5], "page_table"), &pages = tensor(a[6], "free_pages");
+    const int64_t dev = lens.get_device();
+    if (lens.dim() != 1) bad_value("lens must be an int32 vector [batch], got " + list(lens.sizes()));
+    const int64_t batch = lens.size(0);
+    const int32_t* lens_p = vector<int32_t>(a[3], batch, at::kInt, "lens", dev);
+    const int32_t* new_p = vector<int32_t>(a[4], batch, at::kInt, "new_lens", dev);
+    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != batch ||
+        (table.size(1) > 1 && table.stride(1) != 1))
+        bad_value("page_table must be int32 [batch=" + num(batch) + ", max_pages] with contiguous rows, got " + show(table));
+    on_device(table, "page_table", dev);
+    if (pages.dim() != 1) bad_value("free_pages must be an int32 vector [n_pages], got " + list(pages.sizes()));
+    int32_t* free_p = vector<int32_t>(a[6], pages.size(0), at::kInt, "free_pages", dev);
+    tensor(a[7], "free_count");
+    const int32_t* count_p = vector<int32_t>(a[7], 1, at::kInt, "free_count", dev);
+    const int page_size = as_int(whole(a[8], "page_size"), "page_size");
+    const bool packed = a[9] != Py_None;
+    const int64_t tokens = packed ? whole(a[9], "tokens") : batch;
+    if (tokens < 0) bad_value("tokens=" + num(tokens) + " is out of range");
+    int32_t* lens_out = vector<int32_t>(a[10], batch, at::kInt, "lens_out", dev);
+    int32_t* count_out = vector<int32_t>(a[11], 1, at::kInt, "free_count_out", dev);
+    if (!batch) bad_value("lens of no sequences");
+    if (packed && !new_p) bad_value("packed rows (tokens) need new_lens");
+    if (lens_out && new_p && lens_out == new_p) bad_value("lens_out must not be new_lens");
+    on_gpu(lens);
+    // one allocation for what is new: start_pos, kv_lens, cu_seqlens, lens_out, free_count_out
+    const auto ints = lens.options();
+    at::Tensor all = at::empty({3 * batch + (packed ? batch + 1 : 0) + 1}, ints);
+    int64_t at = 0;
+    auto part = [&](int64_t n) {
+        at += n;
+        return all.narrow(0, at - n, n);
+    };
+    const at::Tensor start = part(batch), kv = part(batch), cu = packed ? part(batch + 1) : at::Tensor();
+    const int64_t slot_rows = std::max<int64_t>(tokens, 1);     // (the C entry takes a row at least)
+    at::Tensor slots = at::empty({slot_rows}, ints.dtype(at::kLong));
+    Owned lens_o(lens_out ? new_ref(a[10]) : THPVariable_Wrap(part(batch)));
+    Owned count_o(count_out ? new_ref(a[11]) : THPVariable_Wrap(part(1)));
+    if (!lens_out) lens_out = static_cast<int32_t*>(THPVariable_Unpack(lens_o.p).data_ptr());
+    if (!count_out) count_out = static_cast<int32_t*>(THPVariable_Unpack(count_o.p).data_ptr());
+    {
+        auto call = entry<decltype(&nmi_kv_assign_paged)>(a[2]);
+        void* stream = stream_of(a[1]);
+        const int b = as_int(batch, "batch"), n = as_int(slot_rows, "tokens"), width = as_int(table.size(1), "max_pages");
+        const int n_pages = as_int(pages.size(0), "n_pages");
+        int32_t* table_p = static_cast<int32_t*>(table.data_ptr());
+        const int64_t stride = batch > 1 ? table.stride(0) : table.size(1);
+        int32_t *start_p = static_cast<int32_t*>(start.data_ptr()), *kv_p = static_cast<int32_t*>(kv.data_ptr());
+        int32_t* cu_p = packed ? static_cast<int32_t*>(cu.data_ptr()) : nullptr;
+        int64_t* slots_p = static_cast<int64_t*>(slots.data_ptr());
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = call(lens_p, new_p, table_p, stride, width, page_size, free_p, count_p, n_pages, b, n, start_p, kv_p, cu_p, slots_p,
+                  lens_out, count_out, stream);
+        Py_END_ALLOW_THREADS;
+        check(a[0], rc, "nmi_kv_assign_paged");
+    }
+    if (slot_rows != tokens) slots = slots.narrow(0, 0, tokens);
+    Owned start_o(THPVariable_Wrap(start)), kv_o(THPVariable_Wrap(kv)), slots_o(THPVariable_Wrap(slots));
+    Owned cu_o(packed ? THPVariable_Wrap(cu) : new_ref(Py_None));
+    return PyTuple_Pack(6, start_o.p, kv_o.p, cu_o.p, slots_o.p, lens_o.p, count_o.p);
 }
 
 // _lib.check, stream, entry, q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out -> out
@@ -319,6 +525,9 @@ PyCFunction method() {
 }
 PyMethodDef methods[] = {{"kv_append_paged", method<kv_append_paged, 17>(), METH_FASTCALL, nullptr},
                          {"sdpa_decode_paged", method<sdpa_decode_paged, 15>(), METH_FASTCALL, nullptr},
+                         {"sdpa_decode_paged_sparse", method<sdpa_decode_paged_sparse, 18>(), METH_FASTCALL, nullptr},
+                         {"kv_assign_paged", method<kv_assign_paged, 12>(), METH_FASTCALL, nullptr},
+                         {"kv_bounds_paged", method<kv_bounds_paged, 10>(), METH_FASTCALL, nullptr},
                          {"sdpa_prefill_packed_bf16", method<sdpa_prefill_packed_bf16, 11>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "front", "torch front end of the batched attention operators", -1, methods,

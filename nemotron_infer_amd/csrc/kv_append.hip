@@ -36,15 +36,6 @@ constexpr int kWaves = 4;
 constexpr int kBatch = 2;
 enum { kPlain = 0, kHalves = 1, kInterleaved = 2 };
 
-__device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
-    const uint32_t d[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(d[i]), x[2 * i + 1] = bf16hi_to_f32(d[i]);
-}
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-    return uint4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-}
-
 // x / s as an e4m3 code: to the nearest (ties to even), saturating; NaN stays
 __device__ __forceinline__ float to_e4m3_range(float x, float s) {
     const float y = x / s;

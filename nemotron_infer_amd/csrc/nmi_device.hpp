@@ -110,6 +110,16 @@ __device__ __forceinline__ uint32_t add_bf16x2(uint32_t v, uint32_t res) {
     return pack_bf16(bf16lo_to_f32(res) + bf16lo_to_f32(v), bf16hi_to_f32(res) + bf16hi_to_f32(v));
 }
 
+// Eight bf16 in 16 bytes as floats, and back (to the nearest even).
+__device__ __forceinline__ void unpack8(const uint4 v, float (&x)[8]) {
+    const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = bf16lo_to_f32(d[i]), x[2 * i + 1] = bf16hi_to_f32(d[i]);
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return uint4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+}
+
 __device__ __forceinline__ uint4 rms_scale8(const uint4 v, const float4 g0, const float4 g1, float r) {
     return uint4{pack_bf16(bf16lo_to_f32(v.x) * (r * g0.x), bf16hi_to_f32(v.x) * (r * g0.y)),
                  pack_bf16(bf16lo_to_f32(v.y) * (r * g0.z), bf16hi_to_f32(v.y) * (r * g0.w)),
@@ -167,14 +177,18 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false));
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+// Inclusive maxima over the 64 lanes.
+__device__ __forceinline__ uint32_t wave_scan_max_u32(uint32_t v) {
     v = dpp_max_u32<0x111, 0xF>(v);
     v = dpp_max_u32<0x112, 0xF>(v);
     v = dpp_max_u32<0x114, 0xF>(v);
     v = dpp_max_u32<0x118, 0xF>(v);
     v = dpp_max_u32<0x142, 0xA>(v);
     v = dpp_max_u32<0x143, 0xC>(v);
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan_max_u32(v), 63);
 }
 __device__ __forceinline__ uint32_t lane_u32(uint32_t v, int lane) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);

@@ -280,6 +280,48 @@ struct AppendArgs {
     bool interleaved;
 };
 hipError_t launch_kv_append(const AppendArgs& a, bool e4m3, hipStream_t stream);
+// The same into e4m3 under scales of blocks, which it sets (kv_append_block.hip).
+hipError_t launch_kv_append_block(const AppendArgs& a, hipStream_t stream);
+
+// The smallest and largest keys of the pages that new positions complete (kv_bounds.hip).
+struct BoundsArgs {
+    PagedKv kv;                 // its keys
+    uint16_t* bounds;           // [n_pages, n_kv, 2, 128] bf16
+    const int32_t* cu;          // [batch + 1] or nullptr: one position per sequence
+    const int32_t* start;       // [batch]
+    int batch, tokens;
+};
+hipError_t launch_kv_bounds(const BoundsArgs& a, KvForm form, hipStream_t stream);
+
+// Pages handed to sequences that grow and taken from those that end (kv_assign.hip).
+struct AssignArgs {
+    const int32_t* lens;        // [batch]
+    const int32_t* add;         // [batch] new tokens, negative: ended; nullptr: one each
+    int32_t* table;             // [batch, >= max_pages]
+    int64_t table_stride;
+    int32_t* free_pages;        // [n_pages], the first *free_count of them free
+    const int32_t* free_count;
+    int32_t *start, *kv_lens, *cu, *lens_out, *free_count_out;      // cu: nullptr where every sequence has a row
+    int64_t* slots;             // [tokens]
+    int n_pages, max_pages, page_shift, batch, tokens;
+    uint32_t* error;
+};
+hipError_t launch_kv_assign(const AssignArgs& a, hipStream_t stream);
+
+// The pages that new tokens attend, by their bounds (sdpa_select.hip).
+struct SelectArgs {
+    PagedKv kv;                 // its page table
+    const uint16_t* q;
+    int64_t ldq;
+    const int32_t* lens;        // [batch]
+    const uint16_t* bounds;     // [n_pages, n_kv, 2, 128] bf16
+    float* scores;              // [batch, n_kv, max_pages]
+    int32_t* rows;              // [batch, n_kv, select] the chosen pages' ids, or nullptr
+    int32_t* out_lens;          // [batch] positions in them, or nullptr
+    int32_t* selected;          // [batch, n_kv, select] their places in the sequence, then -1; or nullptr
+    int batch, group, select;
+};
+hipError_t launch_page_select(const SelectArgs& a, hipStream_t stream);
 
 // Decode attention over a paged cache (sdpa_decode_paged.hip): q [batch, ldq] against each sequence's
 // first lens[b] positions.
@@ -298,7 +340,7 @@ struct PagedDecodeArgs {
 };
 int sdpa_decode_paged_waves(int n_kv, int group);
 size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv);
-hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, bool e4m3, void* workspace, hipStream_t stream);
+hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, KvForm form, void* workspace, hipStream_t stream);
 
 // Mamba-2 mixer at decode (mamba_decode.hip): conv1d step + SiLU, SSM state update and
 // output, gated RMSNorm, for `batch` sequences of one token.  Shapes: H heads of P, G groups,

@@ -20,6 +20,8 @@ namespace nmi {
 constexpr int kPagedHead = 128;        // head dim
 constexpr int kPagedTile = 16;         // positions of a tile; a page holds a whole number of them
 constexpr int kPagedMinPage = kPagedTile, kPagedMaxPage = 1 << 20;
+constexpr int kPagedBlock = 16;        // positions under one scale (block scales)
+static_assert(kPagedBlock == kPagedTile, "a tile has one scale");
 
 // Strides in bytes.  A head's vector of position p of sequence b is at page_table[b][p >> page_shift]
 // * page_stride + head * head_stride + (p & (page_size - 1)) * token_stride.
@@ -33,7 +35,32 @@ struct PagedKv {
     const float* v_scale;
     int n_pages, max_pages, page_shift, n_kv;
     uint32_t* error;                    // host word to set where the device data is out of range, or nullptr
+    float* k_blocks;                    // [n_pages, n_kv, page_size / kPagedBlock] scales of blocks, or nullptr
+    float* v_blocks;
+    int64_t table_head_stride;          // entries from a KV head's row of a sequence's pages to the next (0: one row for all)
 };
+
+// What a cache holds: bf16, e4m3 codes under a scale per KV head, or under one per head and block.
+enum class KvForm { Bf16, E4m3, Block };
+
+// The scale of the block of a head that holds position `pos` of a page.
+NMI_HD int64_t block_index(int64_t page, int n_kv, int head, int page_shift, int pos) {
+    return ((page * n_kv + head) << (page_shift - 4)) + ((pos & ((1 << page_shift) - 1)) >> 4);
+}
+
+// The biased exponent of the smallest power of two s, normal, with amax <= 448 s, of the bits of a finite amax >= 0:
+// 448 is 1.75 2^8.  From 1 to 247.
+NMI_HD int block_exponent(uint32_t amax_bits) {
+    const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e < 1 ? 1 : e;
+}
+// That of the smallest power of two that is no less than a scale found in memory: itself, if an append wrote it.
+// Kept to what 2^-e can be had of, whatever the bits.
+NMI_HD int block_exponent_of_scale(uint32_t bits) {
+    const uint32_t b = bits & 0x7FFFFFFFu;
+    const int e = (int)(b >> 23) + ((b & 0x7FFFFFu) ? 1 : 0);
+    return e < 1 ? 1 : (e > 253 ? 253 : e);
+}
 
 // A page id from the table: itself, or page 0 with *bad set where the pool has no such page.
 NMI_HD int checked_page(int id, int n_pages, bool* bad) {
@@ -66,6 +93,40 @@ NMI_HD int checked_span(int c0, int c1, int tokens, int* first, bool* bad) {
 // place there.
 NMI_HD bool span_holds(int c0, int c1, int t) { return c0 <= t && t < c1; }
 NMI_HD int span_place(int c0, int t) { return t - (c0 < 0 ? 0 : c0); }
+
+// The rows of packed sequence b that are stored or counted, where `before` is the end of the earlier sequences' rows
+// (0 at first): [*first, *first + result), none of them an earlier sequence's.  *place: the first one's place in the
+// sequence.
+NMI_HD int later_span(int c0, int c1, int tokens, int before, int* first, int* place, bool* bad) {
+    int f = 0;
+    int n = checked_span(c0, c1, tokens, &f, bad);
+    *place = 0;
+    if (f < before) {
+        if (n > 0) *bad = true;
+        const int cut = before - f < n ? before - f : n;
+        *place = cut;
+        n -= cut;
+        f += cut;
+    }
+    *first = f;
+    return n;
+}
+
+// Blocks of kPagedBlock positions that n positions from `pos` on lie in.
+NMI_HD int blocks_of(int64_t pos, int n) { return n > 0 ? (int)(((pos & (kPagedBlock - 1)) + n + kPagedBlock - 1) / kPagedBlock) : 0; }
+// At most so many of `tokens` rows in `batch` sequences: each has 30 positions at most that are not its own in its blocks.
+NMI_HD int64_t most_blocks(int64_t tokens, int64_t batch) {
+    const int64_t n = batch < tokens ? batch : tokens, by = (tokens + 30 * n) / kPagedBlock;
+    return by < tokens ? by : tokens;
+}
+// Pages that n positions from `pos` on complete, and at most so many of `tokens` rows in `batch` sequences.
+NMI_HD int pages_completed(int64_t pos, int n, int page_shift) {
+    return n > 0 ? (int)(((pos + n) >> page_shift) - (pos >> page_shift)) : 0;
+}
+NMI_HD int64_t most_pages_completed(int64_t tokens, int64_t batch, int page_shift) {
+    const int64_t n = batch < tokens ? batch : tokens;
+    return (tokens >> page_shift) + n;
+}
 
 // cos and sin of 2 pi f, |f| <= 1/2: f = q / 4 + y with |y| <= 1/8, the Taylor polynomials of y's angle
 // t, |t| <= pi / 4, turned by q quarters.  In 64 bits, each rounded once at the end: what the polynomials leave

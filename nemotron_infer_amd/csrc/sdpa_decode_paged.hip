@@ -111,11 +111,13 @@ struct Stage {
     bool valid, first, last, whole;
     bool overlong, bad;     // the length is more than the table holds; a page that the pool does not have
     bf16x8 q[4];            // of a first one: this lane's head as the B operand
+    float ks[2], vs[2];     // block scales: of each tile
 };
 
 // MANY: more sequences than lanes.
-template <bool E4M3, bool MANY>
+template <KvForm FORM, bool MANY>
 __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const PagedDecodeArgs a) {
+    constexpr bool E4M3 = FORM != KvForm::Bf16, BLOCK = FORM == KvForm::Block;
     typedef Form<E4M3> F;
     typedef __attribute__((address_space(3))) void lds_void;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         nx.first = true;
         nx.whole = stop - at == tiles;
         nx.bad = (__builtin_amdgcn_ballot_w64(v.bad) >> i) & 1;
-        nx.row = a.kv.page_table + nx.b * a.kv.table_stride;
+        nx.row = a.kv.page_table + nx.b * a.kv.table_stride + kvh * a.kv.table_head_stride;
         at = stop;
         if (nx.pos < nx.stop) ask();
     };
@@ -253,6 +255,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         for (int t = 0; t < F::kTiles; ++t) {
             const int pos = nx.pos + t * kPagedTile < nx.stop ? nx.pos + t * kPagedTile : nx.pos;
             const int page = checked_page(nx.id[t], a.kv.n_pages, &s.bad);
+            if constexpr (BLOCK) {
+                const int64_t i = block_index(page, a.kv.n_kv, kvh, a.kv.page_shift, pos);
+                s.ks[t] = load_const(a.kv.k_blocks + i);
+                s.vs[t] = load_const(a.kv.v_blocks + i);
+            }
             const int64_t off = page * a.kv.page_stride + head_off + (int64_t)(pos & page_mask) * a.kv.token_stride;
             const uint8_t *kb = a.kv.k_pages + off, *vb = a.kv.v_pages + off;
             const uint32_t ls = lds0 + (uint32_t)((wave * kStages + slot) * kStage + t * F::kTile);
@@ -330,7 +337,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) st[t][k] = kPagedTile * t + k < left ? st[t][k] : -INFINITY;
+            for (int k = 0; k < 4; ++k)
+                st[t][k] = kPagedTile * t + k < left ? (BLOCK ? st[t][k] * s.ks[t] : st[t][k]) : -INFINITY;
         float top = fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3]));
         if constexpr (F::kTiles == 2)
             top = fmaxf(top, fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
@@ -353,6 +361,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
 #pragma unroll
             for (int k = 0; k < 4; ++k) p[k] = fexp2(__builtin_fmaf(st[t][k], sc, -mc));
             l += (p[0] + p[1]) + (p[2] + p[3]);
+            if constexpr (BLOCK)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) p[k] *= s.vs[t];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 hi[t][k] = pack_bf16(p[2 * k], p[2 * k + 1]);
@@ -419,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         return __builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0);
     };
     auto odd_values = [&](int b, int pos, int stop) __attribute__((always_inline)) {
-        const int32_t* row = a.kv.page_table + b * a.kv.table_stride;
+        const int32_t* row = a.kv.page_table + b * a.kv.table_stride + kvh * a.kv.table_head_stride;
         float2 x{0.f, 0.f};
         for (; pos < stop; pos += stride) {
             bool none = false;          // (reported by the stage that met it)
@@ -655,14 +666,14 @@ __global__ __launch_bounds__(64 * kWaves) void sdpa_decode_paged_join_kernel(con
     }
 }
 
-template <bool E4M3, bool MANY>
+template <KvForm FORM, bool MANY>
 hipError_t launch(const PagedDecodeArgs& a, hipStream_t stream) {
     static const hipError_t attr =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_decode_paged_kernel<E4M3, MANY>),
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_decode_paged_kernel<FORM, MANY>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return attr;
     const dim3 grid(a.waves / kWaves, a.kv.n_kv, (a.group + kCols - 1) / kCols);
-    hipLaunchKernelGGL((sdpa_decode_paged_kernel<E4M3, MANY>), grid, dim3(64 * kWaves), kLds, stream, a);
+    hipLaunchKernelGGL((sdpa_decode_paged_kernel<FORM, MANY>), grid, dim3(64 * kWaves), kLds, stream, a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     // Many sequences are in few pieces each, most in one: workgroups that find nothing to do are what it costs.
     const int heads = std::min(8, (int)(((int64_t)a.batch * a.H + 2047) / 2048));
@@ -694,15 +705,19 @@ size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv) {
     return layout(batch, n_heads, sdpa_decode_paged_waves(n_kv, n_heads / n_kv)).total;
 }
 
-hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, bool e4m3, void* workspace, hipStream_t stream) {
+hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, KvForm form, void* workspace, hipStream_t stream) {
     a.waves = sdpa_decode_paged_waves(a.kv.n_kv, a.group);
     const Layout w = layout(a.batch, a.H, a.waves);
     char* base = static_cast<char*>(workspace);
     a.part_o = reinterpret_cast<float*>(base + w.part_o);
     a.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
     a.plan = reinterpret_cast<Pieces*>(base + w.plan);
-    if (a.batch > 64) return e4m3 ? launch<true, true>(a, stream) : launch<false, true>(a, stream);
-    return e4m3 ? launch<true, false>(a, stream) : launch<false, false>(a, stream);
+    const bool many = a.batch > 64;
+    switch (form) {
+        case KvForm::Bf16: return many ? launch<KvForm::Bf16, true>(a, stream) : launch<KvForm::Bf16, false>(a, stream);
+        case KvForm::E4m3: return many ? launch<KvForm::E4m3, true>(a, stream) : launch<KvForm::E4m3, false>(a, stream);
+        default: return many ? launch<KvForm::Block, true>(a, stream) : launch<KvForm::Block, false>(a, stream);
+    }
 }
 
 }  // namespace nmi

@@ -9,6 +9,7 @@ include/nmi_fp8_linear.h; there is no torch or CPU fallback.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -698,7 +699,7 @@ def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
                       scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one token per sequence over a paged cache (nmi_sdpa_decode_paged): q
     [batch, n_heads * 128] bf16 against the first kv_lens[b] (int32) positions of sequence b's pages
-    (as kv_append_paged takes them); a length of 0 gives zeros.  scale: 1 / sqrt(128) unless given.
+    (as kv_append_paged takes them, scales too); a length of 0 gives zeros.  scale: 1 / sqrt(128) unless given.
     Returns o [batch, n_heads * 128] bf16."""
     dev = q.get_device()
     if _elsewhere(dev):
@@ -707,6 +708,71 @@ def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     call, entry, ws_bytes = _front("sdpa_decode_paged", "sdpa_decode_paged_workspace_bytes")
     return call(_lib.check, _stream() if dev >= 0 else 0, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
                 kv_lens, k_scale, v_scale, scale, out)
+
+
+def sdpa_decode_paged_sparse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                             kv_lens: torch.Tensor, k_bounds: torch.Tensor, n_select: int,
+                             k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                             scale: float | None = None, out: torch.Tensor | None = None,
+                             selected: torch.Tensor | None = None) -> torch.Tensor:
+    """sdpa_decode_paged over n_select pages of each sequence (nmi_sdpa_decode_paged_sparse), chosen for each
+    token and KV head: the newest page, and those whose k_bounds (kv_bounds_paged) allow the largest products
+    with one of the KV head's queries; all pages where there are no more.  selected (int32 [batch,
+    n_kv_heads, n_select]) receives their places in the sequence, ascending, then -1.  Returns o."""
+    dev = q.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return sdpa_decode_paged_sparse(q, k_pages, v_pages, page_table, kv_lens, k_bounds, n_select, k_scale, v_scale,
+                                            scale, out, selected)
+    call, entry, ws_bytes = _front("sdpa_decode_paged_sparse", "sdpa_decode_paged_sparse_workspace_bytes")
+    return call(_lib.check, _stream() if dev >= 0 else 0, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
+                kv_lens, k_bounds, n_select, k_scale, v_scale, scale, out, selected)
+
+
+def kv_bounds_paged(k_pages: torch.Tensor, page_table: torch.Tensor, start_pos: torch.Tensor, k_bounds: torch.Tensor,
+                    cu_seqlens: torch.Tensor | None = None, tokens: int | None = None,
+                    k_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """The smallest and largest keys, dim by dim, of every page that a step's new tokens complete
+    (nmi_kv_bounds_paged), after the call of kv_append_paged that stored them: start_pos and cu_seqlens as
+    there, tokens the rows that cu_seqlens divides (None, both: one token per sequence).  Written to
+    k_bounds [n_pages, n_kv_heads, 2, 128] bf16 (minimum, maximum), which is returned; other pages' stay."""
+    dev = k_pages.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_bounds_paged(k_pages, page_table, start_pos, k_bounds, cu_seqlens, tokens, k_scale)
+    call, entry = _front("kv_bounds_paged")
+    return call(_lib.check, _stream() if dev >= 0 else 0, entry, k_pages, page_table, start_pos, k_bounds, cu_seqlens, tokens,
+                k_scale)
+
+
+class PagedStep(NamedTuple):
+    """What kv_assign_paged returns (nmi_kv_assign_paged)."""
+    start_pos: torch.Tensor          # int32 [batch]: first new position, -1 where there is none
+    kv_lens: torch.Tensor            # int32 [batch]: positions to attend, 0 where there is no new token
+    cu_seqlens: torch.Tensor | None  # int32 [batch + 1]: packed offsets; None for one row per sequence
+    slots: torch.Tensor              # int64 [tokens]: page * page_size + place, -1 where not stored
+    lens: torch.Tensor               # int32 [batch]: positions stored after the step, -1 where not in use
+    free_count: torch.Tensor         # int32 [1]
+
+
+def kv_assign_paged(lens: torch.Tensor, new_lens: torch.Tensor | None, page_table: torch.Tensor, free_pages: torch.Tensor,
+                    free_count: torch.Tensor, page_size: int, tokens: int | None = None,
+                    lens_out: torch.Tensor | None = None, free_count_out: torch.Tensor | None = None) -> PagedStep:
+    """Pages for a step's new tokens, handed out on the GPU (nmi_kv_assign_paged): lens int32 [batch] positions
+    stored (negative: not in use), new_lens int32 [batch] new tokens (0 none, negative: the sequence has
+    ended and gives its pages back; None: one each), page_table int32 [batch, max_pages] written where pages are
+    added, free_pages int32 [n_pages] a stack of which the first free_count[0] (int32) are free.  tokens: the rows
+    of packed new tokens; None where every sequence has one row.  A sequence whose tokens do not all fit its row of
+    the table or the pages left is granted none (start_pos -1).  lens_out and free_count_out may be lens and
+    free_count themselves, so that a captured step goes on from where it ended."""
+    dev = lens.get_device()
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return kv_assign_paged(lens, new_lens, page_table, free_pages, free_count, page_size, tokens, lens_out,
+                                   free_count_out)
+    call, entry = _front("kv_assign_paged")
+    return PagedStep(*call(_lib.check, _stream() if dev >= 0 else 0, entry, lens, new_lens, page_table, free_pages, free_count,
+                           page_size, tokens, lens_out, free_count_out))
 
 
 def sdpa_prefill_packed_bf16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, n_heads: int,
