@@ -439,7 +439,8 @@ typedef struct nmi_paged_kv {
  *              A block's scale becomes the smallest power of two s, 2^-126 at least, with |x| <= 448 s for the
  *              call's finite values x of the block, and no less than it was where places of the block before the
  *              call's are in it (they hold earlier positions; a block whose first place is the call's begins
- *              anew; a scale that was no power of two counts as the next one).  Codes are x / s to the nearest
+ *              anew; a scale that was no power of two counts as the next one, one that was not positive and finite
+ *              as none, and the codes under it are lost).  Codes are x / s to the nearest
  *              even, NaN and infinities as NaN; where s grew the block's earlier codes become code * s_old / s to
  *              the nearest even.  Bytes of places after the call's last one stay.
  *   q_out, k_out  the rotated q and k as bf16 (q and q_out both or neither; k_out for the attention over

@@ -434,6 +434,7 @@ PyObject* kv_assign_paged(PyObject* const* a) {
         bad_value("page_table must be int32 [batch=" + num(batch) + ", max_pages] with contiguous rows, got " + show(table));
     on_device(table, "page_table", dev);
     if (pages.dim() != 1) bad_value("free_pages must be an int32 vector [n_pages], got " + list(pages.sizes()));
+    if (!table.size(1) || !pages.size(0)) bad_value("a page table or a pool of no pages");
     int32_t* free_p = vector<int32_t>(a[6], pages.size(0), at::kInt, "free_pages", dev);
     tensor(a[7], "free_count");
     const int32_t* count_p = vector<int32_t>(a[7], 1, at::kInt, "free_count", dev);

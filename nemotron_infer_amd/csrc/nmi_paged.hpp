@@ -54,11 +54,11 @@ NMI_HD int block_exponent(uint32_t amax_bits) {
     const int e = (int)(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return e < 1 ? 1 : e;
 }
-// That of the smallest power of two that is no less than a scale found in memory: itself, if an append wrote it.
-// Kept to what 2^-e can be had of, whatever the bits.
+// That of the smallest power of two that is no less than a scale found in memory: itself, if an append wrote it.  1 for
+// what is no scale (negative, NaN, infinite); at most what 2^-e can be had of.
 NMI_HD int block_exponent_of_scale(uint32_t bits) {
-    const uint32_t b = bits & 0x7FFFFFFFu;
-    const int e = (int)(b >> 23) + ((b & 0x7FFFFFu) ? 1 : 0);
+    if (bits >= 0x7F800000u) return 1;
+    const int e = (int)(bits >> 23) + ((bits & 0x7FFFFFu) ? 1 : 0);
     return e < 1 ? 1 : (e > 253 ? 253 : e);
 }
 

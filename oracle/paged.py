@@ -96,3 +96,107 @@ def round_e4m3(x: np.ndarray) -> np.ndarray:
     x = np.clip(np.asarray(x, np.float64), -E4M3_MAX, E4M3_MAX)
     unit = np.exp2(np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -6))) - 3)
     return np.rint(x / unit) * unit
+
+
+# --- a cache under scales of blocks, pages handed out, pages selected -------------------------------
+
+BLOCK = 16
+
+
+def block_scale(amax: float) -> float:
+    """The smallest power of two s, 2^-126 at least, with amax <= 448 s."""
+    s = 2.0 ** -126
+    while amax > E4M3_MAX * s:
+        s *= 2
+    return s
+
+
+def append_blocks(values: np.ndarray, scales: np.ndarray, x: np.ndarray, rows, table, page: int) -> None:
+    """x [T, n_kv, 128] float64 stored in values [n_pages, n_kv, page, 128] (what the codes stand for without
+    their scale) under scales [n_pages, n_kv, page / 16], both in place; rows: [(row, sequence, position)]."""
+    blocks = {}
+    for t, b, pos in rows:
+        blocks.setdefault((b, pos // BLOCK), []).append((pos, t))
+    for (b, _), new in blocks.items():
+        new.sort()
+        pos0 = new[0][0]
+        p, r0 = int(table[b][pos0 // page]), pos0 % page // BLOCK * BLOCK
+        before = pos0 % BLOCK
+        for h in range(values.shape[1]):
+            got = np.stack([x[t, h] for _, t in new])
+            finite = np.abs(got[np.isfinite(got)])
+            s = block_scale(finite.max() if finite.size else 0.0)
+            if before:
+                was = float(scales[p, h, r0 // BLOCK])
+                s = max(s, 2.0 ** max(-126, int(np.ceil(np.log2(was)))) if 0 < was < np.inf else 0.0)
+                values[p, h, r0:r0 + before] = round_e4m3(values[p, h, r0:r0 + before] * (was / s))
+            scales[p, h, r0 // BLOCK] = s
+            for (pos, _), v in zip(new, got):
+                values[p, h, pos % page] = np.where(np.isfinite(v), round_e4m3(np.where(np.isfinite(v), v, 0.0) / s), np.nan)
+
+
+def assign(lens, new_lens, table, free_pages, free_count: int, page: int, packed: bool):
+    """One step of the pages' life, one sequence after another; table and free_pages (lists) in place."""
+    stack = list(free_pages[:free_count])
+    new = [1] * len(lens) if new_lens is None else [int(n) for n in new_lens]
+    for b, n in enumerate(new):
+        if n < 0 <= lens[b]:
+            stack += [int(i) for i in table[b][:-(-int(lens[b]) // page)]]
+    free_pages[:len(stack)] = stack
+    room = len(stack)
+    start, kv, after, slots, cu = [], [], [], [], [0]
+    for b, n in enumerate(new):
+        have, total = -(-max(0, int(lens[b])) // page), int(lens[b]) + max(0, n)
+        ok = lens[b] >= 0 and n > 0 and total <= len(table[b]) * page
+        need = -(-total // page) - have if ok else 0
+        room -= need
+        ok = ok and (need == 0 or room >= 0)
+        if ok:
+            for j in range(need):
+                table[b][have + j] = stack.pop()
+        start.append(int(lens[b]) if ok else -1)
+        kv.append(total if ok else 0)
+        after.append(-1 if lens[b] >= 0 and n < 0 else total if ok else int(lens[b]))
+        n_rows = max(0, n) if packed else 1
+        slots += [int(table[b][(int(lens[b]) + i) // page]) * page + (int(lens[b]) + i) % page if ok else -1 for i in range(n_rows)]
+        cu.append(cu[-1] + n_rows)
+    return {"start_pos": start, "kv_lens": kv, "cu_seqlens": cu if packed else None, "slots": slots, "lens": after,
+            "free_count": [len(stack)]}
+
+
+def page_bounds(values: np.ndarray) -> np.ndarray:
+    """Minimum and maximum over the positions of pages [n, n_kv, page, 128]; NaN where one is.  [n, n_kv, 2, 128]."""
+    return np.stack((values.min(axis=2), values.max(axis=2)), axis=2)
+
+
+def select(q: np.ndarray, bounds: np.ndarray, table_row, n: int, page: int, n_select: int):
+    """The places of the pages that a token attends: q [H, 128], bounds [n_pages, n_kv, 2, 128]; a list per KV head."""
+    P, n_kv = -(-n // page), bounds.shape[1]
+    if P <= n_select:
+        return [list(range(P))] * n_kv
+    group, kept = q.shape[0] // n_kv, []
+    for g in range(n_kv):
+        lo, hi = (bounds[np.asarray(table_row[:P - 1]), g, i] for i in range(2))
+        score = np.full(P - 1, -np.inf, np.float32)
+        for x in q[g * group:(g + 1) * group]:
+            score = np.maximum(score, (hi @ np.maximum(x, 0) + lo @ np.minimum(x, 0)).astype(np.float32))
+        order = sorted(range(P - 1), key=lambda p: (0, 0.0, p) if np.isnan(score[p]) else (1, -score[p], p))
+        kept.append(sorted(order[:n_select - 1]) + [P - 1])
+    return kept
+
+
+def decode_selected(q, k_pages, v_pages, table, lens, kept, scale=HEAD ** -0.5) -> np.ndarray:
+    """decode over the pages kept[b][g] of each sequence and KV head."""
+    B, H, _ = q.shape
+    n_kv, page = k_pages.shape[1:3]
+    out = np.zeros((B, H, HEAD))
+    for b in range(B):
+        n = int(lens[b])
+        if n <= 0:
+            continue
+        for g in range(n_kv):
+            end = len(kept[b][g]) * page - (-(-n // page) * page - n)
+            heads = slice(g * (H // n_kv), (g + 1) * (H // n_kv))
+            ids = [[int(table[b][p]) for p in kept[b][g]]]
+            out[b, heads] = decode(q[b:b + 1, heads], k_pages[:, g:g + 1], v_pages[:, g:g + 1], ids, [end], scale)[0]
+    return out
