@@ -11,12 +11,18 @@
 //
 // Which pages are chosen must not hang on the order of a sum: scores are summed in 64 bits (the products are exact
 // there) and rounded to float32 once.  With mid = (lo + hi) / 2 and half = (hi - lo) / 2, exact in 64 bits for what
-// bf16 holds, a term is q mid + |q| half: two multiply-adds, the magnitude for nothing.
+// bf16 holds unless they lie 2^45 apart, a term is q mid + |q| half: two multiply-adds, the magnitude for nothing.
+// (Float32 sums instead took 1 us of 20 less for one sequence of 100001 positions, 2 of 43 for 20 documents.)
 //
 // Scores.  Bound: reading the bounds, 512 bytes a page and head.  16 lanes take a page, 8 dims each, the queries in
-// their registers; a wave takes 4 pages at a time.
-// Choice: one workgroup for a sequence's KV head: the n-th largest by four counts of 8 bits each, in LDS, then one
-// pass in order.  Bound: latency.
+// their registers; a wave takes 4 pages at a time, the next ones' bounds on their way.  A sequence's KV head is dealt to
+// as many workgroups as all of them leave it of 8 per CU: 1 / 2 / 4 / 8 / 16 per CU, 20 documents of 900 to 30000 positions
+// (pages of 32, 32 / 8 heads; the whole call) 113 / 62 / 50 / 44.0 / 44.4 us; the pages of all sequences in equal shares
+// 43.4 where this takes 43.1, and one sequence 21.0 where this takes 20.6.
+// Choice: one workgroup for a sequence's KV head: the range of the scores cut into 1024 bins, counted in LDS, the bin
+// with the last one wanted cut again while it has many, its few ranked one against another; then one pass in order.
+// Bound: latency, a handful of barriers: 4.6 us (traced) of 1562 pages, where four passes of 8 bits and a scan for each
+// 256 pages took 12.4.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 #include "nmi_packed.hpp"
@@ -29,7 +35,9 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kHeads = 5;               // query heads at a time: 16 registers each
-constexpr int kKeys = 8192;             // scores of a sequence kept in LDS
+constexpr int kBinBits = 10, kSelectThreads = 1 << kBinBits, kSelectWaves = kSelectThreads / 64;
+constexpr int kKeys = 6144;             // keys and page ids of a sequence kept in LDS
+constexpr int kFew = 64;                // keys ranked by a wave
 
 struct Sequence {
     int len, pages;
@@ -62,14 +70,35 @@ __device__ __forceinline__ double row_sum16_f64(double v) {
 // A workgroup takes every parts-th 16 pages of a sequence's KV head.
 __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a, int parts) {
     const int part = blockIdx.x % parts, g = (int)(blockIdx.x / parts % a.kv.n_kv), b = (int)(blockIdx.x / parts / a.kv.n_kv);
-    const Sequence s = sequence(a, b);
-    if (s.pages <= a.select) return;
     const int lane = threadIdx.x & 63, sub = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int32_t* row = a.kv.page_table + b * a.kv.table_stride;
+    const int first = (part * kWaves + wave) * 4 + (lane >> 4), stride = parts * kWaves * 4;
+    // (entries of the table's row, whatever they hold, asked for beside the length)
+    auto page_id = [&](int64_t p) { return row[min(p, (int64_t)a.kv.max_pages - 1)]; };
+    int32_t first_id[2] = {page_id(first), page_id((int64_t)first + stride)};
+    const Sequence s = sequence(a, b);
+    const int n = s.pages - 1;
+    if (s.pages <= a.select || (part * kWaves + wave) * 4 >= n) return;
+    struct Bounds {
+        uint4 lo, hi;
+        bool bad;
+    };
+    auto load = [&](int32_t id) {
+        Bounds x;
+        x.bad = false;
+        const int page = checked_page(id, a.kv.n_pages, &x.bad);
+        const uint16_t* p = a.bounds + (((int64_t)page * a.kv.n_kv + g) * 2) * kPagedHead + 8 * sub;
+        x.lo = load16(p);
+        x.hi = load16(p + kPagedHead);
+        return x;
+    };
     float* scores = a.scores + ((int64_t)b * a.kv.n_kv + g) * a.kv.max_pages;
     const int chunks = (a.group + kHeads - 1) / kHeads, per = (a.group + chunks - 1) / chunks;
     for (int h0 = 0; h0 < a.group; h0 += per) {
+        // a page's bounds are on their way while those before are used, and the id of the next one's
+        Bounds next = load(first_id[0]);
+        int32_t id = first_id[1];
         const int heads = min(per, a.group - h0);
         double q[kHeads][8];
 #pragma unroll
@@ -79,14 +108,13 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[h][i] = x[i];
         }
-        for (int p0 = (part * kWaves + wave) * 4; p0 < s.pages - 1; p0 += parts * kWaves * 4) {
-            const int p = p0 + (lane >> 4);
-            bool none = p >= s.pages - 1, bad = false;
-            const int page = none ? 0 : checked_page(row[p], a.kv.n_pages, &bad);
-            const uint16_t* bounds = a.bounds + (((int64_t)page * a.kv.n_kv + g) * 2) * kPagedHead + 8 * sub;
+        for (int64_t p = first; __builtin_amdgcn_ballot_w64(p < n); p += stride) {      // (all lanes, for the sums over them)
+            const Bounds now = next;
+            next = load(id);
+            id = page_id(p + 2 * stride);
             float lo[8], hi[8];
-            unpack8(load16(bounds), lo);
-            unpack8(load16(bounds + kPagedHead), hi);
+            unpack8(now.lo, lo);
+            unpack8(now.hi, hi);
             double mid[8], half[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -105,9 +133,9 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a
                 }
                 best = __builtin_elementwise_maximum(best, (float)row_sum16_f64(sum));      // (NaN stays)
             }
-            if (sub == 0 && !none) {
+            if (sub == 0 && p < n) {
                 if (h0) best = __builtin_elementwise_maximum(best, scores[p]);
-                scores[p] = bad ? NAN : best;           // (a bad page is the attention's to report)
+                scores[p] = now.bad ? NAN : best;       // (a bad page is the attention's to report)
             }
         }
     }
@@ -120,90 +148,122 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Inclusive sums over the workgroup, the sum of all to *total.
-__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t (&sums)[kWaves], uint32_t* total) {
+// Inclusive sums over the workgroup, the sum of all to *total.  Every thread takes part; `sums` is free afterwards only
+// behind a barrier.
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t (&sums)[kSelectWaves], uint32_t* total) {
     v = wave_scan_u32(v);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (lane == 63) sums[wave] = v;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        before += w < wave ? sums[w] : 0u;
-        all += sums[w];
-    }
-    *total = all;
-    return before + v;
+    const uint32_t s = wave_scan_u32(lane < kSelectWaves ? sums[lane] : 0u);
+    *total = lane_u32(s, 63);
+    return v + (wave ? lane_u32(s, wave - 1) : 0u);
 }
 
-__global__ __launch_bounds__(kThreads) void page_select_kernel(const SelectArgs a) {
+__global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const SelectArgs a) {
     __shared__ uint32_t keys[kKeys];
-    __shared__ uint32_t bins[256];
-    __shared__ uint32_t sums[kWaves];
-    __shared__ uint32_t found[2];       // a digit, and how many of the larger keys are wanted beside it
-    const int tid = threadIdx.x, g = (int)(blockIdx.x % a.kv.n_kv), b = (int)(blockIdx.x / a.kv.n_kv);
+    __shared__ int32_t ids[kKeys];
+    __shared__ uint32_t bins[kSelectThreads];
+    __shared__ uint32_t sums[3][kSelectWaves];
+    __shared__ uint32_t found[3];                       // a bin, the keys in it, and those in larger ones
+    __shared__ uint32_t few[kFew];
+    const int tid = threadIdx.x, lane = tid & 63, g = (int)(blockIdx.x % a.kv.n_kv), b = (int)(blockIdx.x / a.kv.n_kv);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Sequence s = sequence(a, b);
     const int32_t* row = a.kv.page_table + b * a.kv.table_stride;
     const int64_t mine = ((int64_t)b * a.kv.n_kv + g) * a.select;
-    auto put = [&](int64_t i, int place) {      // (a length that the table does not hold: no page, which the attention reports)
-        if (a.rows) a.rows[mine + i] = s.bad ? -1 : row[place];
+    auto put = [&](int64_t i, int place, int32_t id) {  // (a length that the table does not hold: no page, which the attention reports)
+        if (a.rows) a.rows[mine + i] = s.bad ? -1 : id;
         if (a.selected) a.selected[mine + i] = place;
     };
     const int kept = min(s.pages, a.select);
     if (a.selected)
-        for (int i = kept + tid; i < a.select; i += kThreads) a.selected[mine + i] = -1;
+        for (int i = kept + tid; i < a.select; i += kSelectThreads) a.selected[mine + i] = -1;
     if (g == 0 && tid == 0 && a.out_lens)
         a.out_lens[b] = s.pages <= a.select ? s.len : s.len - ((s.pages - a.select) << a.kv.page_shift);
     if (s.pages <= a.select) {
-        for (int i = tid; i < s.pages; i += kThreads) put(i, i);
+        for (int i = tid; i < s.pages; i += kSelectThreads) put(i, i, row[i]);
         return;
     }
-    const int n = s.pages - 1;                  // those to choose from
-    if (tid == 0) put(a.select - 1, n);
+    const int n = s.pages - 1;                          // those to choose from
+    if (tid == 0) put(a.select - 1, n, row[n]);
     uint32_t want = (uint32_t)a.select - 1;
     if (!want) return;
     const float* scores = a.scores + ((int64_t)b * a.kv.n_kv + g) * a.kv.max_pages;
     const bool here = n <= kKeys;
-    if (here)
-        for (int i = tid; i < n; i += kThreads) keys[i] = key_of(scores[i]);
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;                  // the range of the keys
+    for (int i = tid; i < n; i += kSelectThreads) {
+        const int32_t id = here ? row[i] : 0;
+        const uint32_t k = key_of(scores[i]);
+        if (here) keys[i] = k, ids[i] = id;
+        lo = min(lo, k);
+        hi = max(hi, k);
+    }
     auto key = [&](int i) { return here ? keys[i] : key_of(scores[i]); };
-    // the want-th largest key, 8 bits at a time: `top` its bits so far
-    uint32_t top = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        bins[tid] = 0;
-        __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-        for (int i = tid; i < n; i += kThreads) {
+    lo = ~wave_max_u32(~lo);
+    hi = wave_max_u32(hi);
+    if (lane == 0) sums[0][wave] = ~lo, sums[1][wave] = hi;
+    bins[tid] = 0;
+    __syncthreads();
+    lo = ~wave_max_u32(lane < kSelectWaves ? sums[0][lane] : 0u);
+    hi = wave_max_u32(lane < kSelectWaves ? sums[1][lane] : 0u);
+
+    // The want-th largest key is in [lo, hi], counted from the largest of that range.  The range is cut into as many equal bins as
+    // there are threads, and the bin that has it becomes the range, until few keys are in it or all are equal.
+    for (;;) {
+        const uint32_t span = hi - lo;
+        const int shift = max(0, 32 - (span ? __builtin_clz(span) : 32) - kBinBits);
+        for (int i = tid; i < n; i += kSelectThreads) {
             const uint32_t k = key(i);
-            if ((k & mask) == top) atomicAdd(&bins[k >> shift & 255], 1u);
+            if (k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> shift], 1u);
         }
         __syncthreads();
-        const uint32_t c = bins[255 - tid];     // thread t: digit 255 - t, and the sum of those from there up
+        const uint32_t bin = kSelectThreads - 1 - tid, c = bins[bin];   // thread t: the t-th bin from above
         uint32_t all;
-        const uint32_t upto = group_scan(c, sums, &all);
-        if (upto >= want && upto - c < want) {
-            found[0] = 255 - tid;
-            found[1] = want - (upto - c);
+        const uint32_t upto = group_scan(c, sums[2], &all);
+        if (upto >= want && upto - c < want) found[0] = bin, found[1] = c, found[2] = upto - c;
+        bins[bin] = 0;
+        __syncthreads();
+        const uint32_t in_bin = found[1];
+        want -= found[2];
+        lo += found[0] << shift;
+        hi = lo + min(hi - lo, (1u << shift) - 1);
+        if (in_bin <= kFew || shift == 0) break;
+        __syncthreads();                                // (found is read by all)
+    }
+    // Few: each ranked among them.  `lo` becomes the key itself, `want` the keys equal to it that are taken.
+    if (hi != lo) {
+        for (int i = tid; i < n; i += kSelectThreads) {
+            const uint32_t k = key(i);
+            if (k >= lo && k <= hi) few[atomicAdd(&bins[0], 1u)] = k;
         }
         __syncthreads();
-        top |= found[0] << shift;
-        want = found[1];
-        __syncthreads();
+        const int m = (int)bins[0];
+        const uint32_t k = lane < m ? few[lane] : 0u;
+        uint32_t above = 0, equal = 0;
+        for (int i = 0; i < m; ++i) {
+            const uint32_t other = lane_u32(k, i);
+            above += other > k;
+            equal += other == k;
+        }
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < m && above < want && above + equal >= want);
+        const int who = __builtin_ctzll(hit);
+        lo = lane_u32(k, who);
+        want -= lane_u32(above, who);
     }
     // all that are larger, and the first `want` that are equal
-    uint32_t out = 0, equal = 0;
-    for (int i0 = 0; i0 < n; i0 += kThreads) {
+    uint32_t larger = 0, equal = 0;                     // of those before the ones at hand
+    for (int i0 = 0, turn = 0; i0 < n; i0 += kSelectThreads, turn ^= 1) {
         const int i = i0 + tid;
         const uint32_t k = i < n ? key(i) : 0u;
-        const uint32_t is_equal = i < n && k == top;
-        uint32_t all_equal, all;
-        const uint32_t rank = equal + group_scan(is_equal, sums, &all_equal);
-        const uint32_t take = i < n && (k > top || (is_equal && rank <= want));
-        const uint32_t place = out + group_scan(take, sums, &all);
-        if (take) put(place - 1, i);
-        equal += all_equal;
-        out += all;
+        const uint32_t is_larger = i < n && k > lo, is_equal = i < n && k == lo;
+        uint32_t all;
+        const uint32_t upto = group_scan(is_larger << 16 | is_equal, sums[turn], &all);
+        const uint32_t larger_upto = larger + (upto >> 16), equal_upto = equal + (upto & 0xFFFFu);
+        if (is_larger || (is_equal && equal_upto <= want))
+            put((int64_t)larger_upto + min(equal_upto, want) - 1, i, here ? ids[i] : row[i]);
+        larger += all >> 16;
+        equal += all & 0xFFFFu;
     }
 }
 
@@ -212,13 +272,13 @@ __global__ __launch_bounds__(kThreads) void page_select_kernel(const SelectArgs 
 hipError_t launch_page_select(const SelectArgs& a, hipStream_t stream) {
     const int64_t groups = (int64_t)a.batch * a.kv.n_kv;
     if (a.select < a.kv.max_pages) {
-        // as many workgroups as are resident, or one for each 16 pages that a sequence may have
+        // as many workgroups as keep the CUs busy, or one for each 16 pages that a sequence may have
         const int64_t most = ((int64_t)a.kv.max_pages + 15) / 16, parts = std::max<int64_t>(1, 8 * device_info().num_cu / groups);
         const int p = (int)std::min(most, parts);
         hipLaunchKernelGGL(page_score_kernel, dim3((uint32_t)(groups * p)), dim3(kThreads), 0, stream, a, p);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(page_select_kernel, dim3((uint32_t)groups), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(page_select_kernel, dim3((uint32_t)groups), dim3(kSelectThreads), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -588,6 +588,27 @@ def test_sparse_counts_close_scores_exactly():
     _check_sparse(rng, "bf16", [3000], 3, 1, 16, 50, bounds=close, qscale=1.0)
 
 
+@pytest.mark.parametrize("select", [2, 9, 600, 1249])
+def test_sparse_counts_crowded_scores(select):
+    """Many equal scores, more than are ranked one by one; scores crowded beside one far above, or NaN, or far below."""
+    announce("sparse_crowded", select)
+    rng = np.random.default_rng(select)
+
+    def few(pool):
+        return np.sort(_rand_bits(rng, 3, 1, 2, 128), axis=2)[rng.integers(0, 3, pool.k.shape[0])]
+
+    def beside(value, page):
+        def make(pool):
+            x = rng.standard_normal((pool.k.shape[0], 1, 1, 128)) * 2.0 ** -6 + np.array([-1.0, 1.0]).reshape(2, 1)
+            x = block.bf16_round_exact(x)
+            x[pool.table[0, page], 0, :, 3] = value
+            return x
+        return make
+
+    for bounds in (few, beside(NAN_BF16, 77), beside(0x7F00, 1000), beside(0xFF00, 3)):
+        _check_sparse(rng, "bf16", [20000], 4, 1, 16, select, bounds=bounds, qscale=1.0)
+
+
 def test_sparse_bad_pages_and_lengths_are_reported():
     """A page id out of range, scored or attended, a length past the table: NaN there and NMI_ERR_ASYNC once; the others
     right."""
