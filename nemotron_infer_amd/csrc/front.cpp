@@ -448,17 +448,24 @@ PyObject* kv_assign_paged(PyObject* const* a) {
     if (packed && !new_p) bad_value("packed rows (tokens) need new_lens");
     if (lens_out && new_p && lens_out == new_p) bad_value("lens_out must not be new_lens");
     on_gpu(lens);
-    // one allocation for what is new: start_pos, kv_lens, cu_seqlens, lens_out, free_count_out
-    const auto ints = lens.options();
-    at::Tensor all = at::empty({3 * batch + (packed ? batch + 1 : 0) + 1}, ints);
-    int64_t at = 0;
+    // One allocation for what is new, and tensors over parts of it made directly (a second allocation, and each of torch's
+    // views, cost an eager call 1 us): slots, then start_pos, kv_lens, cu_seqlens, lens_out, free_count_out.
+    const int64_t slot_rows = std::max<int64_t>(tokens, 1);     // (the C entry takes a row at least)
+    const int64_t n_ints = 3 * batch + (packed ? batch + 1 : 0) + 1;
+    const at::Tensor all = at::empty({slot_rows + (n_ints + 1) / 2}, lens.options().dtype(at::kLong));
+    auto over = [&](at::ScalarType type, int64_t first, int64_t n) {
+        auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+        t->set_storage_offset(first);
+        t->set_sizes_contiguous({n});
+        return at::Tensor(std::move(t));
+    };
+    int64_t at = 2 * slot_rows;
     auto part = [&](int64_t n) {
         at += n;
-        return all.narrow(0, at - n, n);
+        return over(at::kInt, at - n, n);
     };
+    const at::Tensor slots = over(at::kLong, 0, tokens);
     const at::Tensor start = part(batch), kv = part(batch), cu = packed ? part(batch + 1) : at::Tensor();
-    const int64_t slot_rows = std::max<int64_t>(tokens, 1);     // (the C entry takes a row at least)
-    at::Tensor slots = at::empty({slot_rows}, ints.dtype(at::kLong));
     Owned lens_o(lens_out ? new_ref(a[10]) : THPVariable_Wrap(part(batch)));
     Owned count_o(count_out ? new_ref(a[11]) : THPVariable_Wrap(part(1)));
     if (!lens_out) lens_out = static_cast<int32_t*>(THPVariable_Unpack(lens_o.p).data_ptr());
@@ -472,7 +479,7 @@ PyObject* kv_assign_paged(PyObject* const* a) {
         const int64_t stride = batch > 1 ? table.stride(0) : table.size(1);
         int32_t *start_p = static_cast<int32_t*>(start.data_ptr()), *kv_p = static_cast<int32_t*>(kv.data_ptr());
         int32_t* cu_p = packed ? static_cast<int32_t*>(cu.data_ptr()) : nullptr;
-        int64_t* slots_p = static_cast<int64_t*>(slots.data_ptr());
+        int64_t* slots_p = static_cast<int64_t*>(all.data_ptr());
         int rc;
         Py_BEGIN_ALLOW_THREADS;
         rc = call(lens_p, new_p, table_p, stride, width, page_size, free_p, count_p, n_pages, b, n, start_p, kv_p, cu_p, slots_p,
@@ -480,7 +487,6 @@ PyObject* kv_assign_paged(PyObject* const* a) {
         Py_END_ALLOW_THREADS;
         check(a[0], rc, "nmi_kv_assign_paged");
     }
-    if (slot_rows != tokens) slots = slots.narrow(0, 0, tokens);
     Owned start_o(THPVariable_Wrap(start)), kv_o(THPVariable_Wrap(kv)), slots_o(THPVariable_Wrap(slots));
     Owned cu_o(packed ? THPVariable_Wrap(cu) : new_ref(Py_None));
     return PyTuple_Pack(6, start_o.p, kv_o.p, cu_o.p, slots_o.p, lens_o.p, count_o.p);
