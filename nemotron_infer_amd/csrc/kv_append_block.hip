@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_block_token_kernel(cons
         }
         if (!stored) continue;
         uint8_t* p = (is_v ? a.kv.v_pages : a.kv.k_pages) + at.off + h * a.kv.head_stride;
-        float* sp = (is_v ? a.kv.v_blocks : a.kv.k_blocks) + at.block + ((int64_t)h << (a.kv.page_shift - 4));
+        float* sp = (is_v ? a.blocks.v : a.blocks.k) + at.block + ((int64_t)h << (a.kv.page_shift - 4));
         const uint32_t old = before ? __float_as_uint(*sp) : 0u;
         uint32_t m = finite_max(y, finite_max(x, 0u));          // over the vector's 8 lanes
         m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xF, 0xF, false));
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_block_kernel(const Appe
             }
         }
         uint8_t* p = (is_v ? a.kv.v_pages : a.kv.k_pages) + at.off + h * a.kv.head_stride;
-        float* sp = (is_v ? a.kv.v_blocks : a.kv.k_blocks) + at.block + ((int64_t)h << (a.kv.page_shift - 4));
+        float* sp = (is_v ? a.blocks.v : a.blocks.k) + at.block + ((int64_t)h << (a.kv.page_shift - 4));
         const uint32_t old = stored && before ? __float_as_uint(*sp) : 0u;
         float x[2][8], y[2][8];
         uint32_t m = 0;

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * kWaves) void kv_bounds_kernel(const BoundsArgs
     const uint8_t* base = a.kv.k_pages + page * a.kv.page_stride + h * a.kv.head_stride + 4 * (CODES ? lane & 31 : lane);
     const int r0 = CODES ? lane >> 5 : 0;
     const float head_scale = FORM == KvForm::E4m3 && a.kv.k_scale ? load_const(a.kv.k_scale + h) : 1.f;
-    const float* block_scale = FORM == KvForm::Block ? a.kv.k_blocks + block_index(page, a.kv.n_kv, h, shift, 0) : nullptr;
+    const float* block_scale = FORM == KvForm::Block ? a.blocks.k + block_index(page, a.kv.n_kv, h, shift, 0) : nullptr;
     float lo[kDims], hi[kDims];
 #pragma unroll
     for (int i = 0; i < kDims; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;

@@ -278,6 +278,7 @@ struct AppendArgs {
     const float* inv_freq;      // [rotary / 2] or nullptr
     int batch, tokens, H, rotary;
     bool interleaved;
+    BlockScales blocks;         // of a cache under scales of blocks
 };
 hipError_t launch_kv_append(const AppendArgs& a, bool e4m3, hipStream_t stream);
 // The same into e4m3 under scales of blocks, which it sets (kv_append_block.hip).
@@ -290,6 +291,7 @@ struct BoundsArgs {
     const int32_t* cu;          // [batch + 1] or nullptr: one position per sequence
     const int32_t* start;       // [batch]
     int batch, tokens;
+    BlockScales blocks;
 };
 hipError_t launch_kv_bounds(const BoundsArgs& a, KvForm form, hipStream_t stream);
 
@@ -337,6 +339,8 @@ struct PagedDecodeArgs {
     int batch, H, group;        // group: query heads per KV head
     int waves;                  // waves per KV head (and 16 of its query heads)
     float scale2;               // log2(e) * softmax scale
+    int table_head_stride;      // entries from a KV head's row of a sequence's pages to the next (0: one row for all)
+    BlockScales blocks;
 };
 int sdpa_decode_paged_waves(int n_kv, int group);
 size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv);

@@ -35,9 +35,12 @@ struct PagedKv {
     const float* v_scale;
     int n_pages, max_pages, page_shift, n_kv;
     uint32_t* error;                    // host word to set where the device data is out of range, or nullptr
-    float* k_blocks;                    // [n_pages, n_kv, page_size / kPagedBlock] scales of blocks, or nullptr
-    float* v_blocks;
-    int64_t table_head_stride;          // entries from a KV head's row of a sequence's pages to the next (0: one row for all)
+};
+
+// Scales of blocks, [n_pages, n_kv, page_size / kPagedBlock] each.
+struct BlockScales {
+    float* k;
+    float* v;
 };
 
 // What a cache holds: bf16, e4m3 codes under a scale per KV head, or under one per head and block.

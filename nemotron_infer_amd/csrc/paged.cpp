@@ -49,7 +49,7 @@ bool rows_ok(const void* p, int64_t ld, int heads) {
 constexpr int64_t kMaxGroups256 = (1 << 24) - 1;
 
 // A cache descriptor as the kernels take it; 0 or an NMI_ERR_* with the message set.
-int check_cache(const char* fn, const nmi_paged_kv* c, PagedKv* out) {
+int check_cache(const char* fn, const nmi_paged_kv* c, PagedKv* out, BlockScales* blocks) {
     if (!c) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL cache", fn);
     if (!c->k_pages || !c->v_pages || !c->page_table)
         return refuse(NMI_ERR_INVALID_ARG, "%s: NULL pages or page table", fn);
@@ -85,8 +85,8 @@ int check_cache(const char* fn, const nmi_paged_kv* c, PagedKv* out) {
     *out = PagedKv{static_cast<uint8_t*>(c->k_pages), static_cast<uint8_t*>(c->v_pages), c->page_stride * size,
                    c->head_stride * size, c->token_stride * size, c->page_table, c->page_table_stride,
                    block ? nullptr : c->k_scale, block ? nullptr : c->v_scale, c->n_pages, c->max_pages,
-                   __builtin_ctz((unsigned)c->page_size), c->n_kv_heads, nullptr,
-                   block ? const_cast<float*>(c->k_scale) : nullptr, block ? const_cast<float*>(c->v_scale) : nullptr, 0};
+                   __builtin_ctz((unsigned)c->page_size), c->n_kv_heads, nullptr};
+    if (block) *blocks = BlockScales{const_cast<float*>(c->k_scale), const_cast<float*>(c->v_scale)};
     return NMI_OK;
 }
 
@@ -99,7 +99,7 @@ int check_decode(const char* fn, const nmi_paged_kv* cache, const void* q_bf16, 
                  const int32_t* kv_lens, int batch, int n_heads, float scale, PagedDecodeArgs* out) {
     if (take_async_error(fn, AsyncKind::Paged)) return NMI_ERR_ASYNC;
     PagedDecodeArgs& a = *out;
-    if (const int rc = check_cache(fn, cache, &a.kv)) return rc;
+    if (const int rc = check_cache(fn, cache, &a.kv, &a.blocks)) return rc;
     if (!q_bf16 || !o_bf16 || !kv_lens) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL q, o or kv_lens", fn);
     const int n_kv = a.kv.n_kv;
     if (batch < 1 || n_heads < n_kv || n_heads % n_kv || n_heads > 65535)
@@ -164,7 +164,7 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
     const char* fn = "nmi_kv_append_paged";
     if (take_async_error(fn, AsyncKind::Paged)) return NMI_ERR_ASYNC;
     AppendArgs a{};
-    if (const int rc = check_cache(fn, cache, &a.kv)) return rc;
+    if (const int rc = check_cache(fn, cache, &a.kv, &a.blocks)) return rc;
     if (!k_bf16 || !v_bf16 || !start_pos) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL k, v or start_pos", fn);
     if (batch < 1 || tokens < 1 || tokens > kMaxGroups256 || (!cu_seqlens && tokens != batch))
         return refuse(NMI_ERR_INVALID_ARG,
@@ -269,7 +269,7 @@ int nmi_kv_bounds_paged(const nmi_paged_kv* cache, void* k_bounds_bf16, const in
     const char* fn = "nmi_kv_bounds_paged";
     if (take_async_error(fn, AsyncKind::Paged)) return NMI_ERR_ASYNC;
     BoundsArgs a{};
-    if (const int rc = check_cache(fn, cache, &a.kv)) return rc;
+    if (const int rc = check_cache(fn, cache, &a.kv, &a.blocks)) return rc;
     if (!k_bounds_bf16 || !start_pos) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL k_bounds or start_pos", fn);
     if (batch < 1 || tokens < 1 || (!cu_seqlens && tokens != batch) || batch > kMaxGroups256 || tokens > kMaxGroups256 ||
         most_pages_completed(tokens, batch, a.kv.page_shift) >= kMaxGroups256 || a.kv.n_kv > 65535)
@@ -342,7 +342,7 @@ int nmi_sdpa_decode_paged_sparse(const nmi_paged_kv* cache, const void* q_bf16, 
         s.out_lens = reinterpret_cast<int32_t*>(base + w.lens);
         a.kv.page_table = s.rows;
         a.kv.table_stride = (int64_t)a.kv.n_kv * n_select;
-        a.kv.table_head_stride = n_select;
+        a.table_head_stride = n_select;
         a.kv.max_pages = n_select;
         a.lens = s.out_lens;
     }

@@ -177,6 +177,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
     const float lowest = sc > 1.f ? -0x1p127f * __builtin_amdgcn_rcpf(sc) : -FLT_MAX;
     const int page_mask = (1 << a.kv.page_shift) - 1;
     const int64_t head_off = kvh * a.kv.head_stride;
+    const int32_t* table = a.kv.page_table + (int64_t)kvh * a.table_head_stride;
 
     // DMA: instruction k brings 1 KiB, rows r = (1024 / kRow) k + lane / (kRow / 16) of a tile
     constexpr int kChunks = F::kRow / 16, kDma = F::kTile / 1024;        // per row; per tile
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         nx.first = true;
         nx.whole = stop - at == tiles;
         nx.bad = (__builtin_amdgcn_ballot_w64(v.bad) >> i) & 1;
-        nx.row = a.kv.page_table + nx.b * a.kv.table_stride + kvh * a.kv.table_head_stride;
+        nx.row = table + nx.b * a.kv.table_stride;
         at = stop;
         if (nx.pos < nx.stop) ask();
     };
@@ -257,8 +258,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
             const int page = checked_page(nx.id[t], a.kv.n_pages, &s.bad);
             if constexpr (BLOCK) {
                 const int64_t i = block_index(page, a.kv.n_kv, kvh, a.kv.page_shift, pos);
-                s.ks[t] = load_const(a.kv.k_blocks + i);
-                s.vs[t] = load_const(a.kv.v_blocks + i);
+                s.ks[t] = load_const(a.blocks.k + i);
+                s.vs[t] = load_const(a.blocks.v + i);
             }
             const int64_t off = page * a.kv.page_stride + head_off + (int64_t)(pos & page_mask) * a.kv.token_stride;
             const uint8_t *kb = a.kv.k_pages + off, *vb = a.kv.v_pages + off;
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         return __builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0);
     };
     auto odd_values = [&](int b, int pos, int stop) __attribute__((always_inline)) {
-        const int32_t* row = a.kv.page_table + b * a.kv.table_stride + kvh * a.kv.table_head_stride;
+        const int32_t* row = table + b * a.kv.table_stride;
         float2 x{0.f, 0.f};
         for (; pos < stop; pos += stride) {
             bool none = false;          // (reported by the stage that met it)
