@@ -649,26 +649,28 @@ def _front(name: str, *also: str):
     """The front end's function of that name, and the addresses of the library's nmi_ entries: its own and
     those of `also`."""
     got = _entries.get(name)
-    L = _lib.lib()
-    if got is None or got[0] is not L:
+    if got is None or got[0] is not _lib._lib:
+        L = _lib.lib()
         try:
             from .csrc import front
         except ImportError as e:
             raise ImportError(f"{e}: build it with `python -m nemotron_infer_amd.build`") from e
         addresses = [ctypes.cast(getattr(L, "nmi_" + n), ctypes.c_void_p).value for n in (name, *also)]
-        got = _entries[name] = (L, getattr(front, name), *addresses)
-    return got[1:]
+        got = _entries[name] = (L, (getattr(front, name), *addresses))
+    return got[1]
 
 
-def _elsewhere(dev: int) -> bool:
-    """Whether `dev` is a GPU other than the current device, by which the stream, the launch and the
-    library's per-device state go (torch.cuda.device makes it so)."""
+def _stream_on(dev: int):
+    """torch's current stream as a hipStream_t where `dev` is the current device, by which the launch and the
+    library's per-device state go; None where it is another GPU (torch.cuda.device makes it so), 0 where
+    it is none (the front end refuses it)."""
     if dev < 0:
-        return False                           # (the front end refuses it)
+        return 0
     try:
-        return dev != torch._C._cuda_getDevice()
-    except AttributeError:                     # private to torch: another version may lack it
-        return dev != torch.cuda.current_device()
+        current = torch._C._cuda_getDevice()
+        return torch._C._cuda_getCurrentRawStream(current) if dev == current else None
+    except AttributeError:                     # private to torch: another version may lack them
+        return torch.cuda.current_stream().cuda_stream if dev == torch.cuda.current_device() else None
 
 
 def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -685,12 +687,13 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     and k_out, which receives the rotated k where it is given; either may be its input itself.  Rows of
     no sequence, or of one that is not in use, are left as they were in both (in a new q_out: undefined)."""
     dev = k.get_device()
-    if _elsewhere(dev):
+    stream = _stream_on(dev)
+    if stream is None:
         with torch.cuda.device(dev):
             return kv_append_paged(k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q, inv_freq, interleaved,
                                    k_scale, v_scale, q_out, k_out)
     call, entry = _front("kv_append_paged")
-    return call(_lib.check, _stream() if dev >= 0 else 0, entry, k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q,
+    return call(_lib.check, stream, entry, k, v, k_pages, v_pages, page_table, start_pos, cu_seqlens, q,
                 inv_freq, interleaved, k_scale, v_scale, q_out, k_out)
 
 
@@ -702,11 +705,12 @@ def sdpa_decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     (as kv_append_paged takes them, scales too); a length of 0 gives zeros.  scale: 1 / sqrt(128) unless given.
     Returns o [batch, n_heads * 128] bf16."""
     dev = q.get_device()
-    if _elsewhere(dev):
+    stream = _stream_on(dev)
+    if stream is None:
         with torch.cuda.device(dev):
             return sdpa_decode_paged(q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale, scale, out)
     call, entry, ws_bytes = _front("sdpa_decode_paged", "sdpa_decode_paged_workspace_bytes")
-    return call(_lib.check, _stream() if dev >= 0 else 0, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
+    return call(_lib.check, stream, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
                 kv_lens, k_scale, v_scale, scale, out)
 
 
@@ -720,12 +724,13 @@ def sdpa_decode_paged_sparse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: to
     with one of the KV head's queries; all pages where there are no more.  selected (int32 [batch,
     n_kv_heads, n_select]) receives their places in the sequence, ascending, then -1.  Returns o."""
     dev = q.get_device()
-    if _elsewhere(dev):
+    stream = _stream_on(dev)
+    if stream is None:
         with torch.cuda.device(dev):
             return sdpa_decode_paged_sparse(q, k_pages, v_pages, page_table, kv_lens, k_bounds, n_select, k_scale, v_scale,
                                             scale, out, selected)
     call, entry, ws_bytes = _front("sdpa_decode_paged_sparse", "sdpa_decode_paged_sparse_workspace_bytes")
-    return call(_lib.check, _stream() if dev >= 0 else 0, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
+    return call(_lib.check, stream, entry, ws_bytes, _workspace, _kept, q, k_pages, v_pages, page_table,
                 kv_lens, k_bounds, n_select, k_scale, v_scale, scale, out, selected)
 
 
@@ -737,11 +742,12 @@ def kv_bounds_paged(k_pages: torch.Tensor, page_table: torch.Tensor, start_pos: 
     there, tokens the rows that cu_seqlens divides (None, both: one token per sequence).  Written to
     k_bounds [n_pages, n_kv_heads, 2, 128] bf16 (minimum, maximum), which is returned; other pages' stay."""
     dev = k_pages.get_device()
-    if _elsewhere(dev):
+    stream = _stream_on(dev)
+    if stream is None:
         with torch.cuda.device(dev):
             return kv_bounds_paged(k_pages, page_table, start_pos, k_bounds, cu_seqlens, tokens, k_scale)
     call, entry = _front("kv_bounds_paged")
-    return call(_lib.check, _stream() if dev >= 0 else 0, entry, k_pages, page_table, start_pos, k_bounds, cu_seqlens, tokens,
+    return call(_lib.check, stream, entry, k_pages, page_table, start_pos, k_bounds, cu_seqlens, tokens,
                 k_scale)
 
 
@@ -766,12 +772,13 @@ def kv_assign_paged(lens: torch.Tensor, new_lens: torch.Tensor | None, page_tabl
     the table or the pages left is granted none (start_pos -1).  lens_out and free_count_out may be lens and
     free_count themselves, so that a captured step goes on from where it ended."""
     dev = lens.get_device()
-    if _elsewhere(dev):
+    stream = _stream_on(dev)
+    if stream is None:
         with torch.cuda.device(dev):
             return kv_assign_paged(lens, new_lens, page_table, free_pages, free_count, page_size, tokens, lens_out,
                                    free_count_out)
     call, entry = _front("kv_assign_paged")
-    return PagedStep(*call(_lib.check, _stream() if dev >= 0 else 0, entry, lens, new_lens, page_table, free_pages, free_count,
+    return PagedStep(*call(_lib.check, stream, entry, lens, new_lens, page_table, free_pages, free_count,
                            page_size, tokens, lens_out, free_count_out))
 
 
@@ -783,11 +790,12 @@ def sdpa_prefill_packed_bf16(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     are prompt b (row-strided views allowed).  scale: 1 / sqrt(128) unless given.  Returns o
     [T, n_heads * 128] bf16; rows of no prompt are left as they were (in a new o: undefined)."""
     dev = q.get_device()
-    if _elsewhere(dev):
+    stream = _stream_on(dev)
+    if stream is None:
         with torch.cuda.device(dev):
             return sdpa_prefill_packed_bf16(q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
     call, entry = _front("sdpa_prefill_packed_bf16")
-    return call(_lib.check, _stream() if dev >= 0 else 0, entry, q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
+    return call(_lib.check, stream, entry, q, k, v, cu_seqlens, n_heads, n_kv_heads, scale, out)
 
 
 class GemvChain:
