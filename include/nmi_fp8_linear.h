@@ -510,7 +510,8 @@ int nmi_kv_bounds_paged(const nmi_paged_kv* cache, void* k_bounds_bf16, const in
  * The work is split by the lengths found on the device: the launch depends on the batch size only.
  * workspace: nmi_sdpa_decode_paged_workspace_bytes(batch, n_heads, n_kv_heads) bytes, 16-byte aligned,
  * no initialisation; NULL takes it from the bump allocator.  Two launches, the second joining the splits
- * in a fixed order: equal calls give the same bytes.  o overlaps no input.  Pages that are not attended may
+ * in a fixed order: equal calls give the same bytes.  (NMI_KV_E4M3_BLOCK where the table's rows hold few positions,
+ * 640, or 1024 with a sequence and KV head for every CU: one launch.)  o overlaps no input.  Pages that are not attended may
  * hold anything; an attended infinity in v gives that infinity in its dim, or NaN beside one of the other
  * sign (or where its weight underflows).  Of NMI_KV_E4M3_BLOCK, scores and weights times their block's scale are rounded
  * to float32 once more, and weights times v's scale have to lie within its range: magnitudes of v between 2^-100 and
@@ -531,8 +532,8 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
  * attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type; scale does not change the
  * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first.
  * workspace: nmi_sdpa_decode_paged_sparse_workspace_bytes(batch, n_heads, n_kv_heads, max_pages, n_select) bytes,
- * 16-byte aligned, no initialisation; NULL takes it from the bump allocator.  Four launches; two where n_select >=
- * max_pages.
+ * 16-byte aligned, no initialisation; NULL takes it from the bump allocator.  Four launches; three where n_select pages
+ * hold as few positions as above; the decode's alone where n_select >= max_pages.
  */
 size_t nmi_sdpa_decode_paged_sparse_workspace_bytes(int batch, int n_heads, int n_kv_heads, int max_pages, int n_select);
 int nmi_sdpa_decode_paged_sparse(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,

@@ -344,7 +344,11 @@ struct PagedDecodeArgs {
 };
 int sdpa_decode_paged_waves(int n_kv, int group);
 size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv);
-hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, KvForm form, void* workspace, hipStream_t stream);
+// whole: a workgroup for each sequence's KV head, in one launch; otherwise all sequences' positions in equal shares, and
+// a launch that joins them.  sdpa_decode_paged_whole: whether the former is faster where no sequence can have more than
+// so many positions: always for few of them, for some more where there are workgroups for every CU.
+bool sdpa_decode_paged_whole(int64_t positions, int batch, int n_kv, int group);
+hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, KvForm form, bool whole, void* workspace, hipStream_t stream);
 
 // Mamba-2 mixer at decode (mamba_decode.hip): conv1d step + SiLU, SSM state update and
 // output, gated RMSNorm, for `batch` sequences of one token.  Shapes: H heads of P, G groups,

@@ -131,6 +131,11 @@ int check_decode(const char* fn, const nmi_paged_kv* cache, const void* q_bf16, 
     return NMI_OK;
 }
 
+// Whether the decode's sequences are short enough for a workgroup each (by what the table's rows can hold).
+bool whole_rows(const PagedDecodeArgs& a) {
+    return sdpa_decode_paged_whole((int64_t)a.kv.max_pages << a.kv.page_shift, a.batch, a.kv.n_kv, a.group);
+}
+
 // A workspace given, checked, or one from the bump allocator.
 int take_workspace(const char* fn, size_t need, void** workspace, size_t bytes) {
     if (!*workspace) return nmi_alloc(need, workspace);
@@ -302,7 +307,10 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
     const size_t need = sdpa_decode_paged_workspace_bytes(batch, n_heads, a.kv.n_kv);
     if (const int rc = take_workspace(fn, need, &workspace, workspace_bytes)) return rc;
     a.kv.error = async_error_word(AsyncKind::Paged);
-    return hip_status(launch_sdpa_decode_paged(a, form_of(cache), workspace, static_cast<hipStream_t>(stream)), fn);
+    const KvForm form = form_of(cache);
+    // (the older forms keep the order of their sums)
+    return hip_status(launch_sdpa_decode_paged(a, form, form == KvForm::Block && whole_rows(a), workspace, static_cast<hipStream_t>(stream)),
+                      fn);
 }
 
 size_t nmi_sdpa_decode_paged_sparse_workspace_bytes(int batch, int n_heads, int n_kv_heads, int max_pages, int n_select) {
@@ -350,7 +358,7 @@ int nmi_sdpa_decode_paged_sparse(const nmi_paged_kv* cache, const void* q_bf16, 
         if (const int rc = hip_status(launch_page_select(s, static_cast<hipStream_t>(stream)), fn)) return rc;
     a.kv.error = async_error_word(AsyncKind::Paged);
     return hip_status(
-        launch_sdpa_decode_paged(a, form_of(cache), base + w.decode, static_cast<hipStream_t>(stream)), fn);
+        launch_sdpa_decode_paged(a, form_of(cache), whole_rows(a), base + w.decode, static_cast<hipStream_t>(stream)), fn);
 }
 
 int nmi_sdpa_prefill_packed_bf16(const void* q_bf16, int64_t ldq, const void* k_bf16, int64_t ldk, const void* v_bf16,

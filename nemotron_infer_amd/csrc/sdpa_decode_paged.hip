@@ -33,6 +33,12 @@
 //   reads transpose pairs of dims, whose bytes are then sorted: the even dims of a block go to one
 //   product, the odd ones to the next.
 //
+// Short sequences of the newer forms (scales of blocks; selected pages) are not split: a workgroup takes a sequence's KV
+// head (sdpa_decode_paged_whole says when), which saves the scan over the lengths and the second launch.  One of 16 /
+// 256 / 512 / 1024 positions 3.9 / 5.0 / 6.9 / 10.6 us, split 6.3 / 8.5 / 8.7 / 8.7; 64 of 512 / 1024 (16 / 4 heads) 8.7 /
+// 13.7, split 12.5 / 17.3.  (Eight waves to a workgroup: 4.3 / 5.1 / 6.5 / 9.0 and 9.0 / 13.5.)  The older forms keep the order
+// of their sums.
+//
 // Measured (graph replays, both launches; 40 query, 8 KV heads): one sequence of 777 positions 8.4 us, of
 // 65536 45 (6.0 TB/s of the cache's bytes; a streaming read of as many 6.5); e4m3, 131072 positions 48.5
 // (5.5); 64 of 90 to 8000 positions, e4m3, 48.6 (4.9); 128 of 500 48.4 (5.4).  What is left of a long one is the
@@ -60,6 +66,7 @@ constexpr int kStages = 2;                      // per wave
 constexpr int kCols = 16;                       // query heads per wave
 constexpr int kLds = kWaves * kStages * kStage;  // the stages; afterwards the waves' parts
 static_assert(kWgs * kLds <= 160 * 1024 && kWaves * kCols * (kD + 2) * 4 <= kLds, "LDS");
+constexpr int kWholeAlways = 640, kWholeMost = 1024;    // sdpa_decode_paged_whole
 constexpr float kLazy = 8.f;                    // log2 of the largest unnormalised weight
 
 __device__ __forceinline__ float fexp2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -114,8 +121,8 @@ struct Stage {
     float ks[2], vs[2];     // block scales: of each tile
 };
 
-// MANY: more sequences than lanes.
-template <KvForm FORM, bool MANY>
+// MANY: more sequences than lanes.  WHOLE: a workgroup takes a sequence's KV head, and no second kernel follows.
+template <KvForm FORM, bool MANY, bool WHOLE>
 __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const PagedDecodeArgs a) {
     constexpr bool E4M3 = FORM != KvForm::Bf16, BLOCK = FORM == KvForm::Block;
     typedef Form<E4M3> F;
@@ -129,24 +136,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
     const uint32_t me = blockIdx.x * kWaves + wave;
 
     // this wave's tiles, and the sequence that they begin in
-    Lanes v = load_lanes(a, 0, 0, lane);
-    uint32_t total = lane_u32(v.upto, 63);
-    if constexpr (MANY) {
-        uint32_t tiles = v.tiles;
-        for (int b0 = 64; b0 < a.batch; b0 += 4 * 64)           // (lengths of four times 64 on their way at once)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tiles += tiles_at(a, b0 + 64 * c + lane);
-        total = lane_u32(wave_scan_u32(tiles), 63);
-    }
-    const int c = range_tiles(total, a.waves, F::kTiles);
-    if (me + 1 == (uint32_t)a.waves && kvh == 0 && r0 == 0) {
-        // for the joining kernel (the last wave: the first to have no tiles)
-        for (Lanes w = v;; w = load_lanes(a, w.b0 + 64, lane_u32(w.upto, 63), lane)) {
-            const Pieces p = w.tiles ? pieces_of(w.upto - w.tiles, w.tiles, c, total) : Pieces{};
-            if (w.b0 + lane < a.batch) a.plan[w.b0 + lane] = p;
-            if (!MANY || w.b0 + 64 >= a.batch) break;
-        }
-    }
+    Lanes v;
+    uint32_t at, end;
+    int i = 0;
+    bool joint;
     // the first sequence with tiles past `at`: its lane; 64 where there is none (only if the lengths change
     // under the launch)
     auto seek = [&](uint32_t at) {
@@ -155,17 +148,52 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
                 v = load_lanes(a, v.b0 + 64, lane_u32(v.upto, 63), lane);
         return __popcll(__builtin_amdgcn_ballot_w64(v.upto <= at));
     };
-    uint32_t at = range_first(blockIdx.x * kWaves, c, total), end = range_first((blockIdx.x + 1) * kWaves, c, total);
-    if (at >= end) return;
-    int i = seek(at);
-    if (MANY && i == 64) return;
-    const bool joint = is_joint(blockIdx.x, lane_u32(v.upto - v.tiles, i), lane_u32(v.tiles, i), c, total);
-    if (!joint) {
-        at = range_first(me, c, total);
-        end = range_first(me + 1, c, total);
+    if constexpr (WHOLE) {
+        // (one sequence: as if it were all that there is)
+        v.b0 = blockIdx.x;
+        v.bad = false;
+        v.len = checked_len(load_const(a.lens + v.b0), a.kv.max_pages, a.kv.page_shift, &v.bad);
+        v.tiles = v.upto = (uint32_t)(v.len + kPagedTile - 1) / kPagedTile;
+        at = 0;
+        end = v.tiles;
+        joint = true;
+        if (!v.len) {
+            uint32_t* o = reinterpret_cast<uint32_t*>(a.o + (int64_t)v.b0 * a.ldo + (int64_t)head0 * kD);
+            for (int k = tid; k < nrow * (kD / 2); k += 64 * kWaves) o[k] = 0u;
+            return;
+        }
+    } else {
+        v = load_lanes(a, 0, 0, lane);
+        uint32_t total = lane_u32(v.upto, 63);
+        if constexpr (MANY) {
+            uint32_t tiles = v.tiles;
+            for (int b0 = 64; b0 < a.batch; b0 += 4 * 64)           // (lengths of four times 64 on their way at once)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tiles += tiles_at(a, b0 + 64 * c + lane);
+            total = lane_u32(wave_scan_u32(tiles), 63);
+        }
+        const int c = range_tiles(total, a.waves, F::kTiles);
+        if (me + 1 == (uint32_t)a.waves && kvh == 0 && r0 == 0) {
+            // for the joining kernel (the last wave: the first to have no tiles)
+            for (Lanes w = v;; w = load_lanes(a, w.b0 + 64, lane_u32(w.upto, 63), lane)) {
+                const Pieces p = w.tiles ? pieces_of(w.upto - w.tiles, w.tiles, c, total) : Pieces{};
+                if (w.b0 + lane < a.batch) a.plan[w.b0 + lane] = p;
+                if (!MANY || w.b0 + 64 >= a.batch) break;
+            }
+        }
+        at = range_first(blockIdx.x * kWaves, c, total);
+        end = range_first((blockIdx.x + 1) * kWaves, c, total);
         if (at >= end) return;
         i = seek(at);
         if (MANY && i == 64) return;
+        joint = is_joint(blockIdx.x, lane_u32(v.upto - v.tiles, i), lane_u32(v.tiles, i), c, total);
+        if (!joint) {
+            at = range_first(me, c, total);
+            end = range_first(me + 1, c, total);
+            if (at >= end) return;
+            i = seek(at);
+            if (MANY && i == 64) return;
+        }
     }
     constexpr int kStep = F::kTiles * kPagedTile;               // positions of a stage
     const int stride = joint ? kWaves * kStep : kStep;          // from one of a wave's stages to its next
@@ -214,7 +242,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void sdpa_decode_paged_kernel(const
         nx.stop = min((int)lane_u32((uint32_t)v.len, i), (int)(stop - first) * kPagedTile);
         nx.first = true;
         nx.whole = stop - at == tiles;
-        nx.bad = (__builtin_amdgcn_ballot_w64(v.bad) >> i) & 1;
+        nx.bad = WHOLE ? v.bad : (__builtin_amdgcn_ballot_w64(v.bad) >> i) & 1;
         nx.row = table + nx.b * a.kv.table_stride;
         at = stop;
         if (nx.pos < nx.stop) ask();
@@ -670,16 +698,26 @@ __global__ __launch_bounds__(64 * kWaves) void sdpa_decode_paged_join_kernel(con
 template <KvForm FORM, bool MANY>
 hipError_t launch(const PagedDecodeArgs& a, hipStream_t stream) {
     static const hipError_t attr =
-        hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_decode_paged_kernel<FORM, MANY>),
+        hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_decode_paged_kernel<FORM, MANY, false>),
                             hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return attr;
     const dim3 grid(a.waves / kWaves, a.kv.n_kv, (a.group + kCols - 1) / kCols);
-    hipLaunchKernelGGL((sdpa_decode_paged_kernel<FORM, MANY>), grid, dim3(64 * kWaves), kLds, stream, a);
+    hipLaunchKernelGGL((sdpa_decode_paged_kernel<FORM, MANY, false>), grid, dim3(64 * kWaves), kLds, stream, a);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     // Many sequences are in few pieces each, most in one: workgroups that find nothing to do are what it costs.
     const int heads = std::min(8, (int)(((int64_t)a.batch * a.H + 2047) / 2048));
     hipLaunchKernelGGL(sdpa_decode_paged_join_kernel, dim3(a.batch, (a.H + heads - 1) / heads), dim3(64 * kWaves), 0, stream,
                        a, heads);
+    return hipGetLastError();
+}
+
+template <KvForm FORM>
+hipError_t launch_whole(const PagedDecodeArgs& a, hipStream_t stream) {
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&sdpa_decode_paged_kernel<FORM, false, true>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (attr != hipSuccess) return attr;
+    const dim3 grid(a.batch, a.kv.n_kv, (a.group + kCols - 1) / kCols);
+    hipLaunchKernelGGL((sdpa_decode_paged_kernel<FORM, false, true>), grid, dim3(64 * kWaves), kLds, stream, a);
     return hipGetLastError();
 }
 
@@ -702,17 +740,29 @@ int sdpa_decode_paged_waves(int n_kv, int group) {
     return std::max(1, kWgs * device_info().num_cu / per) * kWaves;
 }
 
+bool sdpa_decode_paged_whole(int64_t positions, int batch, int n_kv, int group) {
+    if (positions > kWholeMost) return false;
+    return positions <= kWholeAlways || (int64_t)batch * n_kv * ((group + kCols - 1) / kCols) >= device_info().num_cu;
+}
+
 size_t sdpa_decode_paged_workspace_bytes(int batch, int n_heads, int n_kv) {
     return layout(batch, n_heads, sdpa_decode_paged_waves(n_kv, n_heads / n_kv)).total;
 }
 
-hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, KvForm form, void* workspace, hipStream_t stream) {
+hipError_t launch_sdpa_decode_paged(PagedDecodeArgs a, KvForm form, bool whole, void* workspace, hipStream_t stream) {
     a.waves = sdpa_decode_paged_waves(a.kv.n_kv, a.group);
     const Layout w = layout(a.batch, a.H, a.waves);
     char* base = static_cast<char*>(workspace);
     a.part_o = reinterpret_cast<float*>(base + w.part_o);
     a.part_ml = reinterpret_cast<float2*>(base + w.part_ml);
     a.plan = reinterpret_cast<Pieces*>(base + w.plan);
+    if (whole) {
+        switch (form) {
+            case KvForm::Bf16: return launch_whole<KvForm::Bf16>(a, stream);
+            case KvForm::E4m3: return launch_whole<KvForm::E4m3>(a, stream);
+            default: return launch_whole<KvForm::Block>(a, stream);
+        }
+    }
     const bool many = a.batch > 64;
     switch (form) {
         case KvForm::Bf16: return many ? launch<KvForm::Bf16, true>(a, stream) : launch<KvForm::Bf16, false>(a, stream);

@@ -251,7 +251,7 @@ for tokens, batch, packed in ((1, 1, 0), (24, 24, 0), (9000, 9000, 0), (1, 1, 1)
 
 def test_sparse_launches_fit_the_workspace(host):  # noqa: F811
     """Scores, the chosen pages, their lengths and the decode's own workspace, in turn; two launches less where there is
-    nothing to choose."""
+    nothing to choose, one less where few positions are attended."""
     got = host(CACHE + """
 result = []
 for batch, H, n_kv, kind, max_pages, select in ((1, 40, 8, 2, 1563, 32), (20, 32, 8, 0, 900, 63), (70, 4, 2, 1, 8, 1), (3, 16, 4, 2, 8, 8),
@@ -268,12 +268,36 @@ for batch, H, n_kv, kind, max_pages, select in ((1, 40, 8, 2, 1563, 32), (20, 32
 """)
     for batch, H, n_kv, max_pages, select, need, dense, first, again in got:
         groups, up = batch * n_kv, lambda n: -(-n // 16) * 16
+        decode = 1 if 16 * min(select, max_pages) <= 640 else 2
         if select >= max_pages:
-            assert need == dense and len(first) == 2 and again == 3
+            assert need == dense and len(first) == decode and again == decode + 1
             continue
         assert need == up(4 * groups * max_pages) + up(4 * groups * select) + up(4 * batch) + dense
-        assert len(first) == again == 4
+        assert len(first) == again == 2 + decode
         assert first[0][0] % groups == 0 and first[0][0] // groups <= -(-max_pages // 16) and first[1][0] == groups
+    assert {len(first) for *_, first, _ in got} == {1, 3, 4}
+
+
+def test_decode_launches(host):  # noqa: F811
+    """Under scales of blocks one launch, a workgroup to a sequence's KV head (and 16 of its heads), where the rows of the
+    table hold few positions; two otherwise, and always over the older caches."""
+    got = host(CACHE + """
+result = []
+for kind in (0, 1, 2):
+    for batch, H, n_kv, page, max_pages in ((1, 40, 8, 16, 1), (1, 40, 8, 16, 40), (1, 40, 8, 16, 41), (31, 40, 8, 64, 16), (32, 40, 8, 64, 16),
+                                            (300, 40, 8, 64, 17), (300, 33, 1, 32, 20)):
+        c = cache(kind=kind, page=page, max_pages=max_pages, n_kv=n_kv)
+        need = L.nmi_sdpa_decode_paged_workspace_bytes(batch, H, n_kv)
+        rc = L.nmi_sdpa_decode_paged(ctypes.addressof(c), W, H * 128, W, H * 128, W, batch, H, 0.1, W, need, ST)
+        assert rc == 0, L.nmi_last_error()
+        result.append([kind, batch, H, n_kv, page * max_pages, [l[1:] for l in launches()]])
+""")
+    for kind, batch, H, n_kv, most, launches in got:
+        z = -(-(H // n_kv) // 16)
+        if kind == 2 and (most <= 640 or (most <= 1024 and batch * n_kv * z >= 256)):
+            assert launches == [[batch, n_kv, z, 256]]
+        else:
+            assert len(launches) == 2 and launches[0][1:] == [n_kv, z, 256]
 
 
 # --- refusals --------------------------------------------------------------------------------------
