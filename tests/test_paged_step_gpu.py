@@ -116,6 +116,17 @@ def test_decode_any_positive_scales_and_ragged_batches():
         _check_decode(rng, lens, 8, 2, 16, label=f"{len(lens)} sequences")
 
 
+@pytest.mark.parametrize("batch,H,n_kv,page,width", [(3, 40, 8, 16, 40), (3, 40, 8, 16, 41), (40, 16, 8, 64, 16), (40, 16, 8, 64, 17), (70, 33, 1, 32, 32),
+                                                     (300, 4, 1, 256, 4)])
+def test_decode_on_both_sides_of_the_launches_choice(batch, H, n_kv, page, width):
+    """Tables whose rows hold just so many positions as a workgroup takes alone, and more; lengths of all kinds in them."""
+    announce("block_whole", batch, H, n_kv, page * width)
+    rng = np.random.default_rng(batch + width)
+    lens = [int(n) for n in rng.integers(0, page * width + 1, batch)]
+    lens[0], lens[-1], lens[1] = page * width, 1, 0
+    _check_decode(rng, lens, H, n_kv, page, label=f"{page * width}", width=width)
+
+
 def test_decode_is_the_same_every_time_and_equals_scales_of_heads():
     """One scale everywhere: as under a scale per head, up to where float32 rounds (powers of two: nowhere)."""
     announce("block_repeat")
@@ -271,6 +282,56 @@ def test_append_many_sequences_of_odd_lengths():
     lens = [int(n) for n in rng.integers(0, 5, 300)]
     _check_append(rng, [int(s) for s in rng.integers(-2, 40, 300)], lens, 4, 1, 16, 32, True, lead=1, tail=70, grow=4)
     _check_append(rng, [15] * 130, [18] * 130, 2, 2, 32, 0, False)              # the most blocks that rows can need
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_append_rotates_keys_alone(packed):
+    """No q, and no k returned: the cache as with them."""
+    announce("block_append_keys", packed)
+    rng = np.random.default_rng(28)
+    a, b = (BlockPool(np.random.default_rng(29), [3, 20, 7], 2, 32, hold=[40, 40, 40]) for _ in range(2))
+    x, f, start = _dev(_rand_bits(rng, 3, 8 * 128)), _dev(np.ones(64, np.float32)), _dev(np.array([3, 20, 7], np.int32))
+    k, v, q = x[:, :256], x[:, 256:512], x[:, 512:]
+    cu = _dev(np.arange(4, dtype=np.int32)) if packed else None
+    got = ops.kv_append_paged(k, v, a.dk, a.dv, a.dtable, start, cu_seqlens=cu, inv_freq=f, k_scale=a.dks, v_scale=a.dvs)
+    ops.kv_append_paged(k, v, b.dk, b.dv, b.dtable, start, cu_seqlens=cu, q=q, inv_freq=f, k_scale=b.dks, v_scale=b.dvs,
+                        k_out=torch.empty_like(k))
+    assert got == (None, None)
+    for s, t in ((a.dk, b.dk), (a.dv, b.dv), (a.dks, b.dks), (a.dvs, b.dvs)):
+        assert _same(s, t)
+
+
+def test_the_largest_page():
+    """Pages of 2^20 positions: appended across a block border, bounded, and attended."""
+    announce("block_largest_page")
+    rng = np.random.default_rng(30)
+    page, n = 1 << 20, 40
+    pages = [torch.zeros(2, 1, page, 128, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    scales = [torch.ones(2, 1, page // 16, device=DEV) for _ in range(2)]
+    table, start = _dev(np.array([[1, 0]], np.int32)), page - 30
+    k, v, q = (_rand_bits(rng, m, 128) for m in (n, n, 1))
+    args = dict(cu_seqlens=_dev(np.array([0, n], np.int32)), k_scale=scales[0], v_scale=scales[1])
+    ops.kv_append_paged(_dev(k), _dev(v), *pages, table, _dev(np.array([start], np.int32)), **args)
+    bounds = torch.zeros(2, 1, 2, 128, dtype=torch.bfloat16, device=DEV)
+    ops.kv_bounds_paged(pages[0], table, _dev(np.array([start], np.int32)), bounds, cu_seqlens=args["cu_seqlens"], tokens=n, k_scale=scales[0])
+    lens = _dev(np.array([start + n], np.int32))
+    o = ops.sdpa_decode_paged(_dev(q), *pages, table, lens, k_scale=scales[0], v_scale=scales[1], scale=2.0)
+    sparse = ops.sdpa_decode_paged_sparse(_dev(q), *pages, table, lens, bounds, 1, k_scale=scales[0], v_scale=scales[1], scale=2.0)
+    torch.cuda.synchronize()
+    held = []                                             # the new positions' values, and the zeros before them
+    for c, s, x in zip(pages, scales, (k, v)):
+        rows = torch.cat([c[1, 0, -30:], c[0, 0, :10]]).cpu().numpy()
+        by = torch.cat([s[1, 0].repeat_interleave(16)[-30:], s[0, 0, :1].repeat(10)]).cpu().numpy()
+        held.append(LUT[rows] * by[:, None])
+        assert np.abs(held[-1] - _f64(x)).max() <= 2.0 ** -4 * np.abs(_f64(x)).max()
+    e = np.concatenate([np.zeros(start), 2.0 * (held[0] @ _f64(q)[0])])
+    w = np.exp(e - e.max())
+    assert_parity(bits(o), block.bf16_round_exact((w[start:] @ held[1])[None] / w.sum()), "largest page")
+    w = np.exp(e[page:] - e[page:].max())
+    assert_parity(bits(sparse), block.bf16_round_exact((w @ held[1][30:])[None] / w.sum()), "its newest page")
+    whole = np.concatenate([np.zeros((1, 128)), held[0][:30]])
+    assert np.array_equal(_f64(bits(bounds[1, 0])), np.stack([_bf16(whole.min(0)), _bf16(whole.max(0))]))
+    assert not bounds[0].any() and _lib.lib().nmi_async_status() == 0
 
 
 def test_append_token_by_token_follows_the_values():
@@ -638,6 +699,23 @@ def test_sparse_bad_pages_and_lengths_are_reported():
             assert np.array_equal(got[[0, 2]], good[[0, 2]])
         assert _lib.lib().nmi_async_status() == _lib.NMI_ERR_ASYNC and _lib.lib().nmi_async_status() == 0
     assert np.array_equal(run(pool.table, pool.lens), good)
+
+
+@pytest.mark.parametrize("select", [2, 30])
+def test_sparse_strides_and_outputs(select):
+    """q and o as columns of wider buffers; the rest of o's buffer stays as it was."""
+    announce("sparse_strides", select)
+    rng = np.random.default_rng(76)
+    pool = BlockPool(rng, [1000, 5, 0], 2, 32)
+    bounds = _dev(block.bf16_round_exact(np.nan_to_num(paged.page_bounds(_f32_keys(pool)))))
+    wide = torch.full((3, 8 * 128 + 72), 9.0, dtype=torch.bfloat16, device=DEV)
+    wide[:, 8:8 + 1024] = _dev(_rand_bits(rng, 3, 8 * 128))
+    out = torch.full((3, 8 * 128 + 6), 7.0, dtype=torch.bfloat16, device=DEV)
+    args = (pool.dk, pool.dv, pool.dtable, _dev(pool.lens), bounds, select)
+    got = ops.sdpa_decode_paged_sparse(wide[:, 8:1032], *args, k_scale=pool.dks, v_scale=pool.dvs, out=out[:, 2:1026])
+    alone = ops.sdpa_decode_paged_sparse(wide[:, 8:1032].contiguous(), *args, k_scale=pool.dks, v_scale=pool.dvs)
+    assert _same(got, alone) and not alone[2].any() and alone[:2].any()
+    assert (out[:, :2] == 7).all() and (out[:, 1026:] == 7).all()
 
 
 def test_sparse_takes_its_workspace_from_the_allocator():
