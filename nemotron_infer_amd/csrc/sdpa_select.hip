@@ -14,11 +14,14 @@
 // bits for what bf16 holds unless they lie 2^45 apart: two multiply-adds, the magnitude for nothing.
 // (Float32 sums instead took 1 us of 20 less for one sequence of 100001 positions, 2 of 43 for 20 documents.)
 //
-// Scores.  Bound: reading the bounds, 512 bytes a page and head.  16 lanes take a page, 8 dims each, the queries in
-// their registers; a wave takes 4 pages at a time, the next ones' bounds on their way.  A sequence's KV head is dealt to
-// as many workgroups as all of them leave it of 8 per CU: 1 / 2 / 4 / 8 / 16 per CU, 20 documents of 900 to 30000 positions
-// (pages of 32, 32 / 8 heads; the whole call) 113 / 62 / 50 / 44.0 / 44.4 us; the pages of all sequences in equal shares
-// 43.4 where this takes 43.1, and one sequence 21.0 where this takes 20.6.
+// Scores.  Bound: the 64-bit arithmetic of many pages, latency of few (length and page id, then bounds and queries).  16
+// lanes take a page, 8 dims each, the queries in their registers; a wave takes 4 pages at a time, the next ones' bounds
+// on their way, all of the chunk's query heads at once so that their sums hide one another's latency (one head after another,
+// 40 sequences of 4000: 39.0 us for the whole call, so 36.7; 16 pages a wave, 4 lanes each, the queries in LDS: 36.8, but one
+// sequence of 60000 18.6 where this takes 17.0).  A sequence's KV head is dealt to as many workgroups as all of them leave it
+// of 8 per CU: 1 / 2 / 4 / 8 / 16 per CU, 20 documents of 900 to 30000 positions (pages of 32, 32 / 8 heads; the whole
+// call, an earlier form) 113 / 62 / 50 / 44.0 / 44.4 us; the pages of all sequences in equal shares 43.4 where that took
+// 43.1, and one sequence 21.0 where that took 20.6.
 // Choice: one workgroup for a sequence's KV head: the range of the scores cut into 1024 bins, counted in LDS, the bin
 // with the last one wanted cut again while it has many, its few ranked one against another; then one pass in order.
 // Bound: latency, a handful of barriers: 4.6 us (traced) of 1562 pages, where four passes of 8 bits and a scan for each
@@ -34,7 +37,7 @@ namespace nmi {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kHeads = 5;               // query heads at a time: 16 registers each
+constexpr int kHeads = 5;               // query heads at a time at most: 16 registers each
 constexpr int kBinBits = 10, kSelectThreads = 1 << kBinBits, kSelectWaves = kSelectThreads / 64;
 constexpr int kKeys = 6144;             // keys and page ids of a sequence kept in LDS
 constexpr int kFew = 64;                // keys ranked by a wave
@@ -51,7 +54,7 @@ __device__ __forceinline__ Sequence sequence(const SelectArgs& a, int b) {
     return s;
 }
 
-// The sum over 16 lanes, in all of them.
+// The sums over 16 lanes, in all of them.
 template <int CTRL>
 __device__ __forceinline__ double dpp_f64(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
@@ -59,15 +62,25 @@ __device__ __forceinline__ double dpp_f64(double v) {
     const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double row_sum16_f64(double v) {
-    v += dpp_f64<0xB1>(v);
-    v += dpp_f64<0x4E>(v);
-    v += dpp_f64<0x141>(v);
-    v += dpp_f64<0x140>(v);
-    return v;
+template <int CTRL, int N>
+__device__ __forceinline__ void add_dpp_f64(double (&v)[N]) {
+    double w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = dpp_f64<CTRL>(v[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += w[i];
+}
+template <int N>
+__device__ __forceinline__ void row_sums16_f64(double (&v)[N]) {
+    add_dpp_f64<0xB1>(v);
+    add_dpp_f64<0x4E>(v);
+    add_dpp_f64<0x141>(v);
+    add_dpp_f64<0x140>(v);
 }
 
-// A workgroup takes every parts-th 16 pages of a sequence's KV head.
+// A workgroup takes every parts-th 16 pages of a sequence's KV head.  HEADS: query heads at a time (the last ones again where
+// there are fewer: their scores are the same).
+template <int HEADS>
 __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a, int parts) {
     const int part = blockIdx.x % parts, g = (int)(blockIdx.x / parts % a.kv.n_kv), b = (int)(blockIdx.x / parts / a.kv.n_kv);
     const int lane = threadIdx.x & 63, sub = lane & 15;
@@ -94,17 +107,15 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a
         return x;
     };
     float* scores = a.scores + ((int64_t)b * a.kv.n_kv + g) * a.kv.max_pages;
-    const int chunks = (a.group + kHeads - 1) / kHeads, per = (a.group + chunks - 1) / chunks;
-    for (int h0 = 0; h0 < a.group; h0 += per) {
+    for (int h0 = 0; h0 < a.group; h0 += HEADS) {
         // a page's bounds are on their way while those before are used, and the id of the next one's
         Bounds next = load(first_id[0]);
         int32_t id = first_id[1];
-        const int heads = min(per, a.group - h0);
-        double q[kHeads][8];
+        double q[HEADS][8];
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
+        for (int h = 0; h < HEADS; ++h) {
             float x[8];
-            unpack8(load16(a.q + (int64_t)b * a.ldq + (int64_t)(g * a.group + h0 + min(h, heads - 1)) * kPagedHead + 8 * sub), x);
+            unpack8(load16(a.q + (int64_t)b * a.ldq + (int64_t)(g * a.group + min(h0 + h, a.group - 1)) * kPagedHead + 8 * sub), x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[h][i] = x[i];
         }
@@ -121,18 +132,20 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a
                 sum_of[i] = (double)hi[i] + (double)lo[i];
                 span[i] = (double)hi[i] - (double)lo[i];
             }
-            float best = -INFINITY;
+            double sum[HEADS];
 #pragma unroll
-            for (int h = 0; h < kHeads; ++h) {
-                if (h >= heads) break;
-                double sum = 0.0;
+            for (int h = 0; h < HEADS; ++h) {
+                sum[h] = 0.0;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    sum = __builtin_fma(q[h][i], sum_of[i], sum);
-                    sum = __builtin_fma(__builtin_fabs(q[h][i]), span[i], sum);
+                    sum[h] = __builtin_fma(q[h][i], sum_of[i], sum[h]);
+                    sum[h] = __builtin_fma(__builtin_fabs(q[h][i]), span[i], sum[h]);
                 }
-                best = __builtin_elementwise_maximum(best, (float)(0.5 * row_sum16_f64(sum)));      // (NaN stays)
             }
+            row_sums16_f64(sum);
+            float best = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) best = __builtin_elementwise_maximum(best, (float)(0.5 * sum[h]));      // (NaN stays)
             if (sub == 0 && p < n) {
                 if (h0) best = __builtin_elementwise_maximum(best, scores[p]);
                 scores[p] = now.bad ? NAN : best;       // (a bad page is the attention's to report)
@@ -275,7 +288,15 @@ hipError_t launch_page_select(const SelectArgs& a, hipStream_t stream) {
         // as many workgroups as keep the CUs busy, or one for each 16 pages that a sequence may have
         const int64_t most = ((int64_t)a.kv.max_pages + 15) / 16, parts = std::max<int64_t>(1, 8 * device_info().num_cu / groups);
         const int p = (int)std::min(most, parts);
-        hipLaunchKernelGGL(page_score_kernel, dim3((uint32_t)(groups * p)), dim3(kThreads), 0, stream, a, p);
+        const int chunks = (a.group + kHeads - 1) / kHeads;
+        const dim3 grid((uint32_t)(groups * p)), block(kThreads);
+        switch ((a.group + chunks - 1) / chunks) {
+            case 1: hipLaunchKernelGGL(page_score_kernel<1>, grid, block, 0, stream, a, p); break;
+            case 2: hipLaunchKernelGGL(page_score_kernel<2>, grid, block, 0, stream, a, p); break;
+            case 3: hipLaunchKernelGGL(page_score_kernel<3>, grid, block, 0, stream, a, p); break;
+            case 4: hipLaunchKernelGGL(page_score_kernel<4>, grid, block, 0, stream, a, p); break;
+            default: hipLaunchKernelGGL(page_score_kernel<kHeads>, grid, block, 0, stream, a, p);
+        }
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(page_select_kernel, dim3((uint32_t)groups), dim3(kSelectThreads), 0, stream, a);
