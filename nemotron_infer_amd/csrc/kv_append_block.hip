@@ -11,6 +11,14 @@
 // The largest value decides a scale, so k is rotated in 64 bits and rounded to float32 once (each product of
 // a bf16 and a float32 is exact there): equal inputs give equal scales however the rotation is computed.
 // NaN and infinities become NaN (e4m3 has no infinity) and do not count for the scale.
+//
+// Bound: bytes for prompts, latency at decode.  Prompts: a workgroup takes a block of a sequence's positions, or a part of
+// its heads, and forms the cosines of its 16 tokens once, in LDS; a wave takes a head's 16 vectors at a time, 8 lanes to
+// each, so that their largest value is a matter of its own lanes, and the block's earlier codes are at hand to move.  Decode:
+// a wave takes the token or some of its vectors, as in kv_append.hip, and each 8 lanes see to their vector's block.
+// Measured: 8191 tokens of 40 / 8 heads 51.2 us (4.6 TB/s read and written; a large copy: 4.9), 42.8 with outputs that stay in
+// the last-level cache; one token of 24 sequences 3.3 (graph replays).  With the first loads ahead of the look-up of
+// their place, or the next head's ahead of this one's stores, 46.4 and 44.6 where it takes 42.8.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 #include "nmi_packed.hpp"
@@ -22,6 +30,9 @@ namespace nmi {
 namespace {
 
 constexpr int kWaves = 4;
+// Times 8 query vectors of a wave on their way at once.  1 / 2 / 4 (inputs and outputs past the last-level cache, rotated, 40 / 8
+// heads): 8191 tokens 51.7 / 51.7 / 51.2 us, 8 prompts of 1000 50.7 / 50.4 / 50.0, 5 of up to 1801 24.4 / 23.7 / 23.5.
+constexpr int kAhead = 4;
 enum { kPlain = 0, kHalves = 1, kInterleaved = 2 };
 
 // The largest of m and the finite values' magnitudes, as bits.
@@ -326,20 +337,33 @@ __global__ __launch_bounds__(64 * kWaves) void kv_append_block_kernel(const Appe
         }
     }
     if (MODE == kPlain || !a.q) return;
-    // q: 8 vectors at a time, the heads of a token one after another
-    const int vectors = job.n * a.H;
-    for (int v0 = 8 * (part * kWaves + wave); v0 < vectors; v0 += 8 * parts * kWaves) {
-        const int v = v0 + (lane >> 3);
-        if (v >= vectors) continue;
-        const int tok = v / a.H, h = v - tok * a.H;
-        const uint16_t* src = a.q + (int64_t)(job.row + tok) * a.ldq + h * kPagedHead;
-        float x[8], y[8];
-        unpack8(load16(src + d.r0), x);
-        unpack8(load16(src + d.r1), y);
-        rotate<MODE, false>(x, y, &turns[tok][8 * sub], d.turns);
-        uint16_t* o = a.q_out + (int64_t)(job.row + tok) * a.ldqo + h * kPagedHead;
-        *reinterpret_cast<uint4*>(o + d.r0) = pack8(x);
-        *reinterpret_cast<uint4*>(o + d.r1) = pack8(y);
+    // q: 8 vectors at a time, the heads of a token one after another, kAhead times that on their way at once
+    const int vectors = job.n * a.H, stride = 8 * parts * kWaves;
+    for (int v0 = 8 * (part * kWaves + wave) + (lane >> 3); __builtin_amdgcn_ballot_w64(v0 < vectors); v0 += kAhead * stride) {
+        uint4 lo[kAhead], hi[kAhead];
+        int tok[kAhead], h[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int v = v0 + i * stride;
+            tok[i] = v / a.H;
+            h[i] = v - tok[i] * a.H;
+            if (v < vectors) {
+                const uint16_t* src = a.q + (int64_t)(job.row + tok[i]) * a.ldq + h[i] * kPagedHead;
+                lo[i] = load16(src + d.r0);
+                hi[i] = load16(src + d.r1);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (v0 + i * stride >= vectors) break;
+            float x[8], y[8];
+            unpack8(lo[i], x);
+            unpack8(hi[i], y);
+            rotate<MODE, false>(x, y, &turns[tok[i]][8 * sub], d.turns);
+            uint16_t* o = a.q_out + (int64_t)(job.row + tok[i]) * a.ldqo + h[i] * kPagedHead;
+            *reinterpret_cast<uint4*>(o + d.r0) = pack8(x);
+            *reinterpret_cast<uint4*>(o + d.r1) = pack8(y);
+        }
     }
 }
 
@@ -354,6 +378,8 @@ void launch(const AppendArgs& a, hipStream_t stream) {
                            dim3(64 * kWaves), 0, stream, a, parts);
         return;
     }
+    // A block's heads in as many parts as leave four workgroups to a CU (2 / 4 / 8 of them: 8191 tokens 51.5 / 51.2 / 52.5 us,
+    // 5 prompts of up to 1801 24.3 / 23.5 / 23.5, of 16 / 4 heads 10.8 / 11.1 / 12.5).
     const int64_t jobs = most_blocks(a.tokens, a.batch);
     const int most = (vectors + kWaves - 1) / kWaves;
     const int parts = (int)std::min<int64_t>(most, std::max<int64_t>(1, 4 * cus / jobs));
