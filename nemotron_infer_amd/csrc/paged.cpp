@@ -47,6 +47,7 @@ bool rows_ok(const void* p, int64_t ld, int heads) {
 
 // Workgroups along one axis of a launch, of 256 threads each: the axis has less than 2^32 threads.
 constexpr int64_t kMaxGroups256 = (1 << 24) - 1;
+constexpr int64_t kMaxGroups1024 = (1 << 22) - 1;       // of 1024 threads each
 
 // A cache descriptor as the kernels take it; 0 or an NMI_ERR_* with the message set.
 int check_cache(const char* fn, const nmi_paged_kv* c, PagedKv* out, BlockScales* blocks) {
@@ -326,7 +327,7 @@ int nmi_sdpa_decode_paged_sparse(const nmi_paged_kv* cache, const void* q_bf16, 
     if (const int rc = check_decode(fn, cache, q_bf16, ldq, o_bf16, ldo, kv_lens, batch, n_heads, scale, &a)) return rc;
     if (!k_bounds_bf16) return refuse(NMI_ERR_INVALID_ARG, "%s: NULL k_bounds", fn);
     if (n_select < 1) return refuse(NMI_ERR_INVALID_ARG, "%s: n_select=%d (need at least the newest page)", fn, n_select);
-    if ((int64_t)batch * a.kv.n_kv > kMaxGroups256)
+    if ((int64_t)batch * a.kv.n_kv > kMaxGroups1024)
         return refuse(NMI_ERR_INVALID_ARG, "%s: batch=%d n_kv_heads=%d are too many for one launch", fn, batch, a.kv.n_kv);
     if (!aligned(k_bounds_bf16, 16) || !aligned(selected, 4))
         return refuse(NMI_ERR_ALIGNMENT, "%s: k_bounds must be 16-byte aligned, selected 4-byte", fn);

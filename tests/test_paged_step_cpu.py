@@ -355,6 +355,12 @@ def test_sparse_decode_refuses(change, code):
     assert size(0, 40, 8, 4, 2) == size(1, 41, 8, 4, 2) == size(1, 40, 8, 0, 2) == size(1, 40, 8, 4, 0) == 0
 
 
+def test_sparse_decode_refuses_more_groups_than_a_launch_has():
+    """The choice has 1024 threads for each sequence's KV head, and a launch less than 2^32."""
+    assert _sparse(_cache(), batch=2 ** 19, ws_bytes=1 << 40) == BAD
+    assert "too many for one launch" in _lib.lib().nmi_last_error().decode()
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(bounds=0), BAD), (dict(start=0), BAD), (dict(batch=0), BAD), (dict(tokens=0), BAD), (dict(cu=0), BAD),
     (dict(tokens=2 ** 24), BAD), (dict(batch=2 ** 24, tokens=2 ** 24 - 1), BAD), (dict(bounds=FAKE + 8), ALIGN),
