@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const Selec
     };
     const int kept = min(s.pages, a.select);
     if (a.selected)
-        for (int i = kept + tid; i < a.select; i += kSelectThreads) a.selected[mine + i] = -1;
+        for (int64_t i = kept + tid; i < a.select; i += kSelectThreads) a.selected[mine + i] = -1;     // (up to 2^31 - 1)
     if (g == 0 && tid == 0 && a.out_lens)
         a.out_lens[b] = s.pages <= a.select ? s.len : s.len - ((s.pages - a.select) << a.kv.page_shift);
     if (s.pages <= a.select) {

@@ -599,6 +599,22 @@ def test_sparse_sizes(kind, page, lens, select):
     _check_sparse(np.random.default_rng(page), kind, lens, 4, 1, page, select, label=f"{kind} {page}", layout="heads")
 
 
+def test_sparse_selects_as_many_as_the_type_counts():
+    announce("sparse_most")
+    n = 2 ** 31 - 1
+    g = torch.Generator().manual_seed(74)
+    k, v = (torch.randn(4, 1, 16, 128, generator=g).bfloat16().to(DEV) for _ in range(2))
+    q = torch.randn(1, 128, generator=g).bfloat16().to(DEV)
+    table, lens = torch.tensor([[2, 0, 3]], dtype=torch.int32, device=DEV), torch.tensor([40], dtype=torch.int32, device=DEV)
+    bounds = torch.zeros(4, 1, 2, 128, dtype=torch.bfloat16, device=DEV)
+    places = torch.empty(n + 1, dtype=torch.int32, device=DEV).fill_(7)        # (one behind the last)
+    got = ops.sdpa_decode_paged_sparse(q, k, v, table, lens, bounds, n, selected=places[:n].view(1, 1, n))
+    few = ops.sdpa_decode_paged_sparse(q, k, v, table, lens, bounds, 3)
+    assert torch.equal(got, few)
+    assert places[:4].tolist() == [0, 1, 2, -1] and int(places[-1]) == 7
+    assert all(bool((part == -1).all()) for part in places[3:n].split(2 ** 28))
+
+
 @pytest.mark.parametrize("layout", ["tokens", "slice"])
 def test_sparse_layouts_and_scales(layout):
     announce("sparse_layout", layout)
