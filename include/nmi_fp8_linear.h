@@ -474,6 +474,7 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
  *   cu_seqlens [batch + 1]  packed offsets, max(new_lens, 0) rows each whether granted or not; NULL: one row per
  *                       sequence (tokens = batch, and more than one new token is out of range)
  *   slots [tokens]      of each row page * page_size + place, -1 where not granted and behind the last row
+ *                       (tokens may be 0 where the rows are packed: sequences end)
  *   free_count_out [1]  the stack's new height (may be free_count itself)
  * All int32 but slots (int64).  Out of range, and reported (NMI_ERR_ASYNC) by this entry's next call or another of the
  * paged ones: free_count outside [0, n_pages] (cut), a length that the row cannot hold (cut where it has ended, else not

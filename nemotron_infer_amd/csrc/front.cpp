@@ -9,7 +9,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
 
-#include <algorithm>
 #include <string>
 
 #include "nmi_fp8_linear.h"
@@ -450,16 +449,15 @@ PyObject* kv_assign_paged(PyObject* const* a) {
     on_gpu(lens);
     // One allocation for what is new, and tensors over parts of it made directly (a second allocation, and each of torch's
     // views, cost an eager call 1 us): slots, then start_pos, kv_lens, cu_seqlens, lens_out, free_count_out.
-    const int64_t slot_rows = std::max<int64_t>(tokens, 1);     // (the C entry takes a row at least)
     const int64_t n_ints = 3 * batch + (packed ? batch + 1 : 0) + 1;
-    const at::Tensor all = at::empty({slot_rows + (n_ints + 1) / 2}, lens.options().dtype(at::kLong));
+    const at::Tensor all = at::empty({tokens + (n_ints + 1) / 2}, lens.options().dtype(at::kLong));
     auto over = [&](at::ScalarType type, int64_t first, int64_t n) {
         auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
         t->set_storage_offset(first);
         t->set_sizes_contiguous({n});
         return at::Tensor(std::move(t));
     };
-    int64_t at = 2 * slot_rows;
+    int64_t at = 2 * tokens;
     auto part = [&](int64_t n) {
         at += n;
         return over(at::kInt, at - n, n);
@@ -473,7 +471,7 @@ PyObject* kv_assign_paged(PyObject* const* a) {
     {
         auto call = entry<decltype(&nmi_kv_assign_paged)>(a[2]);
         void* stream = stream_of(a[1]);
-        const int b = as_int(batch, "batch"), n = as_int(slot_rows, "tokens"), width = as_int(table.size(1), "max_pages");
+        const int b = as_int(batch, "batch"), n = as_int(tokens, "tokens"), width = as_int(table.size(1), "max_pages");
         const int n_pages = as_int(pages.size(0), "n_pages");
         int32_t* table_p = static_cast<int32_t*>(table.data_ptr());
         const int64_t stride = batch > 1 ? table.stride(0) : table.size(1);

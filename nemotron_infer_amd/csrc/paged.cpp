@@ -239,10 +239,10 @@ int nmi_kv_assign_paged(const int32_t* lens, const int32_t* new_lens, int32_t* p
                       "%s: n_pages=%d max_pages=%d page_table_stride=%lld page_size=%d (need all >= 1, page_table_stride >= "
                       "max_pages, at most 2^30 positions per sequence)",
                       fn, n_pages, max_pages, (long long)page_table_stride, page_size);
-    if (batch < 1 || batch > kMaxGroups256 || tokens < 1 || tokens > kMaxGroups256 || (!cu_seqlens && tokens != batch))
+    if (batch < 1 || batch > kMaxGroups256 || tokens < 0 || tokens > kMaxGroups256 || (!cu_seqlens && tokens != batch))
         return refuse(NMI_ERR_INVALID_ARG,
-                      "%s: batch=%d tokens=%d (need both >= 1 and less than 2^24, and as many tokens as sequences where "
-                      "cu_seqlens is NULL)",
+                      "%s: batch=%d tokens=%d (need batch >= 1, tokens >= 0, both less than 2^24, and as many tokens as "
+                      "sequences where cu_seqlens is NULL)",
                       fn, batch, tokens);
     if (!aligned(lens, 4) || !aligned(new_lens, 4) || !aligned(page_table, 4) || !aligned(free_pages, 4) ||
         !aligned(free_count, 4) || !aligned(start_pos, 4) || !aligned(kv_lens, 4) || !aligned(cu_seqlens, 4) ||

@@ -372,8 +372,8 @@ def test_bounds_refuse(change, code):
 @pytest.mark.parametrize("change,code", [
     *[(dict([(n, 0)]), BAD) for n in ("lens", "table", "free", "count", "start", "kv", "slots", "lens_out", "count_out")],
     (dict(page=8), BAD), (dict(page=24), BAD), (dict(page=1 << 21), BAD), (dict(stride=3), BAD), (dict(max_pages=0), BAD),
-    (dict(n_pages=0), BAD), (dict(max_pages=2 ** 26 + 1, stride=2 ** 27), BAD), (dict(batch=0), BAD), (dict(tokens=0), BAD),
-    (dict(cu=0), BAD), (dict(batch=2 ** 24), BAD), (dict(tokens=2 ** 24), BAD), (dict(slots=FAKE + 4), ALIGN),
+    (dict(n_pages=0), BAD), (dict(max_pages=2 ** 26 + 1, stride=2 ** 27), BAD), (dict(batch=0), BAD), (dict(tokens=-1), BAD),
+    (dict(tokens=0, cu=0), BAD), (dict(cu=0), BAD), (dict(batch=2 ** 24), BAD), (dict(tokens=2 ** 24), BAD), (dict(slots=FAKE + 4), ALIGN),
     *[(dict([(n, FAKE + 2)]), ALIGN) for n in ("lens", "new", "table", "free", "count", "start", "kv", "cu", "lens_out", "count_out")]])
 def test_assign_refuses(change, code):
     assert _assign(**change) == code and _lib.lib().nmi_last_error().decode().startswith("nmi_kv_assign_paged")

@@ -1048,6 +1048,26 @@ def test_two_streams_and_two_threads():
     assert int(servers[0].lens[0]) == 90
 
 
+def test_assign_grants_nothing_to_a_step_of_no_rows():
+    """Sequences end; one that asks for a token all the same is out of range."""
+    announce("assign_no_rows")
+
+    def ints(*v):
+        return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+    table, free, count = torch.tensor([[0, 1], [2, 9], [3, 9]], dtype=torch.int32, device=DEV), ints(4, 5, 6, 7, 8, 8, 8, 8), ints(2)
+    got = ops.kv_assign_paged(ints(20, 16, 3), ints(-1, 0, 0), table, free, count, 16, tokens=0)
+    assert [t.tolist() for t in got] == [[-1] * 3, [0] * 3, [0] * 4, [], [-1, 16, 3], [4]]
+    assert free.tolist() == [4, 5, 0, 1, 8, 8, 8, 8]
+    torch.cuda.synchronize()
+    got = ops.kv_assign_paged(ints(-1, 16, 3), ints(0, 1, 0), table, free, ints(4), 16, tokens=0)
+    assert [t.tolist() for t in got] == [[-1] * 3, [0] * 3, [0] * 4, [], [-1, 16, 3], [4]]
+    assert table.tolist() == [[0, 1], [2, 9], [3, 9]]
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.NmiError):
+        ops.kv_assign_paged(ints(-1), ints(0), table[:1], free, ints(4), 16, tokens=0)
+
+
 def test_the_front_end_keeps_nothing():
     announce("step_front")
     s = Server("block")
