@@ -10,18 +10,23 @@
 // sdpa_decode_paged.hip then goes through; the newest one is last, so that a length says where they end.
 //
 // Which pages are chosen must not hang on the order of a sum: scores are summed in 64 bits (the products are exact
-// there) and rounded to float32 once.  Twice a term is q (hi + lo) + |q| (hi - lo), the sum and the difference exact in 64
-// bits for what bf16 holds unless they lie 2^45 apart: two multiply-adds, the magnitude for nothing.
-// (Float32 sums instead took 1 us of 20 less for one sequence of 100001 positions, 2 of 43 for 20 documents.)
+// there) and rounded to float32 once.  Each dim adds both its products, of which one is 0: what the query does not use
+// takes no bits of the sum, however large it is (and 0 times an infinity is NaN).  (Float32 sums instead, in an earlier
+// form, took 1 us of 20 less for one sequence of 100001 positions, 2 of 43 for 20 documents.)
 //
 // Scores.  Bound: the 64-bit arithmetic of many pages, latency of few (length and page id, then bounds and queries).  16
-// lanes take a page, 8 dims each, the queries in their registers; a wave takes 4 pages at a time, the next ones' bounds
-// on their way, all of the chunk's query heads at once so that their sums hide one another's latency (one head after another,
-// 40 sequences of 4000: 39.0 us for the whole call, so 36.7; 16 pages a wave, 4 lanes each, the queries in LDS: 36.8, but one
-// sequence of 60000 18.6 where this takes 17.0).  A sequence's KV head is dealt to as many workgroups as all of them leave it
-// of 8 per CU: 1 / 2 / 4 / 8 / 16 per CU, 20 documents of 900 to 30000 positions (pages of 32, 32 / 8 heads; the whole
-// call, an earlier form) 113 / 62 / 50 / 44.0 / 44.4 us; the pages of all sequences in equal shares 43.4 where that took
-// 43.1, and one sequence 21.0 where that took 20.6.
+// lanes take a page, 8 dims each, the queries' positive and negative parts in their registers; a wave takes 4 pages at a
+// time, all of the chunk's query heads at once so that their sums hide one another's latency, and asks for the next pages'
+// bounds as those at hand are used: their upper ones first, so that both need not be held at once (4 heads: 166
+// registers, 3 waves to a SIMD, where 178 leave 2: 8 sequences of 60000 33.0 us for the whole call, so 30.6).  (One head after
+// another, in an earlier form, 40 sequences of 4000: 39.0 where that took 36.7; 16 pages a wave, 4 lanes each, the queries
+// in LDS: 36.8, but one sequence of 60000 18.6 where that took 17.0.)
+// A sequence's KV head is dealt to as many workgroups as all of them leave it of 6 per CU, or 2 where there is but one
+// sequence, whose workgroups all have as much to do: 2 / 3 / 4 / 6 / 8 / 12 per CU, 40 / 8 heads, the whole call, one sequence
+// of 100001 positions 18.5 / 19.4 / 19.6 / 19.5 / 19.7 / 19.7 us, 40 of 4000 39.1 / 38.2 / 38.6 / 38.8 / 41.2 / 42.1, 20
+// documents of 900 to 30000 46.7 / 40.0 / 39.2 / 39.8 / 39.9 / 41.4; 16 / 16 heads 17.6 / 17.6 / 17.8 / 18.0 / 18.0 / 18.0,
+// 52.5 / 52.8 / 52.7 / 52.4 / 53.0 / 52.7 and 70.3 / 57.3 / 54.6 / 52.4 / 51.2 / 50.8.  (The pages of all sequences in equal shares, an
+// earlier form: 20 documents 43.4 where that took 43.1, and one sequence 21.0 where that took 20.6.)
 // Choice: one workgroup for a sequence's KV head: the range of the scores cut into 1024 bins, counted in LDS, the bin
 // with the last one wanted cut again while it has many, its few ranked one against another; then one pass in order.
 // Bound: latency, a handful of barriers: 4.6 us (traced) of 1562 pages, where four passes of 8 bits and a scan for each
@@ -37,7 +42,8 @@ namespace nmi {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kHeads = 5;               // query heads at a time at most: 16 registers each
+constexpr int kHeads = 5;               // query heads at a time at most: 32 registers each
+constexpr int kPerCu = 6, kPerCuOne = 2;    // scores' workgroups per CU; of one sequence
 constexpr int kBinBits = 10, kSelectThreads = 1 << kBinBits, kSelectWaves = kSelectThreads / 64;
 constexpr int kKeys = 6144;             // keys and page ids of a sequence kept in LDS
 constexpr int kFew = 64;                // keys ranked by a wave
@@ -88,69 +94,66 @@ __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a
     const int32_t* row = a.kv.page_table + b * a.kv.table_stride;
     const int first = (part * kWaves + wave) * 4 + (lane >> 4), stride = parts * kWaves * 4;
     // (entries of the table's row, whatever they hold, asked for beside the length)
-    auto page_id = [&](int64_t p) { return row[min(p, (int64_t)a.kv.max_pages - 1)]; };
-    int32_t first_id[2] = {page_id(first), page_id((int64_t)first + stride)};
+    auto page_id = [&](int p) { return row[min(p, a.kv.max_pages - 1)]; };
+    int32_t id = page_id(first), id_after = page_id(first + stride);
     const Sequence s = sequence(a, b);
     const int n = s.pages - 1;
     if (s.pages <= a.select || (part * kWaves + wave) * 4 >= n) return;
-    struct Bounds {
-        uint4 lo, hi;
-        bool bad;
+    auto at = [&](int32_t id, bool* bad) {
+        *bad = false;
+        const int page = checked_page(id, a.kv.n_pages, bad);
+        return a.bounds + (((int64_t)page * a.kv.n_kv + g) * 2) * kPagedHead + 8 * sub;
     };
-    auto load = [&](int32_t id) {
-        Bounds x;
-        x.bad = false;
-        const int page = checked_page(id, a.kv.n_pages, &x.bad);
-        const uint16_t* p = a.bounds + (((int64_t)page * a.kv.n_kv + g) * 2) * kPagedHead + 8 * sub;
-        x.lo = load16(p);
-        x.hi = load16(p + kPagedHead);
-        return x;
+    // 8 dims' products with one bound
+    auto add = [](uint4 v, const double (&q)[HEADS][8], double (&sum)[HEADS]) {
+        float x[8];
+        unpack8(v, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double y = x[i];
+#pragma unroll
+            for (int h = 0; h < HEADS; ++h) sum[h] = __builtin_fma(q[h][i], y, sum[h]);
+        }
     };
     float* scores = a.scores + ((int64_t)b * a.kv.n_kv + g) * a.kv.max_pages;
     for (int h0 = 0; h0 < a.group; h0 += HEADS) {
         // a page's bounds are on their way while those before are used, and the id of the next one's
-        Bounds next = load(first_id[0]);
-        int32_t id = first_id[1];
-        double q[HEADS][8];
+        bool bad;
+        const uint16_t* bounds = at(id, &bad);
+        uint4 lo = load16(bounds), hi = load16(bounds + kPagedHead);
+        id = id_after;
+        double above[HEADS][8], below[HEADS][8];        // max(q, 0) and min(q, 0); NaN in both
 #pragma unroll
         for (int h = 0; h < HEADS; ++h) {
             float x[8];
             unpack8(load16(a.q + (int64_t)b * a.ldq + (int64_t)(g * a.group + min(h0 + h, a.group - 1)) * kPagedHead + 8 * sub), x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[h][i] = x[i];
-        }
-        for (int64_t p = first; __builtin_amdgcn_ballot_w64(p < n); p += stride) {      // (all lanes, for the sums over them)
-            const Bounds now = next;
-            next = load(id);
-            id = page_id(p + 2 * stride);
-            float lo[8], hi[8];
-            unpack8(now.lo, lo);
-            unpack8(now.hi, hi);
-            double sum_of[8], span[8];
-#pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sum_of[i] = (double)hi[i] + (double)lo[i];
-                span[i] = (double)hi[i] - (double)lo[i];
+                above[h][i] = __builtin_elementwise_maximum(x[i], 0.f);
+                below[h][i] = __builtin_elementwise_minimum(x[i], 0.f);
             }
+        }
+        for (int p = first; __builtin_amdgcn_ballot_w64(p < n); p += stride) {      // (all lanes, for the sums over them)
+            const bool was_bad = bad;
+            bounds = at(id, &bad);
+            id = page_id(p + 2 * stride);
             double sum[HEADS];
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) {
-                sum[h] = 0.0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum[h] = __builtin_fma(q[h][i], sum_of[i], sum[h]);
-                    sum[h] = __builtin_fma(__builtin_fabs(q[h][i]), span[i], sum[h]);
-                }
-            }
+            for (int h = 0; h < HEADS; ++h) sum[h] = 0.0;
+            add(hi, above, sum);
+            hi = load16(bounds + kPagedHead);
+            add(lo, below, sum);
+            lo = load16(bounds);
             row_sums16_f64(sum);
             float best = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < HEADS; ++h) best = __builtin_elementwise_maximum(best, (float)(0.5 * sum[h]));      // (NaN stays)
+            for (int h = 0; h < HEADS; ++h) best = __builtin_elementwise_maximum(best, (float)sum[h]);      // (NaN stays)
             if (sub == 0 && p < n) {
                 if (h0) best = __builtin_elementwise_maximum(best, scores[p]);
-                scores[p] = now.bad ? NAN : best;       // (a bad page is the attention's to report)
+                scores[p] = was_bad ? NAN : best;       // (a bad page is the attention's to report)
             }
         }
+        if (h0 + HEADS < a.group) id = page_id(first), id_after = page_id(first + stride);
     }
 }
 
@@ -286,7 +289,8 @@ hipError_t launch_page_select(const SelectArgs& a, hipStream_t stream) {
     const int64_t groups = (int64_t)a.batch * a.kv.n_kv;
     if (a.select < a.kv.max_pages) {
         // as many workgroups as keep the CUs busy, or one for each 16 pages that a sequence may have
-        const int64_t most = ((int64_t)a.kv.max_pages + 15) / 16, parts = std::max<int64_t>(1, 8 * device_info().num_cu / groups);
+        const int per_cu = a.batch == 1 ? kPerCuOne : kPerCu;
+        const int64_t most = ((int64_t)a.kv.max_pages + 15) / 16, parts = std::max<int64_t>(1, per_cu * device_info().num_cu / groups);
         const int p = (int)std::min(most, parts);
         const int chunks = (a.group + kHeads - 1) / kHeads;
         const dim3 grid((uint32_t)(groups * p)), block(kThreads);

@@ -1,0 +1,77 @@
+"""GPU tests of a serving step on a paged cache where it is easiest to get wrong: page scores that only one side of a
+bound enters.
+
+Bars (derived before the first run): selected places are whole numbers, equal to those of the oracle, whose scores are
+sums in 64 bits rounded to float32 once as the kernel's are; in another order, so that two scores may change places only if
+they lie within 128 * 2^-53 of the sum of their terms' magnitudes of one another, which random ordinary terms do not.
+"""
+import numpy as np
+import pytest
+import torch
+
+from nemotron_infer_amd import _lib, ops
+from oracle import block, paged
+from tests.gpu_util import DEV, announce, assert_parity, bits
+from tests.test_paged_gpu import Pool, _dev, _f64, _rand_bits
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_pending_error():
+    _lib.lib().nmi_async_status()
+    yield
+    torch.cuda.synchronize()
+    _lib.lib().nmi_async_status()
+
+
+def _selected(pool, q, bounds, select):
+    """(o, places) of one call."""
+    places = torch.full((len(pool.lens), pool.k.shape[1], select), -7, dtype=torch.int32, device=DEV)
+    o = ops.sdpa_decode_paged_sparse(_dev(q), pool.dk, pool.dv, pool.dtable, _dev(pool.lens), _dev(bounds), select, selected=places)
+    torch.cuda.synchronize()
+    assert _lib.lib().nmi_async_status() == 0
+    return o, places.cpu().numpy()
+
+
+LARGEST = (2.0 - 2.0 ** -7) * 2.0 ** 127
+
+
+@pytest.mark.parametrize("far", [2.0 ** 20, 2.0 ** 36, 2.0 ** 50, 2.0 ** 60, 2.0 ** 100, LARGEST])
+@pytest.mark.parametrize("H,n_kv", [(1, 1), (2, 1), (8, 2), (5, 1), (7, 1)])
+def test_scores_take_nothing_from_the_side_that_no_query_uses(far, H, n_kv):
+    """A dim whose queries are all negative and whose largest key is far out, another the other way round: the score is the
+    other dims' and the near side's."""
+    announce("sparse_one_sided", far, H, n_kv)
+    rng = np.random.default_rng(H)
+    pool = Pool(rng, [1500, 700], n_kv, 16, "bf16")
+    q = _f64(_rand_bits(rng, 2, H * 128)).reshape(2, H, 128)
+    q[:, :, 40], q[:, :, 77] = -np.abs(q[:, :, 40]), np.abs(q[:, :, 77])
+    x = np.sort(rng.standard_normal((pool.k.shape[0], n_kv, 2, 128)), axis=2)
+    some = rng.random((pool.k.shape[0], n_kv)) < 0.7
+    x[..., 1, 40] = np.where(some, far, x[..., 1, 40])
+    x[..., 0, 77] = np.where(~some, -far, x[..., 0, 77])
+    q, bounds = block.bf16_round_exact(q), block.bf16_round_exact(x)
+    o, places = _selected(pool, q.reshape(2, -1), bounds, 12)
+    kept = [paged.select(_f64(q[b]), _f64(bounds), pool.table[b], int(n), 16, 12) for b, n in enumerate(pool.lens)]
+    assert np.array_equal(places, kept)
+    want = paged.decode_selected(_f64(q), *pool.values(), pool.table, pool.lens, kept)
+    assert_parity(bits(o).reshape(want.shape), block.bf16_round_exact(want), f"{far}", per_row_scales=True)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_an_infinite_query_scores_infinities(sign):
+    """+inf * hi where hi > 0 is the largest score, where hi < 0 the smallest, whatever lo is (0 * lo = 0); so with the signs
+    turned."""
+    announce("sparse_infinite", sign)
+    rng = np.random.default_rng(5)
+    pool = Pool(rng, [640], 1, 16, "bf16")
+    q = _f64(_rand_bits(rng, 1, 128))
+    q[0, 9] = sign * np.inf
+    x = np.sort(rng.standard_normal((pool.k.shape[0], 1, 2, 128)), axis=2)
+    first = [3, 11, 12, 38]
+    used, other = (1, 0) if sign > 0 else (0, 1)
+    x[:, 0, used, 9], x[:, 0, other, 9] = -sign, -4.0 * sign if sign > 0 else 4.0
+    x[pool.table[0, first], 0, used, 9] = sign
+    _, places = _selected(pool, block.bf16_round_exact(q), block.bf16_round_exact(x), 5)
+    assert places.tolist() == [[first + [39]]]
