@@ -479,7 +479,7 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
  * All int32 but slots (int64).  Out of range, and reported (NMI_ERR_ASYNC) by this entry's next call or another of the
  * paged ones: free_count outside [0, n_pages] (cut), a length that the row cannot hold (cut where it has ended, else not
  * granted), page ids outside [0, n_pages) where they are met (moved as they are; slot -1), more pages pushed than the
- * stack holds (dropped), rows past `tokens` (cut, and not granted).  Outputs overlap each other and the inputs in no
+ * stack holds (dropped unread), rows past `tokens` (cut, and not granted).  Outputs overlap each other and the inputs in no
  * other way.  One launch, two for more than 6144 packed rows; no workspace.
  */
 int nmi_kv_assign_paged(const int32_t* lens, const int32_t* new_lens, int32_t* page_table, int64_t page_table_stride,

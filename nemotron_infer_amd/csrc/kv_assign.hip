@@ -116,14 +116,15 @@ __global__ __launch_bounds__(THREADS) void kv_assign_kernel(const AssignArgs a) 
                 upto[tid] = back[0];
                 base[tid] = (int32_t)mine;
                 __syncthreads();
-                for (uint32_t e = tid; e < total[0]; e += THREADS) {
+                const uint32_t stop = pages_back(total[0], count, a.n_pages, &bad);
+                for (uint32_t e = tid; e < stop; e += THREADS) {
                     const int i = G::search(upto, n, e);
                     const uint32_t j = e - (upto[i] - (uint32_t)base[i]);
                     const int id = a.table[(int64_t)(b0 + i) * a.table_stride + j];
-                    if (id < 0 || id >= a.n_pages || (int64_t)count + e >= a.n_pages) bad = true;
-                    if ((int64_t)count + e < a.n_pages) a.free_pages[count + e] = id;
+                    if (id < 0 || id >= a.n_pages) bad = true;
+                    a.free_pages[count + e] = id;
                 }
-                count = (int)min((int64_t)count + total[0], (int64_t)a.n_pages);
+                count += (int)stop;
             }
             __syncthreads();
         }

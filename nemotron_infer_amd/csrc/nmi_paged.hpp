@@ -115,6 +115,14 @@ NMI_HD int later_span(int c0, int c1, int tokens, int before, int* first, int* p
     return n;
 }
 
+// Of `total` pages that come back to a stack of n_pages, `count` of them there, those that it has room for (*bad where
+// there are more, which are not looked at): whatever the lengths claim, less than 2^31.
+NMI_HD uint32_t pages_back(uint32_t total, int count, int n_pages, bool* bad) {
+    const uint32_t room = (uint32_t)(n_pages - count);
+    if (total > room) *bad = true;
+    return total < room ? total : room;
+}
+
 // Blocks of kPagedBlock positions that n positions from `pos` on lie in.
 NMI_HD int blocks_of(int64_t pos, int n) { return n > 0 ? (int)(((pos & (kPagedBlock - 1)) + n + kPagedBlock - 1) / kPagedBlock) : 0; }
 // At most so many of `tokens` rows in `batch` sequences: each has 30 positions at most that are not its own in its blocks.

@@ -1,5 +1,5 @@
 """GPU tests of a serving step on a paged cache where it is easiest to get wrong: page scores that only one side of a
-bound enters.
+bound enters, more pages coming back than there are.
 
 Bars (derived before the first run): selected places are whole numbers, equal to those of the oracle, whose scores are
 sums in 64 bits rounded to float32 once as the kernel's are; in another order, so that two scores may change places only if
@@ -75,3 +75,22 @@ def test_an_infinite_query_scores_infinities(sign):
     x[pool.table[0, first], 0, used, 9] = sign
     _, places = _selected(pool, block.bf16_round_exact(q), block.bf16_round_exact(x), 5)
     assert places.tolist() == [[first + [39]]]
+
+
+@pytest.mark.parametrize("batch,width,page", [(40, 1024, 1 << 20), (300, 3000, 16)])
+def test_pages_past_the_stack_are_neither_pushed_nor_read(batch, width, page):
+    """Ended sequences whose lengths claim many times the pool's pages: the stack is filled in the sequences' order, the rest
+    dropped, and reported once; ids behind those that fit, out of range here, are not met."""
+    announce("assign_claims", batch, width, page)
+    n_pages, count = 50, 20
+    table = torch.full((batch, width), -9, dtype=torch.int32, device=DEV)
+    table[0, :30] = torch.arange(20, 50)
+    lens = torch.full((batch,), width * page, dtype=torch.int32, device=DEV)
+    free = torch.arange(n_pages, dtype=torch.int32, device=DEV)
+    free[count:] = -5
+    new = torch.full((batch,), -1, dtype=torch.int32, device=DEV)
+    got = ops.kv_assign_paged(lens, new, table, free, torch.tensor([count], dtype=torch.int32, device=DEV), page, tokens=0)
+    torch.cuda.synchronize()
+    assert _lib.lib().nmi_async_status() == _lib.NMI_ERR_ASYNC and _lib.lib().nmi_async_status() == 0
+    assert got.free_count.tolist() == [n_pages] and free.tolist() == list(range(n_pages))
+    assert (got.lens == -1).all() and (got.start_pos == -1).all() and (table[:, 30:] == -9).all()
