@@ -531,7 +531,8 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
  * them.  Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds are not
  * read.  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places in the sequence of the pages
  * attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type; scale does not change the
- * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first.
+ * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first (with
+ * n_select 1 none is scored).
  * workspace: nmi_sdpa_decode_paged_sparse_workspace_bytes(batch, n_heads, n_kv_heads, max_pages, n_select) bytes,
  * 16-byte aligned, no initialisation; NULL takes it from the bump allocator.  Four launches; three where n_select pages
  * hold as few positions as above; the decode's alone where n_select >= max_pages.

@@ -88,6 +88,7 @@ __device__ __forceinline__ void row_sums16_f64(double (&v)[N]) {
 // there are fewer: their scores are the same).
 template <int HEADS>
 __global__ __launch_bounds__(kThreads) void page_score_kernel(const SelectArgs a, int parts) {
+    if (a.select == 1) return;                          // (the newest page, whatever the scores)
     const int part = blockIdx.x % parts, g = (int)(blockIdx.x / parts % a.kv.n_kv), b = (int)(blockIdx.x / parts / a.kv.n_kv);
     const int lane = threadIdx.x & 63, sub = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

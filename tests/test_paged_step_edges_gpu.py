@@ -1,10 +1,12 @@
 """GPU tests of a serving step on a paged cache where it is easiest to get wrong: page scores that only one side of a
-bound enters, more pages coming back than there are.
+bound enters, a choice of one page, more pages coming back than there are.
 
 Bars (derived before the first run): selected places are whole numbers, equal to those of the oracle, whose scores are
 sums in 64 bits rounded to float32 once as the kernel's are; in another order, so that two scores may change places only if
 they lie within 128 * 2^-53 of the sum of their terms' magnitudes of one another, which random ordinary terms do not.
 """
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -75,6 +77,36 @@ def test_an_infinite_query_scores_infinities(sign):
     x[pool.table[0, first], 0, used, 9] = sign
     _, places = _selected(pool, block.bf16_round_exact(q), block.bf16_round_exact(x), 5)
     assert places.tolist() == [[first + [39]]]
+
+
+def test_the_newest_page_alone_needs_no_scores():
+    """n_select 1: places of pages that nothing could score are left as they were, page ids out of range there are not
+    met, and the newest page is attended."""
+    announce("sparse_newest")
+    rng = np.random.default_rng(6)
+    lens = [777, 3000, 16, 0]
+    pool = Pool(rng, lens, 2, 16, "bf16")
+    q, bounds = _rand_bits(rng, 4, 8 * 128), _rand_bits(rng, pool.k.shape[0], 2, 2, 128)
+    pool.table[0, 5], pool.table[1, 0] = -1, pool.k.shape[0]
+    width, L = pool.table.shape[1], _lib.lib()
+    dk, dv, dtable, dlens, dq, dbounds = pool.dk, pool.dv, _dev(pool.table), _dev(pool.lens), _dev(q), _dev(bounds)
+    c = _lib.PagedKv(dk.data_ptr(), dv.data_ptr(), 2 * 16 * 128, 16 * 128, 128, dtable.data_ptr(), width, None, None, 0,
+                     dk.shape[0], 16, width, 2)
+    ws = torch.full((L.nmi_sdpa_decode_paged_sparse_workspace_bytes(4, 8, 2, width, 1),), 0x5A, dtype=torch.uint8, device=DEV)
+    o = torch.empty(4, 8 * 128, dtype=torch.bfloat16, device=DEV)
+    places = torch.empty(4, 2, 1, dtype=torch.int32, device=DEV)
+    rc = L.nmi_sdpa_decode_paged_sparse(ctypes.addressof(c), dq.data_ptr(), 8 * 128, o.data_ptr(), 8 * 128, dlens.data_ptr(),
+                                        dbounds.data_ptr(), 1, places.data_ptr(), 4, 8, 128 ** -0.5, ws.data_ptr(), ws.numel(),
+                                        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, L.nmi_last_error()
+    torch.cuda.synchronize()
+    assert L.nmi_async_status() == 0
+    assert places.tolist() == [[[48]] * 2, [[187]] * 2, [[0]] * 2, [[-1]] * 2]
+    assert (ws[:4 * 2 * width * 4] == 0x5A).all()                                 # (the scores)
+    kept = [[[48]] * 2, [[187]] * 2, [[0]] * 2, [[]] * 2]
+    want = paged.decode_selected(_f64(q).reshape(4, 8, 128), *pool.values(), pool.table, pool.lens, kept)
+    assert_parity(bits(o)[:3].reshape(3, 8, 128), block.bf16_round_exact(want[:3]), "newest", per_row_scales=True)
+    assert not bits(o)[3].any()
 
 
 @pytest.mark.parametrize("batch,width,page", [(40, 1024, 1 << 20), (300, 3000, 16)])
