@@ -440,7 +440,9 @@ PyObject* kv_assign_paged(PyObject* const* a) {
     const int page_size = as_int(whole(a[8], "page_size"), "page_size");
     const bool packed = a[9] != Py_None;
     const int64_t tokens = packed ? whole(a[9], "tokens") : batch;
-    if (tokens < 0) bad_value("tokens=" + num(tokens) + " is out of range");
+    // (before anything of that size is asked for)
+    const int b = as_int(batch, "batch"), n = as_int(tokens, "tokens"), width = as_int(table.size(1), "max_pages");
+    const int n_pages = as_int(pages.size(0), "n_pages");
     int32_t* lens_out = vector<int32_t>(a[10], batch, at::kInt, "lens_out", dev);
     int32_t* count_out = vector<int32_t>(a[11], 1, at::kInt, "free_count_out", dev);
     if (!batch) bad_value("lens of no sequences");
@@ -471,8 +473,6 @@ PyObject* kv_assign_paged(PyObject* const* a) {
     {
         auto call = entry<decltype(&nmi_kv_assign_paged)>(a[2]);
         void* stream = stream_of(a[1]);
-        const int b = as_int(batch, "batch"), n = as_int(tokens, "tokens"), width = as_int(table.size(1), "max_pages");
-        const int n_pages = as_int(pages.size(0), "n_pages");
         int32_t* table_p = static_cast<int32_t*>(table.data_ptr());
         const int64_t stride = batch > 1 ? table.stride(0) : table.size(1);
         int32_t *start_p = static_cast<int32_t*>(start.data_ptr()), *kv_p = static_cast<int32_t*>(kv.data_ptr());

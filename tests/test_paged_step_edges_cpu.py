@@ -1,11 +1,12 @@
 """A serving step on a paged cache without a GPU, where it is easiest to get wrong: loops whose ends come from lengths in
-device memory."""
+device memory, counts past a type's range."""
 import ctypes
 import subprocess
 
 import pytest
+import torch
 
-from nemotron_infer_amd import build
+from nemotron_infer_amd import build, ops
 
 SHIM = """
 #include "nmi_paged.hpp"
@@ -38,3 +39,13 @@ def test_pages_that_come_back_end_with_the_room_for_them(hpp):
                 got = hpp.back(total, count, n_pages, ctypes.byref(bad))
                 assert got == min(total, n_pages - count) and bool(bad.value) == (total > n_pages - count)
                 assert got + 1024 < 2 ** 32 and count + got <= n_pages
+
+
+@pytest.mark.parametrize("tokens", [2 ** 31, 2 ** 40, 2 ** 62, 2 ** 63 - 1, -1])
+def test_front_end_refuses_rows_past_the_type_before_it_asks_for_memory(tokens):
+    """As a count out of range, not as memory that cannot be had."""
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match=f"tokens={tokens} is out of range"):
+        ops.kv_assign_paged(ints(3), ints(3), ints(3, 4), ints(9), ints(1), 16, tokens=tokens)
+    with pytest.raises((ValueError, TypeError), match="tokens"):
+        ops.kv_assign_paged(ints(3), ints(3), ints(3, 4), ints(9), ints(1), 16, tokens=2 ** 64)
