@@ -527,8 +527,10 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
  * The same over the pages of each sequence that a score selects, for each query token and KV head: of P pages all where
  * P <= n_select, else the newest one and the n_select - 1 of the others with the largest
  *   score[p] = max over the KV head's query heads h of f32( sum_d max(q_hd, 0) hi_d + min(q_hd, 0) lo_d ),
- * lo and hi page p's k_bounds (nmi_kv_bounds_paged): the largest product that a key of the page can have with one of
- * them.  Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds are not
+ * lo and hi page p's k_bounds (nmi_kv_bounds_paged): no key of the page has a larger product with one of them, as far as
+ * the bounds are exact.  They are of a bf16 cache and of codes under scales that are powers of two from 2^-124 to 2^119
+ * (bf16 holds those keys); under others a bound's rounding to bf16 may leave it short of the key by 2^-8 of its value.
+ * Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds are not
  * read.  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places in the sequence of the pages
  * attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type; scale does not change the
  * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first (with

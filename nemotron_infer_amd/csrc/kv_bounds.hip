@@ -2,8 +2,9 @@
 //
 //   bounds[page, head, 0, d] = min over the page's positions of k[d],  bounds[page, head, 1, d] = max,
 //
-// of the keys that the page stands for (codes times their scales in float32), rounded to bf16, for every page
-// that the call's new positions complete; a dim with a NaN has NaN for both.  The newest page of a sequence
+// of the keys that the page stands for (codes times their scales in float32), rounded to the nearest bf16, for every page
+// that the call's new positions complete; a dim with a NaN has NaN for both.  bf16 keys, and codes (4 significant bits)
+// under powers of two, lose nothing by it; under other scales a bound may lie 2^-8 of its value inside the keys.  The newest page of a sequence
 // needs none: it is attended whatever its score.
 //
 // Bound: latency (offsets, page id, keys one after another), then reading the pages, once.  A wave's load is one row of

@@ -4,9 +4,10 @@
 //
 //   score = max over the query heads h of the KV head of  sum_d max(q_hd, 0) hi_d + min(q_hd, 0) lo_d,
 //
-// lo, hi the page's bounds (kv_bounds.hip): no key of the page has a larger product with any of these heads.  Ties
-// go to the earlier page, NaN comes first (a page that holds one is attended, as the attention over all would).
-// The chosen ones, in their order, are a page table of their own for each KV head, which the attention of
+// lo, hi the page's bounds (kv_bounds.hip): no key of the page has a larger product with any of these heads, but for what
+// the bounds' rounding to bf16 takes (nothing of bf16 keys and of codes under powers of two).  Ties go to the earlier
+// page, NaN comes first (a page that holds one is attended, as the attention over all would).  The chosen ones, in their
+// order, are a page table of their own for each KV head, which the attention of
 // sdpa_decode_paged.hip then goes through; the newest one is last, so that a length says where they end.
 //
 // Which pages are chosen must not hang on the order of a sum: scores are summed in 64 bits (the products are exact

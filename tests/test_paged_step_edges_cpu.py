@@ -1,12 +1,14 @@
 """A serving step on a paged cache without a GPU, where it is easiest to get wrong: loops whose ends come from lengths in
-device memory, counts past a type's range."""
+device memory, counts past a type's range, what rounded bounds promise."""
 import ctypes
 import subprocess
 
+import numpy as np
 import pytest
 import torch
 
 from nemotron_infer_amd import build, ops
+from oracle import block, e4m3, paged
 
 SHIM = """
 #include "nmi_paged.hpp"
@@ -49,3 +51,38 @@ def test_front_end_refuses_rows_past_the_type_before_it_asks_for_memory(tokens):
         ops.kv_assign_paged(ints(3), ints(3), ints(3, 4), ints(9), ints(1), 16, tokens=tokens)
     with pytest.raises((ValueError, TypeError), match="tokens"):
         ops.kv_assign_paged(ints(3), ints(3), ints(3, 4), ints(9), ints(1), 16, tokens=2 ** 64)
+
+
+def _stored_bounds(keys):
+    """As the operator stores them: of float32 keys, rounded to the nearest bf16."""
+    bits = block.bf16_round_exact(paged.page_bounds(keys.astype(np.float32).astype(np.float64)))
+    return (bits.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+
+
+def test_bounds_as_they_are_stored_bound_the_keys():
+    """Of bf16 keys, and of codes under powers of two from 2^-124 to 2^119, the stored bounds are the keys' own, so that no
+    key's product passes the score; under other scales they may lie 2^-8 of their value inside."""
+    rng = np.random.default_rng(8)
+    lut = e4m3.decode_lut()
+    codes = lut[np.isfinite(lut)][rng.integers(0, 254, (6, 2, 32, 128))]
+    bf16 = rng.integers(0, 0x7F80, (6, 2, 32, 128)) | rng.integers(0, 2, (6, 2, 32, 128)) << 15
+    exact = [(bf16.astype(np.uint32) << 16).view(np.float32).astype(np.float64)]
+    exact += [codes * 2.0 ** e for e in (-124, -60, -7, 0, 5, 60, 119)]
+    for keys in exact:
+        bounds = _stored_bounds(keys)
+        assert np.array_equal(bounds, paged.page_bounds(keys))
+    q = rng.standard_normal((2, 128))
+    short = 0
+    for scale in (0.01, 0.0371, 1.7, 2.0 ** -7 * 1.001):
+        keys = (codes.astype(np.float32) * np.float32(scale)).astype(np.float64)
+        bounds = _stored_bounds(keys)
+        lo, hi = bounds[:, :, 0], bounds[:, :, 1]
+        true = paged.page_bounds(keys)
+        assert (np.abs(bounds - true) <= 2.0 ** -8 * np.abs(true)).all()
+        short += int((hi < true[:, :, 1]).sum() + (lo > true[:, :, 0]).sum())
+        for g in range(2):
+            up, down = np.maximum(q[g], 0), np.minimum(q[g], 0)
+            score = (hi[:, g] * up + lo[:, g] * down).sum(-1)
+            slack = 2.0 ** -8 * (np.abs(true[:, g, 1]) * up - np.abs(true[:, g, 0]) * down).sum(-1)
+            assert ((keys[:, g] @ q[g]).max(-1) <= score + slack + 1e-9 * np.abs(score)).all()
+    assert short > 100                                   # (they do lie inside: the bound is no bound there)
