@@ -467,6 +467,11 @@ int nmi_kv_append_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t l
  * they do not fit its row of the table, or if it needs pages and those needed up to it, by all that fit, are more than
  * the stack holds.  What is not granted leaves the sequence as it was, for the caller to see (start_pos -1 in spite of
  * new tokens); it is no error.
+ * Every page has one owner: a page in use or on the stack occurs there once, which is not checked.  A page that two
+ * sequences in use hold (a shared prefix) would be handed out when the first of them ends, and twice when both have.  So a
+ * sequence that shares pages is not ended here while another holds them: the caller makes its lens negative (with new_lens
+ * 0), puts those of its pages that nobody else holds on the stack, and leaves the shared ones to the last owner, which may
+ * be ended here.  Sequences that share may grow here if they share whole, full pages.
  *   start_pos [batch]   lens where granted, -1 elsewhere: for nmi_kv_append_paged
  *   kv_lens [batch]     lens + new_lens where granted, 0 elsewhere: for the decode attention
  *   lens_out [batch]    lens + new_lens where granted, -1 where ended, lens elsewhere: lens of the next step (may be

@@ -5,7 +5,8 @@
 // its positions'; then those that grow pop theirs in the same order: with need_b pages for sequence b, page j of b is
 // the stack's entry count - 1 - (sum of need_i, i < b) - j.  A sequence is granted all of its new tokens or none: none
 // where its row of the table is too short, or where it needs pages and the needs up to its own are more than the
-// stack holds.  So everything follows from prefix sums, and equal inputs give equal tables.
+// stack holds.  So everything follows from prefix sums, and equal inputs give equal tables.  No page has two owners: there
+// are no counts of them, so what several sequences share must not come back here before its last owner ends.
 //
 // Bound: latency; a step of a batch moves some kilobytes.  One workgroup, since the stack is one: up to 1024 sequences
 // at a time in its threads (256 of them for a decode step of as many: 4.1 us where 1024 threads took 4.9), sums over them

@@ -769,7 +769,9 @@ def kv_assign_paged(lens: torch.Tensor, new_lens: torch.Tensor | None, page_tabl
     ended and gives its pages back; None: one each), page_table int32 [batch, max_pages] written where pages are
     added, free_pages int32 [n_pages] a stack of which the first free_count[0] (int32) are free.  tokens: the rows
     of packed new tokens; None where every sequence has one row.  A sequence whose tokens do not all fit its row of
-    the table or the pages left is granted none (start_pos -1).  lens_out and free_count_out may be lens and
+    the table or the pages left is granted none (start_pos -1).  A page in use or on the stack has one owner: a sequence that
+    shares pages with another in use must not be ended here (make its lens negative and free its own pages by hand; the
+    last owner may be).  lens_out and free_count_out may be lens and
     free_count themselves, so that a captured step goes on from where it ended."""
     dev = lens.get_device()
     stream = _stream_on(dev)

@@ -126,3 +126,36 @@ def test_pages_past_the_stack_are_neither_pushed_nor_read(batch, width, page):
     assert _lib.lib().nmi_async_status() == _lib.NMI_ERR_ASYNC and _lib.lib().nmi_async_status() == 0
     assert got.free_count.tolist() == [n_pages] and free.tolist() == list(range(n_pages))
     assert (got.lens == -1).all() and (got.start_pos == -1).all() and (table[:, 30:] == -9).all()
+
+
+def test_a_shared_prefix_outlives_the_sequence_that_ends_first():
+    """Two sequences share the full pages of a prefix and grow here; the first is ended by hand (its own pages on the stack,
+    its length negative), the last one here.  At each step every page is free, or held by those that share it."""
+    announce("assign_shared")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    page, shared = 16, [7, 3]
+    table, lens = ints([[7, 3, 1, -1, -1], [7, 3, -1, -1, -1], [-1] * 5]), ints([40, 32, -1])
+    free, count = ints([0, 2, 4, 5, 6, -1, -1, -1]), ints([5])
+
+    def step(*new):
+        got = ops.kv_assign_paged(lens, ints(list(new)), table, free, count, page, tokens=sum(max(0, n) for n in new),
+                                  lens_out=lens, free_count_out=count)
+        torch.cuda.synchronize()
+        assert _lib.lib().nmi_async_status() == 0
+        rows = [table[b, :-(-max(0, int(n)) // page)].tolist() for b, n in enumerate(lens)]
+        held = {i for r in rows for i in r}
+        own = [i for r in rows for i in r if i not in shared]
+        assert len(own) == len(set(own)) and sorted([*held, *free[:int(count)].tolist()]) == list(range(8))
+        return got, rows
+
+    got, rows = step(10, 5, 0)
+    assert got.lens.tolist() == [50, 37, -1] and rows == [[7, 3, 1, 6], [7, 3, 5], []]
+    c, own = int(count), table[0, 2:4]
+    free[c:c + own.numel()] = own
+    count += own.numel()
+    lens[0] = -1
+    lens[2] = 0
+    got, rows = step(0, 13, 33)
+    assert got.start_pos.tolist() == [-1, 37, 0] and rows == [[], [7, 3, 5, 6], [1, 4, 2]]
+    got, rows = step(0, -1, 1)
+    assert rows == [[], [], [1, 4, 2]] and free[:int(count)].tolist() == [0, 7, 3, 5, 6]
