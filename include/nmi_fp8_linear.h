@@ -393,7 +393,7 @@ int nmi_attn_forward_fp8(const void* input_bf16, const float* norm_w, const void
  * of either, so [n_pages, n_kv_heads, page_size, 128] and [n_pages, page_size, n_kv_heads, 128] are
  * both possible, as are slices of a pool that several layers share.  page_size is a power of two from
  * 16 to 2^20; page_table has max_pages entries per sequence, of which only those that a sequence's
- * length reaches are read; max_pages * page_size <= 2^30.  Pages and strides are multiples of 16
+ * length reaches are used (and, but for the choice of pages of nmi_sdpa_decode_paged_sparse, read); max_pages * page_size <= 2^30.  Pages and strides are multiples of 16
  * bytes, strides at least 128 elements, token_stride at most 2^24.  The struct is read during the call only.
  *
  * Page tables, lengths, positions and offsets are device data (so that a captured graph can be replayed
@@ -498,7 +498,7 @@ int nmi_kv_assign_paged(const int32_t* lens, const int32_t* new_lens, int32_t* p
  *   k_bounds[page][head][0][d] = min over the page's positions of k[d],  k_bounds[page][head][1][d] = max,
  * bf16 [n_pages, n_kv_heads, 2, 128], 16-byte aligned, of the keys that the cache holds (code * scale in float32)
  * rounded to nearest even; NaN in both where one of the keys has NaN.  Other pages' bounds stay.  The cache's v_pages
- * and v_scale are not read.  One launch, no workspace.
+ * and v_scale are not read, but checked as elsewhere: k's may stand for them.  One launch, no workspace.
  */
 int nmi_kv_bounds_paged(const nmi_paged_kv* cache, void* k_bounds_bf16, const int32_t* cu_seqlens, const int32_t* start_pos,
                         int batch, int tokens, void* stream);
@@ -535,14 +535,15 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
  * lo and hi page p's k_bounds (nmi_kv_bounds_paged): no key of the page has a larger product with one of them, as far as
  * the bounds are exact.  They are of a bf16 cache and of codes under scales that are powers of two from 2^-124 to 2^119
  * (bf16 holds those keys); under others a bound's rounding to bf16 may leave it short of the key by 2^-8 of its value.
- * Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds are not
- * read.  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places in the sequence of the pages
+ * Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds do not
+ * count.  (Table entries past a sequence's pages, within its row, and the bounds of the pages that they name may be read
+ * ahead; whatever they hold changes nothing.)  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places in the sequence of the pages
  * attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type; scale does not change the
  * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first (with
  * n_select 1 none is scored).
  * workspace: nmi_sdpa_decode_paged_sparse_workspace_bytes(batch, n_heads, n_kv_heads, max_pages, n_select) bytes,
  * 16-byte aligned, no initialisation; NULL takes it from the bump allocator.  Four launches; three where n_select pages
- * hold as few positions as above; the decode's alone where n_select >= max_pages.
+ * hold as few positions as above; where n_select >= max_pages the decode's alone, and one before it if selected is given.
  */
 size_t nmi_sdpa_decode_paged_sparse_workspace_bytes(int batch, int n_heads, int n_kv_heads, int max_pages, int n_select);
 int nmi_sdpa_decode_paged_sparse(const nmi_paged_kv* cache, const void* q_bf16, int64_t ldq, void* o_bf16, int64_t ldo,

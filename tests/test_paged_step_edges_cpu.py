@@ -7,8 +7,9 @@ import numpy as np
 import pytest
 import torch
 
-from nemotron_infer_amd import build, ops
+from nemotron_infer_amd import _lib, build, ops
 from oracle import block, e4m3, paged
+from tests.test_host_runtime_cpu import host  # noqa: F401  (a fixture)
 
 SHIM = """
 #include "nmi_paged.hpp"
@@ -86,3 +87,29 @@ def test_bounds_as_they_are_stored_bound_the_keys():
             slack = 2.0 ** -8 * (np.abs(true[:, g, 1]) * up - np.abs(true[:, g, 0]) * down).sum(-1)
             assert ((keys[:, g] @ q[g]).max(-1) <= score + slack + 1e-9 * np.abs(score)).all()
     assert short > 100                                   # (they do lie inside: the bound is no bound there)
+
+
+def test_keys_may_stand_for_values_in_the_bounds_and_not_be_left_out(host):  # noqa: F811
+    """The values are not read, and checked as elsewhere."""
+    got = host("""
+W, ST = 1 << 38, 1 << 12
+result = []
+for v, vs in ((W, W), (None, W), (W, None)):
+    c = _lib.PagedKv(W, v, 8 * 16 * 128, 16 * 128, 128, W, 64, W, vs, 2, 100, 16, 64, 8)
+    result.append([L.nmi_kv_bounds_paged(ctypes.addressof(c), W, None, W, 3, 3, ST), len(launches())])
+""")
+    assert got == [[0, 1], [_lib.NMI_ERR_INVALID_ARG, 0], [_lib.NMI_ERR_INVALID_ARG, 0]]
+
+
+def test_the_places_alone_cost_a_launch_where_all_pages_are_attended(host):  # noqa: F811
+    got = host("""
+W, ST = 1 << 38, 1 << 12
+result = []
+for selected in (None, W):
+    c = _lib.PagedKv(W, W, 8 * 64 * 128, 64 * 128, 128, W, 64, W, W, 2, 100, 64, 64, 8)
+    need = L.nmi_sdpa_decode_paged_sparse_workspace_bytes(2, 40, 8, 64, 64)
+    rc = L.nmi_sdpa_decode_paged_sparse(ctypes.addressof(c), W, 5120, W, 5120, W, W, 64, selected, 2, 40, 0.1, W, need, ST)
+    result.append([rc, [l[0] for l in launches()]])
+""")
+    (rc, decode), (rc_selected, with_places) = got
+    assert rc == rc_selected == 0 and with_places[1:] == decode and "page_select" in with_places[0]

@@ -159,3 +159,27 @@ def test_a_shared_prefix_outlives_the_sequence_that_ends_first():
     assert got.start_pos.tolist() == [-1, 37, 0] and rows == [[], [7, 3, 5, 6], [1, 4, 2]]
     got, rows = step(0, -1, 1)
     assert rows == [[], [], [1, 4, 2]] and free[:int(count)].tolist() == [0, 7, 3, 5, 6]
+
+
+@pytest.mark.parametrize("batch", [1, 3])
+def test_entries_past_a_sequences_pages_change_nothing(batch):
+    """A table far wider than the sequences, its unused entries naming pages that others hold, whose bounds would be chosen
+    first, or no pages: the same bytes as with a table just wide enough."""
+    announce("sparse_wide", batch)
+    rng = np.random.default_rng(batch)
+    lens = [1000, 333, 530][:batch]
+    pool = Pool(rng, lens, 2, 16, "bf16", extra=40)
+    q = _rand_bits(rng, batch, 8 * 128)
+    x = np.sort(rng.standard_normal((pool.k.shape[0], 2, 2, 128)), axis=2)
+    idle = np.setdiff1d(np.arange(len(x)), pool.table)
+    x[idle[::2]], x[idle[1::2]] = np.nan, np.inf
+    bounds = block.bf16_round_exact(x)
+    o, places = _selected(pool, q, bounds, 7)
+    wide = np.full((batch, 4000), 2 ** 31 - 1, np.int32)
+    wide[:, :1500] = rng.choice(idle, (batch, 1500))
+    for b, n in enumerate(lens):
+        used = -(-n // 16)
+        wide[b, :used] = pool.table[b, :used]
+    pool.dtable = _dev(wide)
+    again, places_again = _selected(pool, q, bounds, 7)
+    assert np.array_equal(places, places_again) and np.array_equal(bits(o), bits(again))
