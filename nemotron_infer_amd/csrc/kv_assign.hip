@@ -9,10 +9,10 @@
 // are no counts of them, so what several sequences share must not come back here before its last owner ends.
 //
 // Bound: latency; a step of a batch moves some kilobytes.  One workgroup, since the stack is one: up to 1024 sequences
-// at a time in its threads (256 of them for a decode step of as many: 4.1 us where 1024 threads took 4.9), sums over them
+// at a time in its threads (256 of them for a decode step of as many: 4.0 us where 1024 threads took 4.9), sums over them
 // by DPP and LDS; what varies in length (pages pushed and popped, slots) is dealt to the threads one by one, each finding
 // its sequence by a binary search over the sums in LDS.  Measured (graph replays): a step of 1 / 32 / 256 / 1024 sequences
-// 2.8 / 3.3 / 4.1 / 6.9 us, of 4000 23.
+// 2.8 / 3.3 / 4.0 / 6.9 us, of 4000 23.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 #include "nmi_packed.hpp"

@@ -19,7 +19,7 @@
 // lanes take a page, 8 dims each, the queries' positive and negative parts in their registers; a wave takes 4 pages at a
 // time, all of the chunk's query heads at once so that their sums hide one another's latency, and asks for the next pages'
 // bounds as those at hand are used: their upper ones first, so that both need not be held at once (4 heads: 166
-// registers, 3 waves to a SIMD, where 178 leave 2: 8 sequences of 60000 33.0 us for the whole call, so 30.6).  (One head after
+// registers, 3 waves to a SIMD, where 178 leave 2: 8 sequences of 60000 33.0 us for the whole call, so 31.2).  (One head after
 // another, in an earlier form, 40 sequences of 4000: 39.0 where that took 36.7; 16 pages a wave, 4 lanes each, the queries
 // in LDS: 36.8, but one sequence of 60000 18.6 where that took 17.0.)
 // A sequence's KV head is dealt to as many workgroups as all of them leave it of 6 per CU, or 2 where there is but one
@@ -30,8 +30,8 @@
 // earlier form: 20 documents 43.4 where that took 43.1, and one sequence 21.0 where that took 20.6.)
 // Choice: one workgroup for a sequence's KV head: the range of the scores cut into 1024 bins, counted in LDS, the bin
 // with the last one wanted cut again while it has many, its few ranked one against another; then one pass in order.
-// Bound: latency, a handful of barriers: 4.6 us (traced) of 1562 pages, where four passes of 8 bits and a scan for each
-// 256 pages took 12.4.
+// Bound: latency, a handful of barriers: 5.6 us (traced) of 1562 pages; four passes of 8 bits and a scan for each 256 pages,
+// an earlier form, took 12.4.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
 #include "nmi_packed.hpp"
