@@ -393,8 +393,9 @@ int nmi_attn_forward_fp8(const void* input_bf16, const float* norm_w, const void
  * of either, so [n_pages, n_kv_heads, page_size, 128] and [n_pages, page_size, n_kv_heads, 128] are
  * both possible, as are slices of a pool that several layers share.  page_size is a power of two from
  * 16 to 2^20; page_table has max_pages entries per sequence, of which only those that a sequence's
- * length reaches are used (and, but for the choice of pages of nmi_sdpa_decode_paged_sparse, read); max_pages * page_size <= 2^30.  Pages and strides are multiples of 16
- * bytes, strides at least 128 elements, token_stride at most 2^24.  The struct is read during the call only.
+ * length reaches are used (and, but by nmi_sdpa_decode_paged_sparse, read); max_pages * page_size <= 2^30.
+ * Pages and strides are multiples of 16 bytes, strides at least 128 elements, token_stride at most 2^24.  The
+ * struct is read during the call only.
  *
  * Page tables, lengths, positions and offsets are device data (so that a captured graph can be replayed
  * as the sequences grow) and are not seen by the host.  The kernels never follow one that is out of
@@ -537,9 +538,9 @@ int nmi_sdpa_decode_paged(const nmi_paged_kv* cache, const void* q_bf16, int64_t
  * (bf16 holds those keys); under others a bound's rounding to bf16 may leave it short of the key by 2^-8 of its value.
  * Sums in 64 bits, rounded once; ties go to the earlier page; NaN comes first.  The newest page's bounds do not
  * count.  (Table entries past a sequence's pages, within its row, and the bounds of the pages that they name may be read
- * ahead; whatever they hold changes nothing.)  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places in the sequence of the pages
- * attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type; scale does not change the
- * choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first (with
+ * ahead; whatever they hold changes nothing.)  selected (int32 [batch, n_kv_heads, n_select], or NULL) receives the places
+ * in the sequence of the pages attended, ascending, then -1.  Everything else is nmi_sdpa_decode_paged's (any kv_type;
+ * scale does not change the choice).  Pages that are not selected are not read, but a page id out of range that is scored is selected first (with
  * n_select 1 none is scored).
  * workspace: nmi_sdpa_decode_paged_sparse_workspace_bytes(batch, n_heads, n_kv_heads, max_pages, n_select) bytes,
  * 16-byte aligned, no initialisation; NULL takes it from the bump allocator.  Four launches; three where n_select pages

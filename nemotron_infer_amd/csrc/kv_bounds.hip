@@ -4,8 +4,8 @@
 //
 // of the keys that the page stands for (codes times their scales in float32), rounded to the nearest bf16, for every page
 // that the call's new positions complete; a dim with a NaN has NaN for both.  bf16 keys, and codes (4 significant bits)
-// under powers of two, lose nothing by it; under other scales a bound may lie 2^-8 of its value inside the keys.  The newest page of a sequence
-// needs none: it is attended whatever its score.
+// under powers of two, lose nothing by it; under other scales a bound may lie 2^-8 of its value inside the keys.  The
+// newest page of a sequence needs none: it is attended whatever its score.
 //
 // Bound: latency (offsets, page id, keys one after another), then reading the pages, once.  A wave's load is one row of
 // bf16, or two of e4m3 codes (4 bytes a lane), so that a lane keeps its dims and, where the waves of a workgroup share a

@@ -22,15 +22,15 @@
 // registers, 3 waves to a SIMD, where 178 leave 2: 8 sequences of 60000 33.0 us for the whole call, so 31.2).  (One head after
 // another, in an earlier form, 40 sequences of 4000: 39.0 where that took 36.7; 16 pages a wave, 4 lanes each, the queries
 // in LDS: 36.8, but one sequence of 60000 18.6 where that took 17.0.)
-// A sequence's KV head is dealt to as many workgroups as all of them leave it of 6 per CU, or 2 where there is but one
-// sequence, whose workgroups all have as much to do: 2 / 3 / 4 / 6 / 8 / 12 per CU, 40 / 8 heads, the whole call, one sequence
-// of 100001 positions 18.5 / 19.4 / 19.6 / 19.5 / 19.7 / 19.7 us, 40 of 4000 39.1 / 38.2 / 38.6 / 38.8 / 41.2 / 42.1, 20
-// documents of 900 to 30000 46.7 / 40.0 / 39.2 / 39.8 / 39.9 / 41.4; 16 / 16 heads 17.6 / 17.6 / 17.8 / 18.0 / 18.0 / 18.0,
-// 52.5 / 52.8 / 52.7 / 52.4 / 53.0 / 52.7 and 70.3 / 57.3 / 54.6 / 52.4 / 51.2 / 50.8.  (The pages of all sequences in equal shares, an
+// A sequence's KV head is dealt to as many workgroups as all of them leave it of 2 per CU, which are at work at once; to 8,
+// as far as 6 per CU allow, where that is fewer, since the longest of many sequences would then take long by itself.
+// 2 / 3 / 4 / 6 / 8 / 12 per CU, the whole call, 40 / 8 heads: one sequence of 100001 positions 18.5 / 19.4 / 19.6 / 19.5 / 19.7 /
+// 19.7 us, 8 of 40000 26.5 / 27.6 / 27.9 / 29.5 / 31.6 / 31.1, 40 of 4000 39.1 / 38.2 / 38.6 / 38.8 / 41.2 / 42.1, 20 documents of 900
+// to 30000 46.7 / 40.0 / 39.2 / 39.8 / 39.9 / 41.4; so 18.5, 26.6, 39.0 and 39.6.  (The pages of all sequences in equal shares, an
 // earlier form: 20 documents 43.4 where that took 43.1, and one sequence 21.0 where that took 20.6.)
 // Choice: one workgroup for a sequence's KV head: the range of the scores cut into 1024 bins, counted in LDS, the bin
 // with the last one wanted cut again while it has many, its few ranked one against another; then one pass in order.
-// Bound: latency, a handful of barriers: 5.6 us (traced) of 1562 pages; four passes of 8 bits and a scan for each 256 pages,
+// Bound: latency, a handful of barriers: 5.6 to 6.0 us (traced) of 1562 pages; four passes of 8 bits and a scan for each 256 pages,
 // an earlier form, took 12.4.
 #include "nmi_device.hpp"
 #include "nmi_launch.hpp"
@@ -44,7 +44,7 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kHeads = 5;               // query heads at a time at most: 32 registers each
-constexpr int kPerCu = 6, kPerCuOne = 2;    // scores' workgroups per CU; of one sequence
+constexpr int kPerCu = 2, kPerCuMost = 6, kPerHead = 8;     // scores' workgroups
 constexpr int kBinBits = 10, kSelectThreads = 1 << kBinBits, kSelectWaves = kSelectThreads / 64;
 constexpr int kKeys = 6144;             // keys and page ids of a sequence kept in LDS
 constexpr int kFew = 64;                // keys ranked by a wave
@@ -290,10 +290,10 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(const Selec
 hipError_t launch_page_select(const SelectArgs& a, hipStream_t stream) {
     const int64_t groups = (int64_t)a.batch * a.kv.n_kv;
     if (a.select < a.kv.max_pages) {
-        // as many workgroups as keep the CUs busy, or one for each 16 pages that a sequence may have
-        const int per_cu = a.batch == 1 ? kPerCuOne : kPerCu;
-        const int64_t most = ((int64_t)a.kv.max_pages + 15) / 16, parts = std::max<int64_t>(1, per_cu * device_info().num_cu / groups);
-        const int p = (int)std::min(most, parts);
+        // (no more than one for each 16 pages that a sequence may have)
+        auto per_head = [&](int per_cu) { return std::max<int64_t>(1, per_cu * device_info().num_cu / groups); };
+        const int64_t most = ((int64_t)a.kv.max_pages + 15) / 16;
+        const int p = (int)std::min(most, std::max(per_head(kPerCu), std::min<int64_t>(per_head(kPerCuMost), kPerHead)));
         const int chunks = (a.group + kHeads - 1) / kHeads;
         const dim3 grid((uint32_t)(groups * p)), block(kThreads);
         switch ((a.group + chunks - 1) / chunks) {

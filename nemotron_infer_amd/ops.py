@@ -721,8 +721,9 @@ def sdpa_decode_paged_sparse(q: torch.Tensor, k_pages: torch.Tensor, v_pages: to
                              selected: torch.Tensor | None = None) -> torch.Tensor:
     """sdpa_decode_paged over n_select pages of each sequence (nmi_sdpa_decode_paged_sparse), chosen for each
     token and KV head: the newest page, and those whose k_bounds (kv_bounds_paged) allow the largest products
-    with one of the KV head's queries (up to 2^-8 of a bound under scales that are no powers of two); all pages where there are no more.  selected (int32 [batch,
-    n_kv_heads, n_select]) receives their places in the sequence, ascending, then -1.  Returns o."""
+    with one of the KV head's queries (up to 2^-8 of a bound under scales that are no powers of two); all pages
+    where there are no more.  selected (int32 [batch, n_kv_heads, n_select]) receives their places in the
+    sequence, ascending, then -1.  Returns o."""
     dev = q.get_device()
     stream = _stream_on(dev)
     if stream is None:
